@@ -52,7 +52,9 @@ extern "C" {
 /* 6: the seeded KeyFormer noise (noise == NULL) comes from seven generator rounds instead of ten: same
  * signatures, a different noise stream for a given seed.
  * 7: tri_diag_issue_probe added; nothing else changed.
- * 8: tri_diag_power_probe added; nothing else changed. */
+ * 8: tri_diag_power_probe added; nothing else changed.
+ * (The tri_cache_* entry points came later: nothing that was there changed for them, and a caller finds them by their
+ * symbols.) */
 #define TRI_ABI_VERSION 8
 
 typedef enum tri_dtype {
@@ -60,7 +62,8 @@ typedef enum tri_dtype {
   TRI_BF16 = 1,
   TRI_F32 = 2,
   TRI_U8 = 3,
-  TRI_FP8_E4M3 = 4 /* OCP e4m3 (no infinities, +-448 largest): KV caches only */
+  TRI_FP8_E4M3 = 4, /* OCP e4m3 (no infinities, +-448 largest): KV caches only */
+  TRI_I32 = 5       /* lengths of sequences (tri_cache_*) */
 } tri_dtype;
 
 typedef enum tri_status {
@@ -269,6 +272,80 @@ int tri_validate_roco(const tri_tensor* x, const tri_tensor* norm_w, const tri_t
                       const tri_tensor* wv, const tri_tensor* k_cache, const tri_tensor* v_cache,
                       const tri_tensor* scratch, const tri_tensor* out, const tri_tensor* sum_out,
                       const tri_tensor* sumsq_out, int32_t as_mean_var, const tri_attn_params* p);
+
+/* ------------------------------------------------------------------ caches of several sequences
+ * The tri_cache_* entry points keep and read the keys and values of `batch` sequences of different lengths, 16-bit or
+ * in 4 bits, and attend to them, also in a sliding window behind a few first tokens that stay visible.  No counterpart
+ * in the reference, whose caches hold one sequence in fp16 without a window (baseline/ref_rms.py:28-82).
+ *
+ * Sequence b has n = lens[b] keys, in rows [0, n) of its part of the cache, those of the call's `seq` tokens among them:
+ * token i stands at position n - seq + i.  A negative position is padding - the first tokens of a sequence with fewer than
+ * seq; a sequence of length 0 is nothing else.  Padding is not written to the cache, and reads and attends to nothing.
+ * Lengths live on the device, so that a captured graph can be replayed as they grow; a value outside [0, kv_len] counts
+ * as the nearer end.
+ *
+ * Tensors:
+ *   16-bit caches  [batch, n_kv_heads, rows >= kv_len, D] (or without the first dimension where batch is 1), of the call's
+ *                  element type; scales NULL.  Any strides that are multiples of 8, the innermost 1 (a [batch, rows,
+ *                  heads, D] cache is passed as its transposed view).
+ *   4-bit caches   TRI_U8 [batch, n_kv_heads, rows, D / 2], strides multiples of 16, with scales TRI_U8 [batch, n_kv_heads,
+ *                  rows, D / 32], strides multiples of D / 32.  The OCP microscaling format: 32 consecutive channels share
+ *                  a power of two 2^e, stored as the byte e + 127 (255: the block is NaN; bytes 1 to 254 are read as they
+ *                  are), and each is sign and magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 to 7, 8 more for the sign)
+ *                  times 2^e, two codes a byte, the even channel in the low half.  4.25 bits a value.  The element type
+ *                  of the call that reads a cache has to hold its values (fp16: blocks written from bf16 values beyond
+ *                  65504 read as infinities).
+ *   lens           TRI_I32 [batch], or NULL: every sequence has kv_len keys.
+ * The rows a call reads are those of keys that some token of it sees; no others need hold numbers.  Within a call a NaN or
+ * infinity among the values of a key reaches the tokens that see it and may reach others of the same call. */
+typedef struct tri_cache_params {
+  int32_t batch;
+  int32_t n_q_heads;  /* (tri_cache_attention only) */
+  int32_t n_kv_heads;
+  int32_t head_dim;   /* 64 or 128 */
+  int32_t seq;        /* tokens per sequence of this call; tri_cache_read: rows to read per sequence */
+  int32_t kv_len;     /* keys of the longest sequence the call may meet, at most the rows of the caches */
+  /* the rest: tri_cache_attention only */
+  float scale;        /* multiplies q.k before the softmax; must be > 0 */
+  int32_t causal;     /* a token at position t sees keys j <= t; otherwise all keys of its sequence */
+  int32_t window;     /* > 0 (causal only): ... of those, keys j > t - window */
+  int32_t sinks;      /* ... and keys j < sinks */
+} tri_cache_params;
+
+/* Writes k and v [batch * seq, n_kv_heads * D] (token i of sequence b in row b * seq + i) to rows n - seq + i of the
+ * caches: copied, or in 4 bits.  e is the least exponent >= -110 with max |x| < 7 * 2^e over the block, x / 2^e goes to the
+ * nearest magnitude, ties to the even code; a block that holds an infinity or NaN gets the byte 255.  The rows of
+ * positions that a cache does not have, and all others, stay as they are. */
+int tri_cache_append(const tri_tensor* k, const tri_tensor* v, tri_tensor* k_cache, tri_tensor* k_scales /* nullable */,
+                     tri_tensor* v_cache, tri_tensor* v_scales /* nullable */, const tri_tensor* lens /* nullable */,
+                     const tri_cache_params* p, void* hip_stream);
+int tri_validate_cache_append(const tri_tensor* k, const tri_tensor* v, const tri_tensor* k_cache,
+                              const tri_tensor* k_scales, const tri_tensor* v_cache, const tri_tensor* v_scales,
+                              const tri_tensor* lens, const tri_cache_params* p);
+
+/* Reads the last seq rows of every sequence back: k and v [batch, n_kv_heads, seq, D], 16-bit (either type from 4-bit
+ * caches), strides as for caches; row i is position n - seq + i, zeros where that is padding. */
+int tri_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scales /* nullable */, const tri_tensor* v_cache,
+                   const tri_tensor* v_scales /* nullable */, const tri_tensor* lens /* nullable */, tri_tensor* k,
+                   tri_tensor* v, const tri_cache_params* p, void* hip_stream);
+int tri_validate_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scales, const tri_tensor* v_cache,
+                            const tri_tensor* v_scales, const tri_tensor* lens, const tri_tensor* k, const tri_tensor* v,
+                            const tri_cache_params* p);
+
+/* out = softmax(scale * q.K^T over the keys that each token sees).V, from caches that hold the call's tokens already.
+ *   q, out [batch * seq, n_q_heads * D]; lse fp32 [batch, n_q_heads, seq] contiguous or NULL: the natural log-sum-exp.
+ * A row without a visible key (padding) gets zeros, and -inf as its lse.  scratch: 1-D TRI_U8, 256-byte aligned, or NULL;
+ * with tri_cache_scratch_bytes the call runs its fastest plan, with less (or none) it cuts the key axis into
+ * fewer parts - same results to rounding.  The size does not depend on the lengths below kv_len. */
+int64_t tri_cache_scratch_bytes(const tri_cache_params* p, int32_t four_bit);
+int tri_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales /* nullable */,
+                        const tri_tensor* v_cache, const tri_tensor* v_scales /* nullable */,
+                        const tri_tensor* lens /* nullable */, tri_tensor* scratch /* nullable */,
+                        tri_tensor* lse /* nullable */, tri_tensor* out, const tri_cache_params* p, void* hip_stream);
+int tri_validate_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales,
+                                 const tri_tensor* v_cache, const tri_tensor* v_scales, const tri_tensor* lens,
+                                 const tri_tensor* scratch, const tri_tensor* lse, const tri_tensor* out,
+                                 const tri_cache_params* p);
 
 /* Issue probe (measurement only; no counterpart in the reference).  Launches `workgroups` workgroups of
  * 4 * waves_per_simd waves, one workgroup per CU, every wave looping `iters` times (a multiple of 8) over a group

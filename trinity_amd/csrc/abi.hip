@@ -60,6 +60,7 @@ using tri::few_attn_workspace_bytes;
 using tri::split_attn_workspace_bytes;
 using tri::gemm_workspace_bytes;
 using tri::qkv_workspace_bytes;
+using tri::cache_attn_workspace_bytes;
 
 namespace {
 
@@ -343,6 +344,79 @@ int check_noise(const tri_tensor* t, int64_t Hq, int64_t S, int64_t L, int dtype
   return TRI_OK;
 }
 
+// ---- caches of several sequences
+constexpr int64_t kInt32End = (int64_t)1 << 31;
+
+int check_cache_params(const tri_cache_params* p, bool attention) {
+  if (p == nullptr) return TRI_ERR_NULL;
+  if (p->head_dim != 64 && p->head_dim != 128) return TRI_ERR_UNSUPPORTED;
+  if (p->batch < 0 || p->seq < 0 || p->kv_len < 0 || p->n_kv_heads <= 0) return TRI_ERR_SHAPE;
+  // (threads and workgroups are counted in 32 bits, with room for the largest tile)
+  if ((int64_t)p->batch * p->seq >= kInt32End || (int64_t)p->batch * p->seq * p->n_kv_heads * (p->head_dim / 8) >= kInt32End - 4096)
+    return TRI_ERR_UNSUPPORTED;
+  if (p->kv_len >= (1 << 30) || p->seq >= (1 << 30)) return TRI_ERR_UNSUPPORTED;
+  if (!attention) return TRI_OK;
+  if (p->n_q_heads <= 0 || p->n_q_heads % p->n_kv_heads != 0) return TRI_ERR_SHAPE;
+  if ((int64_t)p->batch * p->seq * p->n_q_heads * (p->head_dim / 8) >= kInt32End - 4096) return TRI_ERR_UNSUPPORTED;
+  if (!(p->scale > 0.f) || !(p->scale < INFINITY)) return TRI_ERR_UNSUPPORTED;
+  if (p->window < 0 || p->sinks < 0) return TRI_ERR_SHAPE;
+  if (p->window > 0 && !p->causal) return TRI_ERR_UNSUPPORTED;
+  return TRI_OK;
+}
+
+// [B, H, >= rows, n] (or [H, rows, n] where B is 1) with contiguous rows; `unit`: what its strides are multiples of.  `write`:
+// rows must not share memory (their order is free, and a stride larger than another's extent is not asked for: a
+// transposed view interleaves heads and rows).
+int check_cache4(const tri_tensor* t, int64_t B, int64_t H, int64_t rows, bool exact_rows, int64_t n, int64_t unit, int align,
+                 int dtype, bool write) {
+  if (t == nullptr) return TRI_ERR_NULL;
+  if (t->dtype != dtype) return TRI_ERR_DTYPE;
+  if (t->ndim != 4 && !(t->ndim == 3 && B == 1)) return TRI_ERR_SHAPE;
+  const int64_t* sh = t->shape + (t->ndim - 3);
+  const int64_t* st = t->stride + (t->ndim - 3);
+  if ((t->ndim == 4 && t->shape[0] != B) || sh[0] != H || sh[2] != n) return TRI_ERR_SHAPE;
+  if (exact_rows ? sh[1] != rows : sh[1] < rows) return TRI_ERR_SHAPE;
+  if (sh[1] >= kInt32End) return TRI_ERR_UNSUPPORTED;
+  if (B == 0 || sh[1] == 0) return TRI_OK;  // no elements: no storage
+  if (t->ptr == nullptr) return TRI_ERR_NULL;
+  if (st[2] != 1) return TRI_ERR_STRIDE;
+  const int64_t sb = t->ndim == 4 ? t->stride[0] : 0;
+  if ((B > 1 && sb % unit != 0) || (H > 1 && st[0] % unit != 0) || (sh[1] > 1 && st[1] % unit != 0)) return TRI_ERR_STRIDE;
+  if ((B > 1 && sb < 0) || (H > 1 && st[0] < 0) || (sh[1] > 1 && st[1] < 0)) return TRI_ERR_STRIDE;
+  if (write && ((B > 1 && sb < n) || (H > 1 && st[0] < n) || (sh[1] > 1 && st[1] < n))) return TRI_ERR_STRIDE;
+  if (((uintptr_t)t->ptr & (uintptr_t)(align - 1)) != 0) return TRI_ERR_ALIGN;
+  return TRI_OK;
+}
+
+// one cache with its scales (NULL: 16-bit elements of type dt, -1: of either 16-bit type)
+int check_cache_pair(const tri_tensor* c, const tri_tensor* x, const tri_cache_params* p, int dt, bool write) {
+  if (c == nullptr) return TRI_ERR_NULL;
+  if (x == nullptr) return check_cache4(c, p->batch, p->n_kv_heads, p->kv_len, false, p->head_dim, 8, 16, dt, write);
+  const int xa = p->head_dim / 32;
+  TRI_TRY(check_cache4(c, p->batch, p->n_kv_heads, p->kv_len, false, p->head_dim / 2, 16, 16, TRI_U8, write));
+  TRI_TRY(check_cache4(x, p->batch, p->n_kv_heads, p->kv_len, false, xa, xa, xa, TRI_U8, write));
+  if (x->shape[x->ndim - 2] != c->shape[c->ndim - 2]) return TRI_ERR_SHAPE;
+  return TRI_OK;
+}
+
+int check_caches(const tri_tensor* kc, const tri_tensor* kx, const tri_tensor* vc, const tri_tensor* vx, const tri_tensor* lens,
+                 const tri_cache_params* p, int dt, bool write) {
+  if ((kx == nullptr) != (vx == nullptr)) return TRI_ERR_NULL;  // one format
+  TRI_TRY(check_cache_pair(kc, kx, p, dt, write));
+  TRI_TRY(check_cache_pair(vc, vx, p, dt, write));
+  if (kc->shape[kc->ndim - 2] != vc->shape[vc->ndim - 2]) return TRI_ERR_SHAPE;
+  if (lens != nullptr) {
+    if (lens->dtype != TRI_I32) return TRI_ERR_DTYPE;
+    if (lens->ndim != 1 || lens->shape[0] != p->batch) return TRI_ERR_SHAPE;
+    if (p->batch > 0 && lens->ptr == nullptr) return TRI_ERR_NULL;
+    if (p->batch > 1 && lens->stride[0] != 1) return TRI_ERR_STRIDE;
+    if (((uintptr_t)lens->ptr & 3u) != 0) return TRI_ERR_ALIGN;
+  }
+  return TRI_OK;
+}
+
+inline bool cache_is_empty(const tri_cache_params* p) { return p->batch == 0 || p->seq == 0; }
+
 }  // namespace
 
 // The launch sequences exist once per element type: the same text, compiled against the fp16 kernels
@@ -583,6 +657,83 @@ int tri_roco(const tri_tensor* x, const tri_tensor* norm_w, const tri_tensor* wq
              void* hip_stream) {
   TRI_TRY(tri_validate_roco(x, norm_w, wq, wk, wv, k_cache, v_cache, scratch, out, sum_out, sumsq_out, as_mean_var, p));
   return TRI_DISPATCH(x, impl_roco(x, norm_w, wq, wk, wv, k_cache, v_cache, scratch, out, sum_out, sumsq_out, as_mean_var, p, hip_stream));
+}
+
+// ---------------------------------------------------------------- caches of several sequences
+int tri_validate_cache_append(const tri_tensor* k, const tri_tensor* v, const tri_tensor* k_cache,
+                              const tri_tensor* k_scales, const tri_tensor* v_cache, const tri_tensor* v_scales,
+                              const tri_tensor* lens, const tri_cache_params* p) {
+  TRI_TRY(check_cache_params(p, false));
+  const int dt = elem_dtype(k);
+  const int64_t rows = (int64_t)p->batch * p->seq, cols = (int64_t)p->n_kv_heads * p->head_dim;
+  TRI_TRY(check_mat(k, rows, cols, dt));
+  TRI_TRY(check_mat(v, rows, cols, dt));
+  return check_caches(k_cache, k_scales, v_cache, v_scales, lens, p, dt, true);
+}
+
+int tri_cache_append(const tri_tensor* k, const tri_tensor* v, tri_tensor* k_cache, tri_tensor* k_scales, tri_tensor* v_cache,
+                     tri_tensor* v_scales, const tri_tensor* lens, const tri_cache_params* p, void* hip_stream) {
+  TRI_TRY(tri_validate_cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, p));
+  if (cache_is_empty(p) || p->kv_len == 0) return TRI_OK;
+  return TRI_DISPATCH(k, impl_cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, p, hip_stream));
+}
+
+int tri_validate_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scales, const tri_tensor* v_cache,
+                            const tri_tensor* v_scales, const tri_tensor* lens, const tri_tensor* k, const tri_tensor* v,
+                            const tri_cache_params* p) {
+  TRI_TRY(check_cache_params(p, false));
+  const int dt = elem_dtype(k);
+  TRI_TRY(check_cache4(k, p->batch, p->n_kv_heads, p->seq, true, p->head_dim, 8, 16, dt, true));
+  TRI_TRY(check_cache4(v, p->batch, p->n_kv_heads, p->seq, true, p->head_dim, 8, 16, dt, true));
+  return check_caches(k_cache, k_scales, v_cache, v_scales, lens, p, dt, false);
+}
+
+int tri_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scales, const tri_tensor* v_cache, const tri_tensor* v_scales,
+                   const tri_tensor* lens, tri_tensor* k, tri_tensor* v, const tri_cache_params* p, void* hip_stream) {
+  TRI_TRY(tri_validate_cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, p));
+  if (cache_is_empty(p)) return TRI_OK;
+  return TRI_DISPATCH(k, impl_cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, p, hip_stream));
+}
+
+int64_t tri_cache_scratch_bytes(const tri_cache_params* p, int32_t four_bit) {
+  TRI_TRY(check_cache_params(p, true));
+  if (cache_is_empty(p) || p->kv_len == 0) return 0;
+  const int all = 1 << 30;  // (more than any position)
+  return cache_attn_workspace_bytes(p->batch, p->seq, p->n_q_heads, p->n_kv_heads, p->head_dim, p->kv_len,
+                                    p->window < all ? p->window : all, p->sinks < all ? p->sinks : all, four_bit != 0);
+}
+
+int tri_validate_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales,
+                                 const tri_tensor* v_cache, const tri_tensor* v_scales, const tri_tensor* lens,
+                                 const tri_tensor* scratch, const tri_tensor* lse, const tri_tensor* out,
+                                 const tri_cache_params* p) {
+  TRI_TRY(check_cache_params(p, true));
+  const int dt = elem_dtype(q);
+  const int64_t rows = (int64_t)p->batch * p->seq, cols = (int64_t)p->n_q_heads * p->head_dim;
+  TRI_TRY(check_mat(q, rows, cols, dt));
+  TRI_TRY(check_mat(out, rows, cols, dt));
+  TRI_TRY(check_caches(k_cache, k_scales, v_cache, v_scales, lens, p, dt, false));
+  TRI_TRY(check_ws(scratch));
+  if (scratch != nullptr && scratch->shape[0] > 0 && ((uintptr_t)scratch->ptr & 255u) != 0) return TRI_ERR_ALIGN;
+  if (lse != nullptr) {
+    if (lse->dtype != TRI_F32) return TRI_ERR_DTYPE;
+    if (lse->ndim != 3 || lse->shape[0] != p->batch || lse->shape[1] != p->n_q_heads || lse->shape[2] != p->seq) return TRI_ERR_SHAPE;
+    if (cache_is_empty(p)) return TRI_OK;
+    if (lse->ptr == nullptr) return TRI_ERR_NULL;
+    if ((p->seq > 1 && lse->stride[2] != 1) || (p->n_q_heads > 1 && lse->stride[1] != p->seq) ||
+        (p->batch > 1 && lse->stride[0] != (int64_t)p->n_q_heads * p->seq))
+      return TRI_ERR_STRIDE;
+    if (((uintptr_t)lse->ptr & 3u) != 0) return TRI_ERR_ALIGN;
+  }
+  return TRI_OK;
+}
+
+int tri_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales, const tri_tensor* v_cache,
+                        const tri_tensor* v_scales, const tri_tensor* lens, tri_tensor* scratch, tri_tensor* lse,
+                        tri_tensor* out, const tri_cache_params* p, void* hip_stream) {
+  TRI_TRY(tri_validate_cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, p));
+  if (cache_is_empty(p)) return TRI_OK;
+  return TRI_DISPATCH(q, impl_cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, p, hip_stream));
 }
 
 }  // extern "C"

@@ -7,6 +7,7 @@
 // Every function takes the tensors (or descriptors of them) in the order of the C entry point (None where it allows
 // NULL), then its scalars, then the stream as an integer, and returns the status; trinity_amd/ext.py turns a status into
 // an exception.
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -48,6 +49,7 @@ bool to_tri(PyObject* o, tri_tensor& v, tri_tensor*& p) {
     case at::kFloat: v.dtype = TRI_F32; break;
     case at::kByte: v.dtype = TRI_U8; break;
     case at::kFloat8_e4m3fn: v.dtype = TRI_FP8_E4M3; break;
+    case at::kInt: v.dtype = TRI_I32; break;
     default: PyErr_Format(PyExc_TypeError, "unsupported dtype %s", at::toString(t.scalar_type())); return false;
   }
   const int64_t nd = t.dim();
@@ -76,17 +78,39 @@ bool marshal(PyObject* const* args, Py_ssize_t nargs, int ntensors, int nscalars
   return true;
 }
 
-// the bytes of a ctypes structure (tri_attn_params)
-struct Params {
-  Py_buffer buf{};
-  const tri_attn_params* p = nullptr;
-  explicit Params(PyObject* o) {
-    if (PyObject_GetBuffer(o, &buf, PyBUF_SIMPLE) != 0) return;
-    if (buf.len == (Py_ssize_t)sizeof(tri_attn_params)) p = static_cast<const tri_attn_params*>(buf.buf);
-    else PyErr_SetString(PyExc_TypeError, "expected TriAttnParams");
+// The tensors of a call are on one device (a length or a scale read from host memory would fault the GPU), which is the
+// current one while the call launches.
+struct OneDevice {
+  c10::OptionalDeviceGuard guard;
+  bool ok = true;
+  OneDevice(PyObject* const* args, int ntensors) {
+    const at::Tensor* first = nullptr;
+    for (int i = 0; i < ntensors && ok; ++i) {
+      if (!THPVariable_Check(args[i])) continue;
+      const at::Tensor& t = THPVariable_Unpack(args[i]);
+      if (first == nullptr) first = &t;
+      ok = t.device() == first->device();
+    }
+    if (!ok) PyErr_SetString(PyExc_ValueError, "the tensors of a call have to be on one device");
+    else if (first != nullptr && first->is_cuda()) guard.reset_device(first->device());
   }
-  ~Params() { if (buf.obj != nullptr) PyBuffer_Release(&buf); }
 };
+
+// the bytes of a ctypes structure (tri_attn_params, tri_cache_params)
+template <class T>
+struct ParamsOf {
+  static_assert(sizeof(tri_attn_params) != sizeof(tri_cache_params), "told apart by their sizes");
+  Py_buffer buf{};
+  const T* p = nullptr;
+  explicit ParamsOf(PyObject* o) {
+    if (PyObject_GetBuffer(o, &buf, PyBUF_SIMPLE) != 0) return;
+    if (buf.len == (Py_ssize_t)sizeof(T)) p = static_cast<const T*>(buf.buf);
+    else PyErr_SetString(PyExc_TypeError, sizeof(T) == sizeof(tri_attn_params) ? "expected TriAttnParams" : "expected TriCacheParams");
+  }
+  ~ParamsOf() { if (buf.obj != nullptr) PyBuffer_Release(&buf); }
+};
+using Params = ParamsOf<tri_attn_params>;
+using CacheParams = ParamsOf<tri_cache_params>;
 
 void* stream_of(PyObject* o) { return PyLong_AsVoidPtr(o); }
 
@@ -213,8 +237,50 @@ TRI_BIND(roco) {  // (as_mean_var comes before the parameters, as in the C entry
     });
   });
 }
+TRI_BIND(cache_append) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 7, 1, t)) return 0;
+    const OneDevice device(a, 7);
+    if (!device.ok) return 0;
+    const CacheParams p(a[7]);
+    void* s = stream_of(a[8]);
+    return call([&] { return tri_cache_append(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], p.p, s); });
+  });
+}
+TRI_BIND(cache_read) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 7, 1, t)) return 0;
+    const OneDevice device(a, 7);
+    if (!device.ok) return 0;
+    const CacheParams p(a[7]);
+    void* s = stream_of(a[8]);
+    return call([&] { return tri_cache_read(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], p.p, s); });
+  });
+}
+TRI_BIND(cache_attention) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 9, 1, t)) return 0;
+    const OneDevice device(a, 9);
+    if (!device.ok) return 0;
+    const CacheParams p(a[9]);
+    void* s = stream_of(a[10]);
+    return call([&] {
+      return tri_cache_attention(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], t.p[7], t.p[8], p.p, s);
+    });
+  });
+}
 #undef TRI_BIND
 
+PyObject* cache_scratch_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) return PyErr_Format(PyExc_TypeError, "expected 2 arguments, got %zd", n);
+  const CacheParams p(a[0]);
+  const long four_bit = PyLong_AsLong(a[1]);
+  if (PyErr_Occurred() != nullptr) return nullptr;
+  return PyLong_FromLongLong(tri_cache_scratch_bytes(p.p, four_bit != 0));
+}
 PyObject* qkv_scratch_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) return PyErr_Format(PyExc_TypeError, "expected 2 arguments, got %zd", n);
   const Params p(a[0]);
@@ -238,6 +304,8 @@ PyMethodDef methods[] = {
     TRI_METHOD("keyformer", keyformer), TRI_METHOD("roco", roco), TRI_METHOD("qkv_scratch_bytes", qkv_scratch_bytes),
     TRI_METHOD("gemm_workspace_bytes", workspace_bytes<tri_gemm_workspace_bytes>),
     TRI_METHOD("ffn_workspace_bytes", workspace_bytes<tri_ffn_workspace_bytes>),
+    TRI_METHOD("cache_append", cache_append), TRI_METHOD("cache_read", cache_read),
+    TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -260,6 +260,43 @@ enum ScoreForm { kScoreBlock, kScoreBlockPair, kScoreHalfBlock, kScoreHalfBlockP
 int score_form(int S, int P, int Hq, bool causal);
 int launch_scores_few(const ScoreArgs& a, hipStream_t stream);  // S <= kFewMaxQueries; 1 = not applicable
 
+// Caches of several sequences (tri_cache_*): one format per call, 16-bit elements or 4-bit blocks.  Element (b, h, row) of
+// a cache starts at p + b * sb + h * sh + row * sr, in elements of 16 bits, or in bytes; scales likewise.
+struct CacheView {
+  void* p;
+  int64_t sb, sh, sr;
+  uint8_t* scales;  // nullptr: 16-bit elements
+  int64_t xb, xh, xr;
+};
+// k, v of tri_cache_append [B * S, Hkv * D] (element (b, h, row) at b * sb + h * sh + row * sr here too), and of tri_cache_read
+struct CacheRowsArgs {
+  half_t *k, *v;
+  int64_t k_sb, k_sh, k_sr, v_sb, v_sh, v_sr;
+  CacheView kc, vc;
+  const int32_t* lens;
+  int B, S, Hkv, D, kv_len, rows;  // rows: of the caches
+};
+int launch_cache_append(const CacheRowsArgs& a, hipStream_t stream);
+int launch_cache_read(const CacheRowsArgs& a, hipStream_t stream);
+
+struct CacheAttnArgs {
+  const half_t* q;  // [B * S, Hq * D]
+  int64_t ldq;
+  CacheView kc, vc;
+  const int32_t* lens;
+  half_t* out;
+  int64_t ldo;
+  float* lse;  // nullable [B, Hq, S]
+  int B, S, Hq, Hkv, D, kv_len;
+  float scale;
+  int causal, window, sinks;
+  float* ws;  // nullable: partial results of the runs
+  int64_t ws_bytes;
+  int runs;  // set by the launcher: parts that a row block's keys are cut into
+};
+int launch_cache_attention(const CacheAttnArgs& a, hipStream_t stream);
+int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
+
 }  // namespace tri
 
 #endif  // once per element type

@@ -17,9 +17,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtrinity_amd.so")
 NATIVE_PATH = os.path.join(_HERE, "_native.so")
 
-TRI_F16, TRI_BF16, TRI_F32, TRI_U8, TRI_FP8_E4M3 = 0, 1, 2, 3, 4
+TRI_F16, TRI_BF16, TRI_F32, TRI_U8, TRI_FP8_E4M3, TRI_I32 = 0, 1, 2, 3, 4, 5
 _DTYPES = {torch.float16: TRI_F16, torch.bfloat16: TRI_BF16, torch.float32: TRI_F32, torch.uint8: TRI_U8,
-           torch.float8_e4m3fn: TRI_FP8_E4M3}
+           torch.float8_e4m3fn: TRI_FP8_E4M3, torch.int32: TRI_I32}
 
 
 class TriTensor(ctypes.Structure):
@@ -52,6 +52,21 @@ class TriAttnParams(ctypes.Structure):
     ]
 
 
+class TriCacheParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("seq", ctypes.c_int32),
+        ("kv_len", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+    ]
+
+
 class TrinityError(RuntimeError):
     def __init__(self, fn, status, text):
         super().__init__("%s failed: status %d (%s)" % (fn, status, text))
@@ -73,6 +88,9 @@ EXPORTS = [
     "tri_qkv_attention", "tri_validate_qkv_attention", "tri_qkv_attention_static",
     "tri_keyformer", "tri_validate_keyformer",
     "tri_roco", "tri_validate_roco",
+    "tri_cache_append", "tri_validate_cache_append",
+    "tri_cache_read", "tri_validate_cache_read",
+    "tri_cache_scratch_bytes", "tri_cache_attention", "tri_validate_cache_attention",
     "tri_diag_issue_probe", "tri_diag_power_probe",
 ]
 
@@ -301,6 +319,51 @@ def roco(x, norm_w, wq, wk, wv, k_cache, v_cache, scratch, out, sum_out, sumsq_o
                        params, _stream_ptr(x))
     if st:
         _check("tri_roco", st)
+    return st
+
+
+def cache_params(batch, n_kv_heads, head_dim, seq, kv_len, n_q_heads=None, scale=None, causal=True, window=0, sinks=0):
+    p = TriCacheParams()
+    p.batch, p.n_kv_heads, p.head_dim, p.seq, p.kv_len = batch, n_kv_heads, head_dim, seq, kv_len
+    p.n_q_heads = n_kv_heads if n_q_heads is None else n_q_heads
+    p.scale = (1.0 / math.sqrt(head_dim)) if scale is None else scale
+    p.causal, p.window, p.sinks = int(bool(causal)), window, sinks
+    return p
+
+
+def cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_cache_append", [k, v, k_cache, k_scales, v_cache, v_scales, lens, ctypes.byref(params)], True)
+    st = native().cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, _stream_ptr(k))
+    if st:
+        _check("tri_cache_append", st)
+    return st
+
+
+def cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_cache_read", [k_cache, k_scales, v_cache, v_scales, lens, k, v, ctypes.byref(params)], True)
+    st = native().cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, _stream_ptr(k))
+    if st:
+        _check("tri_cache_read", st)
+    return st
+
+
+def cache_scratch_bytes(params, four_bit):
+    """Bytes of scratch with which cache_attention runs its fastest plan (0: it needs none)."""
+    n = native().cache_scratch_bytes(params, int(bool(four_bit)))
+    if n < 0:
+        _check("tri_cache_scratch_bytes", n)
+    return n
+
+
+def cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_cache_attention", [q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out,
+                                                      ctypes.byref(params)], True)
+    st = native().cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, _stream_ptr(q))
+    if st:
+        _check("tri_cache_attention", st)
     return st
 
 
