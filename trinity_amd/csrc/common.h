@@ -50,6 +50,16 @@ __device__ __forceinline__ float16v mfma32(half8v a, half8v b, float16v c) {
 #endif
 }
 
+// D[16x16] += A[16x32] * B[32x16].  Lane l supplies row (l % 16) of A and column (l % 16) of B, eight consecutive k each,
+// k-group (l / 16); it receives column (l % 16) of D, register r being row 4*(l/16) + r.
+__device__ __forceinline__ float4v mfma16(half8v a, half8v b, float4v c) {
+#ifdef TRI_BF16
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#endif
+}
+
 // two probabilities (non-negative, at most 2^8) to the element type: fp16 truncates (one instruction), bf16 rounds
 __device__ __forceinline__ half2v pack_prob(float a, float b) {
 #ifdef TRI_BF16

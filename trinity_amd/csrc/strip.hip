@@ -12,16 +12,6 @@
 
 namespace tri {
 
-// D[16 x 16] += A[16 x 32] * B[32 x 16].  Lane l supplies row (l % 16) of A and column (l % 16) of B, eight consecutive k
-// each, k-group (l / 16), and receives column (l % 16), rows 4 * (l / 16) + r of D.
-__device__ __forceinline__ float4v mfma16(half8v a, half8v b, float4v c) {
-#ifdef TRI_BF16
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-#else
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-#endif
-}
-
 constexpr int kStripCols = 16, kStripPiece = 128, kStripWaves = 4;
 // Three stages: 48 KB, so that three workgroups fit a CU (4 rows x [4544, 18176], 1136 workgroups, 27.3 us, with four 31.9;
 // with one workgroup a CU level: one row x [14336, 4096] within 0.3).
