@@ -12,6 +12,8 @@
 // Scores are computed transposed, S^T[key, row] = K . Q^T, so that a lane owns one row and sixteen keys of a block of 32,
 // the running maximum and sum are per-lane scalars, and the probabilities lie in the registers as O^T += V^T . P^T wants
 // them.
+#include <type_traits>
+
 #include "common.h"
 #include "fp4.h"
 #include "launch.h"
@@ -81,32 +83,149 @@ struct CacheLds {
   __device__ static __forceinline__ int fv(int row) { return D == 128 ? ((row & 3) << 2) : (((row >> 1) & 1) << 2); }
 };
 
-// blockIdx.x: (run, row block, KV head, sequence), the last one outermost
+// Workgroups go to the eight XCDs in turn, each with an L2 of its own: the row blocks of one KV head, which read the same
+// keys, stay on one XCD.  Per XCD the latest row blocks, which see most, come first.
+__device__ __forceinline__ void cache_wg_map(int id, int heads, int nrb, int runs, int& bh, int& rb, int& run) {
+  const int per = nrb * runs;
+  if (heads % 8 == 0) {
+    const int x = id % 8, s = id / 8, hx = heads / 8;
+    bh = x * hx + s % hx;
+    id = s / hx;
+  } else {
+    bh = id / per;
+    id %= per;
+  }
+  rb = nrb - 1 - id / runs;
+  run = id % runs;
+}
+
+// ---------------------------------------------------------------------------------------------------- many rows
+// Four waves of 32 rows walk tiles of 64 keys.  Inside each wave the matrix pipe works on S^T of tile t + 1 while the
+// probabilities of tile t are computed, and on O^T of tile t while the maximum of tile t + 1 is found; a slot below holds
+// the MFMAs of one K or V fragment, the LDS read of a fragment PD slots ahead, and its share of the vector arithmetic.
+// Step t reads K(t + 1) and V(t), so K tiles travel two steps ahead and V tiles one; each has two buffers.  16-bit tiles go
+// from memory to LDS directly.  4-bit tiles are a 16-byte block per thread: it travels through registers, a step longer,
+// and is turned into 16 bits in the slots of O^T, which have little else to do.
+template <int D>
+struct TilePipe {
+  static constexpr int KSTEPS = D / 16, DT = D / 32;
+  static constexpr int NKF = 2 * KSTEPS, NVF = 4 * DT;  // K / V fragments (MFMAs) per tile
+  static constexpr int GPS = 16 / NKF, EPS = 32 / NVF;  // pairs of probabilities per S^T slot; scores per O^T slot
+  static constexpr int PD = 3, RING = 4;
+};
+
 template <int D, bool FP4>
-__device__ __forceinline__ void cache_attn_body(const CacheAttnArgs& a, half_t* lds) {
+__device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, half_t* lds, const half_t* __restrict__ qglob) {
+  // (qglob = a.q.  Inlined, every LDS access of this function carries "does not alias q", and an LDS read with alias
+  // information is not made to wait for the loads to LDS in flight; barriers and explicit waits order those here.)
   using L = CacheLds<D>;
-  constexpr int KSTEPS = D / 16, DT = D / 32, CPR = D / 8;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  using P = TilePipe<D>;
+  constexpr int KSTEPS = P::KSTEPS, DT = P::DT, NKF = P::NKF, NVF = P::NVF, GPS = P::GPS, EPS = P::EPS, PD = P::PD, RING = P::RING;
+  constexpr int CPR = L::CPR;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, g = lane >> 5;
   const int group = a.Hq / a.Hkv, rows = a.S * group, nrb = (rows + kCacheRows - 1) / kCacheRows;
-  int id = (int)blockIdx.x;
-  const int run = id % a.runs; id /= a.runs;
-  const int rb = nrb - 1 - id % nrb; id /= nrb;  // (the latest rows, which see most, first)
-  const int hk = id % a.Hkv, b = id / a.Hkv;
-  const int r0 = rb * kCacheRows;
+  int bh, rb, run;
+  cache_wg_map((int)blockIdx.x, a.B * a.Hkv, nrb, a.runs, bh, rb, run);
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int r0 = rb * kCacheRows, w0 = r0 + wave * 32;
   const KeyList kl = key_list(a, b, r0 / group, (min(r0 + kCacheRows, rows) - 1) / group);
   const int ntiles = (kl.n + kCacheTile - 1) / kCacheTile;
-  const int per = (ntiles + a.runs - 1) / a.runs, tile0 = min(run * per, ntiles), tile1 = min(tile0 + per, ntiles);
+  const int per = (ntiles + a.runs - 1) / a.runs, tile0 = min(run * per, ntiles);
+  const int nsteps = min(per, ntiles - tile0);
 
-  const int row = r0 + wave * 32 + l32, rowc = min(row, rows - 1);
+  const int row = w0 + l32, rowc = min(row, rows - 1);
   const int tok = rowc / group, head = hk * group + rowc % group;
   const int pos = kl.len - a.S + tok;
+  // positions of the wave's rows (it may have none)
+  const int pos0 = kl.len - a.S + min(w0, rows - 1) / group, pos1 = kl.len - a.S + min(w0 + 31, rows - 1) / group;
+  // the steps that hold a key some row of the wave sees are [0, nact)
+  const int seen = a.causal ? min(kl.n, pos1 + 1 - kl.gap) : kl.n;  // ... of the list
+  const int nact = w0 >= rows ? 0 : max(0, min(nsteps, (seen + kCacheTile - 1) / kCacheTile - tile0));
+
   half8v qf[KSTEPS];
-  const half_t* qp = a.q + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)head * D + g * 8;
+  const half_t* qp = qglob + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)head * D + g * 8;
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *reinterpret_cast<const half8v*>(qp + ks * 16);
 
-  half_t *const kt = lds, *const vt = lds + L::HALFS;
+  // ---- tiles: a thread's pieces of 16 bytes (16-bit: chunks, 4-bit: blocks) and the row of the tile each is of
+  constexpr int PPR = FP4 ? D / 32 : CPR;              // pieces per row
+  constexpr int NP = kCacheTile * PPR / 256;           // per thread (4-bit, D = 64: half the threads have one)
+  constexpr bool HALF = NP == 0;
+  constexpr int NPA = HALF ? 1 : NP;
+  constexpr int ES = FP4 ? 1 : 2;
+  const uint8_t* const kbase = static_cast<const uint8_t*>(a.kc.p) + (b * a.kc.sb + hk * a.kc.sh) * ES;
+  const uint8_t* const vbase = static_cast<const uint8_t*>(a.vc.p) + (b * a.vc.sb + hk * a.vc.sh) * ES;
+  const uint8_t* const kxbase = FP4 ? a.kc.scales + b * a.kc.xb + hk * a.kc.xh : nullptr;
+  const uint8_t* const vxbase = FP4 ? a.vc.scales + b * a.vc.xb + hk * a.vc.xh : nullptr;
+  const int64_t ksr = a.kc.sr * ES, vsr = a.vc.sr * ES;
+  half_t *const kt = lds, *const vt = lds + 2 * L::HALFS;
+  // key of row r of a tile (past the last key: the last one again, whose scores are masked)
+  auto key_of = [&](int step, int r) {
+    const int li = min((tile0 + step) * kCacheTile + r, kl.n - 1);
+    return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
+  };
+  auto load16 = [&](int step, bool isv) {  // 16-bit: to LDS, 1 KB an instruction
+    half_t* const dst = (isv ? vt : kt) + (step & 1) * L::HALFS;
+#pragma unroll
+    for (int i = 0; i < NPA; ++i) {
+      const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
+      const uint8_t* src = (isv ? vbase : kbase) + key_of(step, r) * (isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src,
+                                       (TRI_LDS void*)(dst + (i * 4 + wave) * 512), 16, 0, 0);
+    }
+  };
+  uint4v kraw, vraw;
+  uint32_t kxraw = 0, vxraw = 0;
+  const int pr = (HALF ? t % 128 : t) / PPR, pc = (HALF ? t % 128 : t) % PPR;  // 4-bit: the thread's row and block (HALF: K for the first 128 threads, V for the others)
+  const bool has_k = !HALF || t < 128, has_v = !HALF || t >= 128;
+  auto fetch4 = [&](int step, bool isv) {
+    const int64_t key = key_of(step, pr);
+    if (isv) {
+      vraw = *reinterpret_cast<const uint4v*>(vbase + key * vsr + pc * 16);
+      vxraw = vxbase[key * a.vc.xr + pc];
+    } else {
+      kraw = *reinterpret_cast<const uint4v*>(kbase + key * ksr + pc * 16);
+      kxraw = kxbase[key * a.kc.xr + pc];
+    }
+  };
+  auto commit4 = [&](int step, bool isv, int j) {  // chunk j of the block
+    half_t* const dst = (isv ? vt : kt) + (step & 1) * L::HALFS;
+    if (isv ? has_v : has_k)
+      *reinterpret_cast<half8v*>(dst + pr * D + (((pc * 4 + j) ^ (isv ? L::fv(pr) : L::fk(pr))) << 3)) =
+          fp4x8_to_half8(isv ? vraw[j] : kraw[j], fp4_scale(isv ? vxraw : kxraw));
+  };
+
+  // ---- fragments: K fragment j = (16 channels j / 2, key half j % 2), V fragment v = (key half, key quarter, 32 channels)
+  int kbyte[KSTEPS], vbyte[DT];
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ++ks) {
+    kbyte[ks] = (l32 * D + (((ks * 2 + g) ^ L::fk(l32)) << 3)) * 2;
+    asm volatile("" : "+v"(kbyte[ks]));
+  }
+  const int j4 = (lane & 15) >> 2;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    vbyte[dt] = (int)(uint32_t)(uintptr_t)lds + (2 * L::HALFS + (4 * g + j4) * D + ((chunk ^ L::fv(j4)) << 3) + (lane & 1) * 4) * 2;
+    asm volatile("" : "+v"(vbyte[dt]));
+  }
+  const char* const ldsb = reinterpret_cast<const char*>(lds);
+  auto read_kf = [&](int par, int j) {
+    return *reinterpret_cast<const half8v*>(ldsb + kbyte[j / 2] + (par * L::HALFS + (j % 2) * 32 * D) * 2);
+  };
+  auto read_vf = [&](int par, int v) {
+    TRI_LDS char* vp = (TRI_LDS char*)(uintptr_t)(uint32_t)vbyte[v % DT] +
+                       (par * L::HALFS + ((v / (2 * DT)) * 32 + ((v / DT) % 2) * 16) * D) * 2;
+    const short4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TRI_LDS short4s*)vp);
+    const short4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TRI_LDS short4s*)(vp + 8 * D * 2));
+    half4v hl, hh;
+    __builtin_memcpy(&hl, &lo, 8);
+    __builtin_memcpy(&hh, &hi, 8);
+    return cat8(hl, hh);
+  };
+
   const float c2 = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;
   float16v o[DT];
@@ -115,55 +234,34 @@ __device__ __forceinline__ void cache_attn_body(const CacheAttnArgs& a, half_t* 
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
 
-  const int j4 = (lane & 15) >> 2;
-  for (int tile = tile0; tile < tile1; ++tile) {
-    __syncthreads();
-    // ---- K and V to LDS (past the last key: the last one again, whose scores are masked)
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const CacheView& c = kv ? a.vc : a.kc;
-      half_t* const dst = kv ? vt : kt;
-      for (int p = t; p < kCacheTile * CPR; p += 256) {
-        const int r = p / CPR, ch = p % CPR;
-        const int li = min(tile * kCacheTile + r, kl.n - 1);
-        const int64_t key = li + (li < kl.sinks ? 0 : kl.gap);
-        half8v x;
-        if (FP4) {
-          const uint8_t* src = static_cast<const uint8_t*>(c.p) + b * c.sb + hk * c.sh + key * c.sr + ch * 4;
-          x = fp4x8_to_half8(*reinterpret_cast<const uint32_t*>(src), fp4_scale(c.scales[b * c.xb + hk * c.xh + key * c.xr + ch / 4]));
-        } else {
-          x = *reinterpret_cast<const half8v*>(static_cast<const half_t*>(c.p) + b * c.sb + hk * c.sh + key * c.sr + ch * 8);
-        }
-        *reinterpret_cast<half8v*>(dst + r * D + ((ch ^ (kv ? L::fv(r) : L::fk(r))) << 3)) = x;
-      }
-    }
-    __syncthreads();
-    // ---- S^T = K . Q^T
-    float16v st[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) st[mt][r] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KSTEPS; ++ks)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-        st[mt] = mfma32(lds_read8(kt + (mt * 32 + l32) * D + (((ks * 2 + g) ^ L::fk(l32)) << 3)), qf[ks], st[mt]);
-    // ---- mask, maximum
-    float mx = -INFINITY;
+  auto need_mask = [&](int step) {  // (see the kernel of few rows)
+    const int li0 = (tile0 + step) * kCacheTile, li1 = li0 + kCacheTile - 1;
+    return li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0) ||
+           (a.window > 0 && li0 + (li0 < kl.sinks ? 0 : kl.gap) <= pos1 - a.window && li1 >= a.sinks);
+  };
+  auto apply_mask = [&](float16v (&s)[2], int step) {
+    // visible: keys up to `last`, and from `from` on or below a.sinks
+    const int last = pos < 0 ? -1 : (a.causal ? pos : kl.len - 1), from = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int li = tile * kCacheTile + mt * 32 + (r >> 2) * 8 + g * 4 + (r & 3);
+        const int li = (tile0 + step) * kCacheTile + mt * 32 + (r >> 2) * 8 + g * 4 + (r & 3);
         const int key = li + (li < kl.sinks ? 0 : kl.gap);
-        const bool hidden = li >= kl.n || pos < 0 || (a.causal && key > pos) ||
-                            (a.window > 0 && key <= pos - a.window && key >= a.sinks);
-        if (hidden) st[mt][r] = -INFINITY;
-        mx = fmaxf(mx, st[mt][r]);
+        if (li >= kl.n || key > last || (key < from && key >= a.sinks)) s[mt][r] = -INFINITY;
       }
+  };
+  auto tile_max = [&](const float16v (&s)[2]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
+    return mx;
+  };
+  auto raise = [&](float mx) {  // mx: the lane's maximum of the raw scores
     mx = pair_max(mx) * c2;
-    if (__builtin_amdgcn_ballot_w64(mx > m + kCacheLazyMax) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mx > m + kCacheLazyMax) != 0) {  // wave-uniform
       const float mnew = fmaxf(m, mx);
       const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m - mnew);
       m = mnew;
@@ -171,30 +269,142 @@ __device__ __forceinline__ void cache_attn_body(const CacheAttnArgs& a, half_t* 
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : -m;
-    // ---- probabilities, rounded to nearest (half the error of cutting them off), their sum before that
-    half8v pf[2][2];
+  };
+  auto zero = [&](float16v (&s)[2]) {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+      for (int r = 0; r < 16; ++r) s[mt][r] = 0.f;
+  };
+  // probabilities (two keys) of group gi, rounded to nearest - half the error of cutting them off -, their sum before that
+  half8v pf[2][2];
+  float sum, nm;
+  auto softmax_pair = [&](const float16v (&s)[2], int gi) {
+    const int mt = gi / 8, hh = (gi / 4) % 2, e = (gi % 4) * 2;
+    const float p0 = fast_exp2(fmaf(s[mt][hh * 8 + e], c2, nm));
+    const float p1 = fast_exp2(fmaf(s[mt][hh * 8 + e + 1], c2, nm));
+    sum += p0 + p1;
+    pf[mt][hh][e] = (half_t)p0;
+    pf[mt][hh][e + 1] = (half_t)p1;
+  };
+
+  // this wave's share of the tiles is in LDS - 4-bit: written, lgkmcnt(0); 16-bit: landed, vmcnt(0) - and everybody's
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    if constexpr (FP4) __builtin_amdgcn_s_waitcnt(0xC07F);
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");  // (to the compiler the barrier is no memory access)
+  };
+
+  half8v fr[RING];
+  // One step.  cur: S^T of its tile, masked, its maximum folded into m; next: receives S^T of the next tile.
+  auto step = [&](int st, auto parc, float16v (&cur)[2], float16v (&next)[2]) __attribute__((always_inline)) {
+    constexpr int PAR = decltype(parc)::value;
+    meet();  // K(st + 1) and V(st) are there, K(st) and V(st - 1) retired
+    if constexpr (!FP4) {
+      if (st + 2 < nsteps) load16(st + 2, false);
+      if (st + 1 < nsteps) load16(st + 1, true);
+    }
+    auto commit_all = [&]() {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = fast_exp2(fmaf(st[mt][hh * 8 + e], c2, nm));
-          l += p;
-          pf[mt][hh][e] = (half_t)p;
+      for (int j = 0; j < 4; ++j) {
+        commit4(st, false, j);      // K(st + 2): the buffer of K(st)
+        commit4(st + 1, true, j);
+      }
+    };
+    if (st < nact) {
+      // ---- S^T(st + 1) = K . Q^T beside the probabilities of tile st (after the wave's last tile the product is not used)
+#pragma unroll
+      for (int j = 0; j < PD; ++j) fr[j] = read_kf(PAR ^ 1, j);
+      zero(next);
+      sum = 0.f;
+      nm = m == -INFINITY ? 0.f : -m;
+      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NKF; ++j) {
+        if (j + PD < NKF) fr[(j + PD) % RING] = read_kf(PAR ^ 1, j + PD);
+        else fr[(j + PD) % RING] = read_vf(PAR, j + PD - NKF);
+        next[j % 2] = mfma32(fr[j % RING], qf[j / 2], next[j % 2]);
+#pragma unroll
+        for (int x = 0; x < GPS; ++x) softmax_pair(cur, j * GPS + x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // ---- O^T += V^T . P^T of tile st beside the maximum of tile st + 1
+      float mx = -INFINITY;
+      __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int v = 0; v < NVF; ++v) {
+        if (v + PD < NVF) fr[(NKF + v + PD) % RING] = read_vf(PAR, v + PD);
+        o[v % DT] = mfma32(fr[(NKF + v) % RING], pf[v / (2 * DT)][(v / DT) % 2], o[v % DT]);
+#pragma unroll
+        for (int x = 0; x < EPS; ++x) {
+          const int idx = v * EPS + x;
+          mx = fmaxf(mx, next[idx / 16][idx % 16]);
         }
-    // ---- O^T += V^T . P^T
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-          const half_t* vp = vt + (mt * 32 + hh * 16 + 4 * g + j4) * D + ((chunk ^ L::fv(j4)) << 3) + (lane & 1) * 4;
-          o[dt] = mfma32(cat8(lds_read_tr16(vp), lds_read_tr16(vp + 8 * D)), pf[mt][hh], o[dt]);
+        if constexpr (FP4) {
+          if (v % (NVF / 8) == 0) {
+            const int j = v / (NVF / 8);
+            commit4(st + (j % 2), j % 2 != 0, j / 2);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l += sum;
+      if (st + 1 < nact) {
+        if (need_mask(st + 1)) {  // wave-uniform
+          asm volatile("");
+          apply_mask(next, st + 1);
+          mx = tile_max(next);
+        }
+        raise(mx);
+      }
+    } else if constexpr (FP4) {
+      commit_all();
+    }
+    if constexpr (FP4) {  // (past the last step: its last keys again)
+      fetch4(st + 3, false);
+      fetch4(st + 2, true);
+    }
+  };
+
+  if (nsteps > 0) {
+    // ---- prologue: K(0), K(1), V(0); S^T of tile 0
+    if constexpr (FP4) {
+      fetch4(0, false);
+      fetch4(0, true);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        commit4(0, false, j);
+        commit4(0, true, j);
+      }
+      fetch4(1, false);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) commit4(1, false, j);
+      fetch4(2, false);
+      fetch4(1, true);
+    } else {
+      load16(0, false);
+      if (1 < nsteps) load16(1, false);
+      load16(0, true);
+    }
+    meet();
+    float16v sa[2], sb[2];
+    if (0 < nact) {
+      zero(sa);
+#pragma unroll
+      for (int j = 0; j < NKF; ++j) sa[j % 2] = mfma32(read_kf(0, j), qf[j / 2], sa[j % 2]);
+      if (need_mask(0)) {
+        asm volatile("");
+        apply_mask(sa, 0);
+      }
+      raise(tile_max(sa));
+    }
+    for (int st = 0; st < nsteps; st += 2) {
+      step(st, std::integral_constant<int, 0>{}, sa, sb);
+      if (st + 1 < nsteps) step(st + 1, std::integral_constant<int, 1>{}, sb, sa);
+    }
   }
 
   l = pair_sum(l);
@@ -208,9 +418,9 @@ __device__ __forceinline__ void cache_attn_body(const CacheAttnArgs& a, half_t* 
 }
 
 template <int D, bool FP4>
-__global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) half_t lds[2 * CacheLds<D>::HALFS];
-  cache_attn_body<D, FP4>(a, lds);
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_tile_kernel(CacheAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) half_t lds[4 * CacheLds<D>::HALFS];
+  cache_attn_tile_body<D, FP4>(a, lds, a.q);
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows
@@ -588,7 +798,7 @@ template <int D, bool FP4>
 static void launch_t(const CacheAttnArgs& a, int nt, unsigned nwg, hipStream_t stream) {
   if (nt == 1) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
   else if (nt == 2) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 2>), dim3(nwg), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((cache_attn_kernel<D, FP4>), dim3(nwg), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4>), dim3(nwg), dim3(256), 0, stream, a);
 }
 
 template <int D>
