@@ -26,6 +26,11 @@ constexpr int kCacheRows = 128;      // stacked rows per workgroup, 32 a wave
 // sums are rescaled rarely
 constexpr float kCacheLazyMax = 8.0f;
 
+// row / group, with the launcher's multiplier (a division takes forty instructions, and there is one per row that is stored)
+__device__ __forceinline__ int row_token(const CacheAttnArgs& a, int row) {
+  return (int)(__umulhi((uint32_t)row << 4, a.div_mul) >> a.div_sh);
+}
+
 // what a row block of a sequence sees
 struct KeyList {
   int len;        // keys of the sequence
@@ -49,7 +54,7 @@ __device__ __forceinline__ KeyList key_list(const CacheAttnArgs& a, int b, int t
 // zeros and -inf)
 template <int D>
 __device__ __forceinline__ void store_row(const CacheAttnArgs& a, int b, int hk, int row, int d4, float m, float l, float4v acc) {
-  const int group = a.Hq / a.Hkv, tok = row / group, head = hk * group + row % group;
+  const int group = a.Hq / a.Hkv, tok = row_token(a, row), head = hk * group + row - tok * group;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   half4v hv;
 #pragma unroll
@@ -130,16 +135,16 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   cache_wg_map((int)blockIdx.x, a.B * a.Hkv, nrb, a.runs, bh, rb, run);
   const int b = bh / a.Hkv, hk = bh % a.Hkv;
   const int r0 = rb * kCacheRows, w0 = r0 + wave * 32;
-  const KeyList kl = key_list(a, b, r0 / group, (min(r0 + kCacheRows, rows) - 1) / group);
+  const KeyList kl = key_list(a, b, row_token(a, r0), row_token(a, min(r0 + kCacheRows, rows) - 1));
   const int ntiles = (kl.n + kCacheTile - 1) / kCacheTile;
   const int per = (ntiles + a.runs - 1) / a.runs, tile0 = min(run * per, ntiles);
   const int nsteps = min(per, ntiles - tile0);
 
   const int row = w0 + l32, rowc = min(row, rows - 1);
-  const int tok = rowc / group, head = hk * group + rowc % group;
+  const int tok = row_token(a, rowc), head = hk * group + rowc - tok * group;
   const int pos = kl.len - a.S + tok;
   // positions of the wave's rows (it may have none)
-  const int pos0 = kl.len - a.S + min(w0, rows - 1) / group, pos1 = kl.len - a.S + min(w0 + 31, rows - 1) / group;
+  const int pos0 = kl.len - a.S + row_token(a, min(w0, rows - 1)), pos1 = kl.len - a.S + row_token(a, min(w0 + 31, rows - 1));
   // the steps that hold a key some row of the wave sees are [0, nact)
   const int seen = a.causal ? min(kl.n, pos1 + 1 - kl.gap) : kl.n;  // ... of the list
   const int nact = w0 >= rows ? 0 : max(0, min(nsteps, (seen + kCacheTile - 1) / kCacheTile - tile0));
@@ -408,6 +413,36 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   }
 
   l = pair_sum(l);
+  if (a.runs == 1) {
+    // ---- a lane has sixteen pieces of 8 bytes of its row: stored as they are, every store instruction touches 32 lines, so
+    // each wave turns its rows around in LDS and stores whole ones, 16 bytes a lane
+    constexpr int LDO = D + 8;
+    half_t* const stage = lds + wave * 32 * LDO;
+    __syncthreads();  // (every wave is done with the tiles)
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        half4v hv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hv[e] = (half_t)(o[dt][rq * 4 + e] * inv);
+        *reinterpret_cast<half4v*>(stage + l32 * LDO + dt * 32 + rq * 8 + g * 4) = hv;
+      }
+    if (a.lse != nullptr && g == 0 && row < rows)
+      a.lse[((int64_t)b * a.Hq + head) * a.S + tok] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    constexpr int RPI = 64 / CPR;  // rows per store instruction
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int r = i * RPI + lane / CPR, c = lane % CPR;
+      const half8v v = *reinterpret_cast<const half8v*>(stage + r * LDO + c * 8);
+      if (w0 + r < rows) {
+        const int tk = row_token(a, w0 + r), hd = hk * group + w0 + r - tk * group;
+        *reinterpret_cast<half8v*>(a.out + ((int64_t)b * a.S + tk) * a.ldo + (int64_t)hd * D + c * 8) = v;
+      }
+    }
+    return;
+  }
   if (row >= rows) return;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -463,9 +498,9 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
   int pos[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int row = min(nt * 16 + l16, rows - 1), tok = row / group;
+    const int row = min(nt * 16 + l16, rows - 1), tok = row_token(a, row);
     pos[nt] = kl.len - a.S + tok;
-    const half_t* qp = a.q + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)(hk * group + row % group) * D;
+    const half_t* qp = a.q + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)(hk * group + row - tok * group) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[nt][s] = *reinterpret_cast<const half8v*>(qp + (FP4 ? g * (D / 4) + s * 8 : s * 32 + g * 8));
   }
@@ -811,10 +846,13 @@ static void launch_merge(const CacheAttnArgs& a, hipStream_t stream) {
 }
 
 int launch_cache_attention(const CacheAttnArgs& args, hipStream_t stream) {
-  CacheAttnArgs a = args;
+  CacheAttnArgs a = args;  // (div_sh: 0)
   const CachePlan p = cache_plan(a.B, a.S, a.Hq, a.Hkv, a.kv_len, a.window, a.sinks);
   const int64_t fit = a.ws != nullptr ? a.ws_bytes / run_bytes(a.B, a.S, a.Hq, a.D) : 0;
   a.runs = (int)(fit < p.runs ? (fit < 1 ? 1 : fit) : p.runs);
+  const uint32_t group = (uint32_t)(a.Hq / a.Hkv);
+  while ((1u << a.div_sh) < group) ++a.div_sh;
+  a.div_mul = (uint32_t)((((uint64_t)1 << (28 + a.div_sh)) + group - 1) / group);
   const unsigned nwg = (unsigned)(p.nwg * a.runs);
   const bool fp4 = a.kc.scales != nullptr;
   if (a.D == 128) fp4 ? launch_t<128, true>(a, p.nt, nwg, stream) : launch_t<128, false>(a, p.nt, nwg, stream);

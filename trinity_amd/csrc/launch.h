@@ -292,7 +292,9 @@ struct CacheAttnArgs {
   int causal, window, sinks;
   float* ws;  // nullable: partial results of the runs
   int64_t ws_bytes;
-  int runs;  // set by the launcher: parts that a row block's keys are cut into
+  // set by the launcher: parts that a row block's keys are cut into; n / (Hq / Hkv) = (umulhi(16 n, div_mul) >> div_sh) below 2^28
+  int runs;
+  uint32_t div_mul, div_sh;
 };
 int launch_cache_attention(const CacheAttnArgs& a, hipStream_t stream);
 int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
