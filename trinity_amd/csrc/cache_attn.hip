@@ -239,22 +239,33 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
 
-  auto need_mask = [&](int step) {  // (see the kernel of few rows)
+  // Masks in terms of list indices: visible are those up to `last`, and of them those from `from` on or below a.sinks (in
+  // front of a gap all of these are sinks).  `last` differs between the wave's rows by less than 32, `from` as much.
+  const int last = pos < 0 ? -1 : (a.causal ? pos - kl.gap : kl.n - 1), from = a.window > 0 ? pos - a.window + 1 - kl.gap : 0;
+  auto need_mask = [&](int step) {
     const int li0 = (tile0 + step) * kCacheTile, li1 = li0 + kCacheTile - 1;
-    return li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0) ||
-           (a.window > 0 && li0 + (li0 < kl.sinks ? 0 : kl.gap) <= pos1 - a.window && li1 >= a.sinks);
+    return li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0) || (a.window > 0 && li0 + kl.gap <= pos1 - a.window && li1 >= a.sinks);
   };
   auto apply_mask = [&](float16v (&s)[2], int step) {
-    // visible: keys up to `last`, and from `from` on or below a.sinks
-    const int last = pos < 0 ? -1 : (a.causal ? pos : kl.len - 1), from = a.window > 0 ? pos - a.window + 1 : 0;
+    const int base = (tile0 + step) * kCacheTile + g * 4;  // the lane's scores are of indices base + (0 to 3) + 8 i
+    const int end = min(last, kl.n - 1) - base;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int li = (tile0 + step) * kCacheTile + mt * 32 + (r >> 2) * 8 + g * 4 + (r & 3);
-        const int key = li + (li < kl.sinks ? 0 : kl.gap);
-        if (li >= kl.n || key > last || (key < from && key >= a.sinks)) s[mt][r] = -INFINITY;
-      }
+      for (int r = 0; r < 16; ++r)
+        if (mt * 32 + (r >> 2) * 8 + (r & 3) > end) s[mt][r] = -INFINITY;
+    const int li0 = (tile0 + step) * kCacheTile;
+    if (a.window > 0 && li0 + kl.gap <= pos1 - a.window) {  // wave-uniform: the window of some row begins in the tile, or behind it
+      asm volatile("");
+      const int begin = from - base, sinks = a.sinks - base;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int c = mt * 32 + (r >> 2) * 8 + (r & 3);
+          if (c < begin && c >= sinks) s[mt][r] = -INFINITY;
+        }
+    }
   };
   auto tile_max = [&](const float16v (&s)[2]) {
     float mx = -INFINITY;
@@ -398,8 +409,12 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
     float16v sa[2], sb[2];
     if (0 < nact) {
       zero(sa);
+      half8v kf[NKF];  // (all reads on their way before the first product waits for one)
 #pragma unroll
-      for (int j = 0; j < NKF; ++j) sa[j % 2] = mfma32(read_kf(0, j), qf[j / 2], sa[j % 2]);
+      for (int j = 0; j < NKF; ++j) kf[j] = read_kf(0, j);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NKF; ++j) sa[j % 2] = mfma32(kf[j], qf[j / 2], sa[j % 2]);
       if (need_mask(0)) {
         asm volatile("");
         apply_mask(sa, 0);
@@ -592,7 +607,7 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
     // ---- mask: needed where the list ends, a token's keys end, or the window of a later token has begun
     const int li0 = tile * kFewRowTile, li1 = li0 + kFewRowTile - 1;
     const bool masked = li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0) ||
-                        (a.window > 0 && li0 + (li0 < kl.sinks ? 0 : kl.gap) <= pos1 - a.window && li1 >= a.sinks);
+                        (a.window > 0 && li0 + kl.gap <= pos1 - a.window && li1 >= a.sinks);
     half8v pf[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -601,11 +616,11 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int li = li0 + kb * 16 + g * 4 + r, key = li + (li < kl.sinks ? 0 : kl.gap);
-            if (li >= kl.n || pos[nt] < 0 || (a.causal && key > pos[nt]) ||
-                (a.window > 0 && key <= pos[nt] - a.window && key >= a.sinks))
-              st[nt][kb][r] = -INFINITY;
+          for (int r = 0; r < 4; ++r) {  // (visible: see the kernel of many rows)
+            const int li = li0 + kb * 16 + g * 4 + r;
+            const int last = pos[nt] < 0 ? -1 : (a.causal ? pos[nt] - kl.gap : kl.n - 1);
+            const int from = a.window > 0 ? pos[nt] - a.window + 1 - kl.gap : 0;
+            if (li >= kl.n || li > last || (li < from && li >= a.sinks)) st[nt][kb][r] = -INFINITY;
           }
       }
       float mx = -INFINITY;
