@@ -26,10 +26,10 @@ constexpr int kCacheRows = 128;      // stacked rows per workgroup, 32 a wave
 // sums are rescaled rarely
 constexpr float kCacheLazyMax = 8.0f;
 
-// row / group, with the launcher's multiplier (a division takes forty instructions, and there is one per row that is stored)
-__device__ __forceinline__ int row_token(const CacheAttnArgs& a, int row) {
-  return (int)(__umulhi((uint32_t)row << 4, a.div_mul) >> a.div_sh);
-}
+// (divisions by what the launcher knows are multiplications: a division of integers takes forty instructions, one after the
+// other, and the place of a workgroup takes four)
+__device__ __forceinline__ int div_by(int n, CacheDiv d) { return (int)(__umulhi((uint32_t)n << 4, d.mul) >> d.sh); }
+__device__ __forceinline__ int row_token(const CacheAttnArgs& a, int row) { return div_by(row, a.by_group); }
 
 // what a row block of a sequence sees
 struct KeyList {
@@ -54,7 +54,7 @@ __device__ __forceinline__ KeyList key_list(const CacheAttnArgs& a, int b, int t
 // zeros and -inf)
 template <int D>
 __device__ __forceinline__ void store_row(const CacheAttnArgs& a, int b, int hk, int row, int d4, float m, float l, float4v acc) {
-  const int group = a.Hq / a.Hkv, tok = row_token(a, row), head = hk * group + row - tok * group;
+  const int tok = row_token(a, row), head = hk * a.group + row - tok * a.group;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   half4v hv;
 #pragma unroll
@@ -71,7 +71,7 @@ __device__ __forceinline__ void finish_row(const CacheAttnArgs& a, int b, int hk
     store_row<D>(a, b, hk, row, d4, m, l, acc);
     return;
   }
-  const int64_t rows = (int64_t)a.S * (a.Hq / a.Hkv), at = (((int64_t)b * a.Hkv + hk) * rows + row) * a.runs + run;
+  const int64_t rows = a.rows, at = (((int64_t)b * a.Hkv + hk) * rows + row) * a.runs + run;
   *reinterpret_cast<float4v*>(a.ws + at * D + d4 * 4) = acc;
   if (d4 == 0) {
     float* ps = a.ws + (int64_t)a.B * a.Hkv * rows * a.runs * D + at * 2;
@@ -90,18 +90,22 @@ struct CacheLds {
 
 // Workgroups go to the eight XCDs in turn, each with an L2 of its own: the row blocks of one KV head, which read the same
 // keys, stay on one XCD.  Per XCD the latest row blocks, which see most, come first.
-__device__ __forceinline__ void cache_wg_map(int id, int heads, int nrb, int runs, int& bh, int& rb, int& run) {
-  const int per = nrb * runs;
+__device__ __forceinline__ void cache_wg_map(const CacheAttnArgs& a, int id, int& b, int& hk, int& rb, int& run) {
+  const int heads = a.B * a.Hkv;
+  int bh;
   if (heads % 8 == 0) {
-    const int x = id % 8, s = id / 8, hx = heads / 8;
-    bh = x * hx + s % hx;
-    id = s / hx;
+    const int s = id >> 3, hx = heads >> 3;  // (by_heads: hx)
+    id = div_by(s, a.by_heads);
+    bh = (s - id * hx) * 8 + (int)(blockIdx.x & 7);  // (an XCD has heads of all sequences, the long ones and the short)
   } else {
-    bh = id / per;
-    id %= per;
+    id = div_by(id, a.by_heads);
+    bh = (int)blockIdx.x - id * heads;
   }
-  rb = nrb - 1 - id / runs;
-  run = id % runs;
+  const int back = a.runs == 1 ? id : div_by(id, a.by_runs);
+  rb = a.nrb - 1 - back;
+  run = id - back * a.runs;
+  b = a.B == 1 ? 0 : div_by(bh, a.by_hkv);
+  hk = bh - b * a.Hkv;
 }
 
 // ---------------------------------------------------------------------------------------------------- many rows
@@ -130,14 +134,13 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, g = lane >> 5;
-  const int group = a.Hq / a.Hkv, rows = a.S * group, nrb = (rows + kCacheRows - 1) / kCacheRows;
-  int bh, rb, run;
-  cache_wg_map((int)blockIdx.x, a.B * a.Hkv, nrb, a.runs, bh, rb, run);
-  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int group = a.group, rows = a.rows;
+  int b, hk, rb, run;
+  cache_wg_map(a, (int)blockIdx.x, b, hk, rb, run);
   const int r0 = rb * kCacheRows, w0 = r0 + wave * 32;
   const KeyList kl = key_list(a, b, row_token(a, r0), row_token(a, min(r0 + kCacheRows, rows) - 1));
   const int ntiles = (kl.n + kCacheTile - 1) / kCacheTile;
-  const int per = (ntiles + a.runs - 1) / a.runs, tile0 = min(run * per, ntiles);
+  const int per = div_by(ntiles + a.runs - 1, a.by_runs), tile0 = min(run * per, ntiles);
   const int nsteps = min(per, ntiles - tile0);
 
   const int row = w0 + l32, rowc = min(row, rows - 1);
@@ -171,8 +174,8 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
     const int li = min((tile0 + step) * kCacheTile + r, kl.n - 1);
     return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
   };
-  auto load16 = [&](int step, bool isv) {  // 16-bit: to LDS, 1 KB an instruction
-    half_t* const dst = (isv ? vt : kt) + (step & 1) * L::HALFS;
+  auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
+    half_t* const dst = (isv ? vt : kt) + buf * L::HALFS;
 #pragma unroll
     for (int i = 0; i < NPA; ++i) {
       const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
@@ -319,8 +322,8 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
     constexpr int PAR = decltype(parc)::value;
     meet();  // K(st + 1) and V(st) are there, K(st) and V(st - 1) retired
     if constexpr (!FP4) {
-      if (st + 2 < nsteps) load16(st + 2, false);
-      if (st + 1 < nsteps) load16(st + 1, true);
+      if (st + 2 < nsteps) load16(st + 2, false, PAR);
+      if (st + 1 < nsteps) load16(st + 1, true, PAR ^ 1);
     }
     auto commit_all = [&]() {
 #pragma unroll
@@ -401,11 +404,18 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
       fetch4(2, false);
       fetch4(1, true);
     } else {
-      load16(0, false);
-      if (1 < nsteps) load16(1, false);
-      load16(0, true);
+      load16(0, false, 0);
+      load16(0, true, 0);
+      load16(min(1, nsteps - 1), false, 1);  // (not under a condition: the wait below counts it)
     }
-    meet();
+    if constexpr (FP4) {
+      meet();
+    } else {  // K(0) is there, V(0) and K(1) may still be on their way
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * NPA));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
     float16v sa[2], sb[2];
     if (0 < nact) {
       zero(sa);
@@ -501,13 +511,12 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
   constexpr int KB = T::KB, KS = T::KS, DB = T::DB;
   const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int group = a.Hq / a.Hkv, rows = a.S * group;
-  int id = (int)blockIdx.x;
-  const int run = id % a.runs; id /= a.runs;
-  const int hk = id % a.Hkv, b = id / a.Hkv;
+  const int group = a.group, rows = a.rows;
+  const int bh = a.runs == 1 ? (int)blockIdx.x : div_by((int)blockIdx.x, a.by_runs), run = (int)blockIdx.x - bh * a.runs;
+  const int b = a.B == 1 ? 0 : div_by(bh, a.by_hkv), hk = bh - b * a.Hkv;
   const KeyList kl = key_list(a, b, 0, a.S - 1);
   const int ntiles = (kl.n + kFewRowTile - 1) / kFewRowTile;
-  const int per = (ntiles + a.runs - 1) / a.runs, tile0 = min(run * per, ntiles), tile1 = min(tile0 + per, ntiles);
+  const int per = div_by(ntiles + a.runs - 1, a.by_runs), tile0 = min(run * per, ntiles), tile1 = min(tile0 + per, ntiles);
 
   half8v qf[NT][KS];
   int pos[NT];
@@ -750,7 +759,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_few_kernel(CacheAttnArgs a)
 template <int D, int WAYS>
 __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
   constexpr int LPR = D / 4, LANES = 256 / WAYS, UNROLL = 8;
-  const int group = a.Hq / a.Hkv, rows = a.S * group;
+  const int rows = a.rows;
   const int64_t total = (int64_t)a.B * a.Hkv * rows;
   const int way = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   const int64_t idx = (int64_t)blockIdx.x * LANES + lane;
@@ -814,33 +823,61 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
 }
 
 // ---- which kernel, and in how many runs
-constexpr int kFewRowsMost = 32;        // stacked rows of a KV head, up to which the kernel of few rows runs
+constexpr int kFewRowsMost = 32;  // stacked rows of a KV head, up to which the kernel of few rows runs
+constexpr int kCacheMaxRuns = 64;
+// Few rows: as many runs as give 512 workgroups (eight waves a CU), of at least four tiles, one a wave (8 KV heads in 4 bits,
+// 512 / 256 / 1024 workgroups: 32 sequences of 8192 keys 41.0 / 54.6 / 41.1 us, 8 of 4000 11.7 / 13.1 / 14.5; one of 4096, 128 /
+// 64 / 256 keys a run 7.5 / 8.9 / 7.9).
+constexpr int kFewRowWorkgroups = 512, kFewRowKeys = 4 * kFewRowTile;
+// Many rows: what a call takes in us, fitted over sixteen calls of 71 to 65536 rows in 1 to 64 runs: a tile alone on its CU and
+// beside another workgroup's, fixed costs with and without the merge, and the partial results' way to memory and back
+// (8 KV heads, 64 tokens against 2000 keys in 4 / 8 / 16 / 32 runs 21.1 / 18.5 / 21.7 / 30.5 us; 512 against 16512 in 2 / 4 / 8
+// 202 / 164 / 175; 71 heads on one, one token against 8000 in 16 / 32 / 64 15.6 / 11.8 / 10.3).
+constexpr float kTileAloneUs = 1.2f, kTileBesideUs = 2.0f, kTileFixedUs = 5.0f, kTileMergeUs = 7.8f, kTilePartBytesPerUs = 4.1e6f;
+constexpr int kTileRound = 512;  // workgroups at a time, two a CU
+
 struct CachePlan {
-  int nt;       // few rows: column tiles of 16 rows (0: the tile kernel)
+  int nt;       // few rows: column tiles of 16 rows (0: the kernel of many rows)
   int runs;
   int64_t nwg;  // workgroups per run
 };
-static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int kv_len, int window, int sinks) {
-  const int rows = S * (Hq / Hkv);
+static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks) {
+  const int group = Hq / Hkv, rows = S * group;
+  const int64_t heads = (int64_t)B * Hkv;
   CachePlan p;
   p.nt = rows <= kFewRowsMost ? (rows + 15) / 16 : 0;
-  p.nwg = p.nt > 0 ? (int64_t)Hkv * B : (int64_t)((rows + kCacheRows - 1) / kCacheRows) * Hkv * B;
+  p.nwg = p.nt > 0 ? heads : (rows + kCacheRows - 1) / kCacheRows * heads;
   // most keys of a row block
-  const int64_t toks = p.nt > 0 ? S : (kCacheRows + Hq / Hkv - 1) / (Hq / Hkv) + 1;
+  const int64_t toks = p.nt > 0 ? S : (kCacheRows + group - 1) / group + 1;
   int64_t keys = kv_len;
   if (window > 0 && toks + window + sinks < keys) keys = toks + window + sinks;
-  const int64_t least = p.nt > 0 ? 4 * kFewRowTile : 4 * kCacheTile;  // keys per run
-  int64_t runs = 512 / p.nwg;
-  if (runs > keys / least) runs = keys / least;
-  if (runs > 64) runs = 64;
-  p.runs = runs < 1 ? 1 : (int)runs;
+  if (p.nt > 0) {
+    int64_t runs = kFewRowWorkgroups / p.nwg;
+    if (runs > keys / kFewRowKeys) runs = keys / kFewRowKeys;
+    p.runs = (int)(runs < 1 ? 1 : (runs > kCacheMaxRuns ? kCacheMaxRuns : runs));
+    return p;
+  }
+  const int64_t tiles = (keys + kCacheTile - 1) / kCacheTile;
+  const int64_t most = tiles < kCacheMaxRuns ? tiles : kCacheMaxRuns;
+  const float part_us = (float)(heads * rows) * (float)D * 8.f / kTilePartBytesPerUs;
+  float best = 0.f;
+  p.runs = 1;
+  for (int r = 1; r <= most && (r == 1 || p.nwg * r <= 4 * kTileRound); ++r) {
+    const int64_t wgs = p.nwg * r, per = (tiles + r - 1) / r;
+    const float steps = wgs <= kTileRound / 2 ? kTileAloneUs : kTileBesideUs * (float)((wgs + kTileRound - 1) / kTileRound);
+    const float us = (float)per * steps + (r == 1 ? kTileFixedUs : kTileMergeUs + (float)r * part_us);
+    if (r == 1 || us < best) {
+      best = us;
+      p.runs = r;
+    }
+  }
   return p;
 }
 
 static int64_t run_bytes(int B, int S, int Hq, int D) { return (int64_t)B * S * Hq * (D + 2) * 4; }
 
 int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool /*four_bit*/) {
-  const int runs = cache_plan(B, S, Hq, Hkv, kv_len, window, sinks).runs;
+  const int runs = cache_plan(B, S, Hq, Hkv, D, kv_len, window, sinks).runs;
   return runs > 1 ? runs * run_bytes(B, S, Hq, D) : 0;
 }
 
@@ -860,14 +897,26 @@ static void launch_merge(const CacheAttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((cache_merge_kernel<D, 1>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a);
 }
 
+static CacheDiv cache_div(int d) {
+  CacheDiv r{0, 0};
+  while (((int64_t)1 << r.sh) < d) ++r.sh;
+  r.mul = (uint32_t)((((uint64_t)1 << (28 + r.sh)) + d - 1) / d);
+  return r;
+}
+
 int launch_cache_attention(const CacheAttnArgs& args, hipStream_t stream) {
-  CacheAttnArgs a = args;  // (div_sh: 0)
-  const CachePlan p = cache_plan(a.B, a.S, a.Hq, a.Hkv, a.kv_len, a.window, a.sinks);
+  CacheAttnArgs a = args;
+  const CachePlan p = cache_plan(a.B, a.S, a.Hq, a.Hkv, a.D, a.kv_len, a.window, a.sinks);
   const int64_t fit = a.ws != nullptr ? a.ws_bytes / run_bytes(a.B, a.S, a.Hq, a.D) : 0;
   a.runs = (int)(fit < p.runs ? (fit < 1 ? 1 : fit) : p.runs);
-  const uint32_t group = (uint32_t)(a.Hq / a.Hkv);
-  while ((1u << a.div_sh) < group) ++a.div_sh;
-  a.div_mul = (uint32_t)((((uint64_t)1 << (28 + a.div_sh)) + group - 1) / group);
+  a.group = a.Hq / a.Hkv;
+  a.rows = a.S * a.group;
+  a.nrb = p.nt > 0 ? 1 : (a.rows + kCacheRows - 1) / kCacheRows;
+  const int heads = a.B * a.Hkv;
+  a.by_group = cache_div(a.group);
+  a.by_runs = cache_div(a.runs);
+  a.by_hkv = cache_div(a.Hkv);
+  a.by_heads = cache_div(heads % 8 == 0 ? heads / 8 : heads);
   const unsigned nwg = (unsigned)(p.nwg * a.runs);
   const bool fp4 = a.kc.scales != nullptr;
   if (a.D == 128) fp4 ? launch_t<128, true>(a, p.nt, nwg, stream) : launch_t<128, false>(a, p.nt, nwg, stream);

@@ -279,6 +279,10 @@ struct CacheRowsArgs {
 int launch_cache_append(const CacheRowsArgs& a, hipStream_t stream);
 int launch_cache_read(const CacheRowsArgs& a, hipStream_t stream);
 
+// n / d = umulhi(16 n, mul) >> sh for n < 2^28
+struct CacheDiv {
+  uint32_t mul, sh;
+};
 struct CacheAttnArgs {
   const half_t* q;  // [B * S, Hq * D]
   int64_t ldq;
@@ -292,9 +296,10 @@ struct CacheAttnArgs {
   int causal, window, sinks;
   float* ws;  // nullable: partial results of the runs
   int64_t ws_bytes;
-  // set by the launcher: parts that a row block's keys are cut into; n / (Hq / Hkv) = (umulhi(16 n, div_mul) >> div_sh) below 2^28
-  int runs;
-  uint32_t div_mul, div_sh;
+  // set by the launcher: stacked rows of a KV head and its query heads, row blocks, parts that a row block's keys are cut into,
+  // and the divisors that a workgroup's place and a row's token come from
+  int rows, group, nrb, runs;
+  CacheDiv by_group, by_runs, by_hkv, by_heads;  // (by_heads: KV heads of all sequences, or an eighth of them)
 };
 int launch_cache_attention(const CacheAttnArgs& a, hipStream_t stream);
 int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
