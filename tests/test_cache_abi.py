@@ -159,5 +159,10 @@ def test_class_refuses():
         blocks.CachedAttention(Hq, Hkv, 96).attend(_h(B * S, Hq * 96), _h(B, Hkv, L, 96), _h(B, Hkv, L, 96))
     with pytest.raises(ext.TrinityError):
         blocks.CachedAttention(Hq, Hkv, D, causal=False, window=8).attend(_h(B * S, Hq * D), _h(B, Hkv, L, D), _h(B, Hkv, L, D))
+    with pytest.raises(ValueError):
+        op.read(_h(B, Hkv, L, D), _h(B, Hkv, L, D), dtype=torch.bfloat16)
+    c, x = _four()
+    with pytest.raises(ValueError):
+        op.read(c, c, x, x, dtype=torch.float32)
     codes, scales = op.make_cache(2, Hkv, 7, D, "cpu")
     assert codes.shape == (2, Hkv, 7, 64) and scales.shape == (2, Hkv, 7, 4)

@@ -116,59 +116,51 @@ class CachedAttention:
         return (torch.zeros(batch, n_kv_heads, rows, head_dim // 2, dtype=torch.uint8, device=device),
                 torch.ones(batch, n_kv_heads, rows, head_dim // 32, dtype=torch.uint8, device=device))
 
-    def _params(self, what, batch, seq, kv_len, four_bit=False):
-        """Parameters and scratch size of a call; the last ones of a kind are kept, since most callers repeat a shape."""
-        key = (batch, seq, kv_len, four_bit, self.scale, self.causal, self.window, self.sinks)
+    def _params(self, what, k_cache, rows, kv_len, four_bit=False):
+        """Parameters and scratch size of a call with `rows` rows; the last ones of a kind are kept, since most callers repeat a
+        shape."""
+        key = (k_cache.shape, rows, kv_len, four_bit, self.scale, self.causal, self.window, self.sinks)
         last = self._last.get(what)
         if last is None or last[0] != key:
-            p = ext.cache_params(batch, self.n_kv_heads, self.head_dim, seq, kv_len, n_q_heads=self.n_q_heads,
-                                 scale=self.scale, causal=self.causal, window=self.window, sinks=self.sinks)
+            batch = k_cache.shape[0] if k_cache.dim() == 4 else 1
+            if what != "read":  # (`read`: rows of each sequence)
+                if batch and rows % batch:
+                    raise ValueError("%d rows are not as many for each of %d sequences" % (rows, batch))
+                rows = rows // batch if batch else 0
+            p = ext.cache_params(batch, self.n_kv_heads, self.head_dim, rows, k_cache.shape[-2] if kv_len is None else kv_len,
+                                 n_q_heads=self.n_q_heads, scale=self.scale, causal=self.causal, window=self.window,
+                                 sinks=self.sinks)
             need = ext.cache_scratch_bytes(p, four_bit) if what == "attend" else 0
             self._last[what] = last = (key, p, need)
         return last[1], last[2]
 
-    @staticmethod
-    def _sizes(k_cache, kv_len):
-        batch = k_cache.shape[0] if k_cache.dim() == 4 else 1
-        return batch, (k_cache.shape[-2] if kv_len is None else kv_len)
-
-    @staticmethod
-    def _seq(rows, batch):
-        if batch and rows % batch:
-            raise ValueError("%d rows are not as many for each of %d sequences" % (rows, batch))
-        return rows // batch if batch else 0
-
     def append(self, K, V, k_cache, v_cache, k_scales=None, v_scales=None, lens=None, kv_len=None):
         """K, V [batch * tokens, KV heads * head_dim] to the last rows of their sequences."""
-        batch, kv_len = self._sizes(k_cache, kv_len)
-        p, _ = self._params("append", batch, self._seq(K.shape[0], batch), kv_len)
+        p, _ = self._params("append", k_cache, K.shape[0], kv_len)
         ext.cache_append(K, V, k_cache, k_scales, v_cache, v_scales, lens, p)
 
     def read(self, k_cache, v_cache, k_scales=None, v_scales=None, dtype=None, rows=None, lens=None, kv_len=None):
         """The last `rows` rows of every sequence (None: `kv_len`) as k, v [batch, KV heads, rows, head_dim]; zeros where a
         sequence has fewer."""
-        batch, kv_len = self._sizes(k_cache, kv_len)
-        rows = kv_len if rows is None else rows
-        if dtype is None:
-            dtype = k_cache.dtype if k_scales is None else torch.float16
-        p, _ = self._params("read", batch, rows, kv_len)
-        k, v = (torch.empty(batch, self.n_kv_heads, rows, self.head_dim, dtype=dtype, device=k_cache.device) for _ in range(2))
-        ext.cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, p)
-        return k, v
+        if k_scales is None:
+            if dtype is not None and dtype != k_cache.dtype:
+                raise ValueError("rows of a 16-bit cache are read as they are, %s" % k_cache.dtype)
+            dtype = k_cache.dtype
+        elif dtype not in (None, torch.float16, torch.bfloat16):
+            raise ValueError("rows are read as float16 or bfloat16")
+        if rows is None:
+            rows = k_cache.shape[-2] if kv_len is None else kv_len
+        p, _ = self._params("read", k_cache, rows, kv_len)
+        return ext.cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, dtype is torch.bfloat16, p)
 
     def attend(self, Q, k_cache, v_cache, k_scales=None, v_scales=None, lens=None, kv_len=None, out=None, want_lse=False):
         """Q [batch * tokens, query heads * head_dim] over the caches, which hold the tokens' own keys already.  Returns
         the output like Q, and with `want_lse` the log-sum-exp [batch, query heads, tokens] beside it."""
-        batch, kv_len = self._sizes(k_cache, kv_len)
-        seq = self._seq(Q.shape[0], batch)
-        p, need = self._params("attend", batch, seq, kv_len, k_scales is not None)
-        if need and (self._scratch is None or self._scratch.numel() < need or self._scratch.device != Q.device):
-            self._scratch = torch.empty(need, dtype=torch.uint8, device=Q.device)
-        if out is None:
-            out = torch.empty(Q.shape[0], self.n_q_heads * self.head_dim, dtype=Q.dtype, device=Q.device)
-        lse = torch.empty(batch, self.n_q_heads, seq, dtype=torch.float32, device=Q.device) if want_lse else None
-        ext.cache_attention(Q, k_cache, k_scales, v_cache, v_scales, lens, self._scratch if need else None, lse, out, p)
-        return (out, lse) if want_lse else out
+        p, need = self._params("attend", k_cache, Q.shape[0], kv_len, k_scales is not None)
+        scratch = self._scratch if need else None
+        if need and (scratch is None or scratch.numel() < need or scratch.device != Q.device):
+            self._scratch = scratch = torch.empty(need, dtype=torch.uint8, device=Q.device)
+        return ext.cache_attention_new(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, p)
 
 
 class FfnBlockPlan:

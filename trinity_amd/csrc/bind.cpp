@@ -7,6 +7,7 @@
 // Every function takes the tensors (or descriptors of them) in the order of the C entry point (None where it allows
 // NULL), then its scalars, then the stream as an integer, and returns the status; trinity_amd/ext.py turns a status into
 // an exception.
+#include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -274,6 +275,107 @@ TRI_BIND(cache_attention) {
 }
 #undef TRI_BIND
 
+// The two calls of blocks.CachedAttention that return new tensors make them here: torch.empty from Python takes as long as the
+// rest of a call without its launch.  They return what they made, or the status as an integer.
+at::Tensor new_tensor(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::empty(sizes, like.options().dtype(type));
+}
+template <class F>
+PyObject* run_new(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// (k_cache, k_scales, v_cache, v_scales, lens, whether in bfloat16, parameters, stream) -> (k, v)
+PyObject* cache_read_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 5, 2, t)) return nullptr;
+    const OneDevice device(a, 5);
+    const CacheParams p(a[6]);
+    void* s = stream_of(a[7]);
+    const int bf16 = PyObject_IsTrue(a[5]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    if (!THPVariable_Check(a[0])) return PyErr_Format(PyExc_TypeError, "the cache has to be a tensor");
+    const at::Tensor& c = THPVariable_Unpack(a[0]);
+    const int64_t sizes[4] = {p.p->batch, p.p->n_kv_heads, p.p->seq, p.p->head_dim};
+    at::Tensor out[2];
+    tri_tensor d[2];
+    for (int i = 0; i < 2; ++i) {
+      out[i] = new_tensor(c, sizes, bf16 != 0 ? at::kBFloat16 : at::kHalf);
+      d[i].ptr = out[i].data_ptr();
+      d[i].ndim = 4;
+      d[i].dtype = bf16 != 0 ? TRI_BF16 : TRI_F16;
+      for (int j = 0; j < 4; ++j) {
+        d[i].shape[j] = sizes[j];
+        d[i].stride[j] = out[i].stride(j);
+      }
+    }
+    const int st = call([&] { return tri_cache_read(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], &d[0], &d[1], p.p, s); });
+    if (st != 0) return PyLong_FromLong(st);
+    PyObject *const k = THPVariable_Wrap(out[0]), *const v = THPVariable_Wrap(out[1]);
+    PyObject* const r = k != nullptr && v != nullptr ? PyTuple_Pack(2, k, v) : nullptr;
+    Py_XDECREF(k);
+    Py_XDECREF(v);
+    return r;
+  });
+}
+
+// (q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out or None, want_lse, parameters, stream) -> out, or (out, lse)
+PyObject* cache_attention_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 8, 2, t)) return nullptr;
+    const OneDevice device(a, 8);
+    const CacheParams p(a[9]);
+    void* s = stream_of(a[10]);
+    const int want_lse = PyObject_IsTrue(a[8]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    if (!THPVariable_Check(a[0])) return PyErr_Format(PyExc_TypeError, "q has to be a tensor");
+    const at::Tensor& q = THPVariable_Unpack(a[0]);
+    at::Tensor made, lse;
+    tri_tensor o, l;
+    tri_tensor *out = t.p[7], *lp = nullptr;
+    if (out == nullptr) {
+      const int64_t cols = (int64_t)p.p->n_q_heads * p.p->head_dim;
+      made = new_tensor(q, {q.size(0), cols}, q.scalar_type());
+      o.ptr = made.data_ptr();
+      o.ndim = 2;
+      o.dtype = t.p[0]->dtype;
+      o.shape[0] = q.size(0); o.shape[1] = cols; o.stride[0] = cols; o.stride[1] = 1;
+      out = &o;
+    }
+    if (want_lse != 0) {
+      const int64_t sizes[3] = {p.p->batch, p.p->n_q_heads, p.p->seq};
+      lse = new_tensor(q, sizes, at::kFloat);
+      l.ptr = lse.data_ptr();
+      l.ndim = 3;
+      l.dtype = TRI_F32;
+      for (int j = 0; j < 3; ++j) {
+        l.shape[j] = sizes[j];
+        l.stride[j] = lse.stride(j);
+      }
+      lp = &l;
+    }
+    const int st = call([&] {
+      return tri_cache_attention(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], lp, out, p.p, s);
+    });
+    if (st != 0) return PyLong_FromLong(st);
+    PyObject* r = made.defined() ? THPVariable_Wrap(made) : a[7];
+    if (!made.defined()) Py_INCREF(r);
+    if (r == nullptr || want_lse == 0) return r;
+    PyObject* const x = THPVariable_Wrap(lse);
+    PyObject* const both = x != nullptr ? PyTuple_Pack(2, r, x) : nullptr;
+    Py_DECREF(r);
+    Py_XDECREF(x);
+    return both;
+  });
+}
+
 PyObject* cache_scratch_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) return PyErr_Format(PyExc_TypeError, "expected 2 arguments, got %zd", n);
   const CacheParams p(a[0]);
@@ -305,7 +407,8 @@ PyMethodDef methods[] = {
     TRI_METHOD("gemm_workspace_bytes", workspace_bytes<tri_gemm_workspace_bytes>),
     TRI_METHOD("ffn_workspace_bytes", workspace_bytes<tri_ffn_workspace_bytes>),
     TRI_METHOD("cache_append", cache_append), TRI_METHOD("cache_read", cache_read),
-    TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
+    TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_read_new", cache_read_new),
+    TRI_METHOD("cache_attention_new", cache_attention_new), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

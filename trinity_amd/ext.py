@@ -367,6 +367,22 @@ def cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse,
     return st
 
 
+def cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, bf16, params):
+    """cache_read into new tensors [batch, KV heads, seq, head_dim]."""
+    r = native().cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, bf16, params, _stream_ptr(k_cache))
+    if type(r) is int:
+        _check("tri_cache_read", r)
+    return r
+
+
+def cache_attention_new(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, params):
+    """cache_attention into a new tensor where `out` is None: returns the output, and a new log-sum-exp beside it if wanted."""
+    r = native().cache_attention_new(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, params, _stream_ptr(q))
+    if type(r) is int:
+        _check("tri_cache_attention", r)
+    return r
+
+
 def issue_probe(with_mfma, n_valu, n_trans, waves_per_simd, iters=4096, workgroups=256, device="cuda:0"):
     """tri_diag_issue_probe: (s_memtime ticks, nanoseconds) per group of one MFMA (or none), n_valu v_fma_f32 and
     n_trans v_exp_f32, from a workgroup's start to the end of its last wave, averaged over the workgroups (one per
