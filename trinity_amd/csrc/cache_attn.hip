@@ -537,34 +537,70 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
   const uint8_t* const kxbase = FP4 ? a.kc.scales + b * a.kc.xb + hk * a.kc.xh : nullptr;
   const uint8_t* const vxbase = FP4 ? a.vc.scales + b * a.vc.xb + hk * a.vc.xh : nullptr;
   const int64_t ksr = a.kc.sr * ES, vsr = a.vc.sr * ES;
+  // one row of K, one piece of V: the tile's place (kp, kxp, vp, vxp) and the offsets of a lane in it, of either width
+  auto fetch_k = [&](T& x, int kb, const uint8_t* kp, const uint8_t* kxp, auto off, auto xoff) __attribute__((always_inline)) {
+    if constexpr (FP4) {
+      if constexpr (D == 128) {
+        x.k[kb][0] = *reinterpret_cast<const uint4v*>(kp + off);
+      } else {
+        const uint2v h = *reinterpret_cast<const uint2v*>(kp + off);
+        x.k[kb][0] = uint4v{h[0], h[1], 0u, 0u};
+      }
+      x.kx[kb] = kxp[xoff];
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x.k[kb][s] = *reinterpret_cast<const uint4v*>(kp + off + s * 64);
+    }
+  };
+  auto fetch_v = [&](T& x, int i, const uint8_t* vp, const uint8_t* vxp, auto off, auto xoff) __attribute__((always_inline)) {
+    x.v[i] = *reinterpret_cast<const uint4v*>(vp + off);
+    if constexpr (FP4) x.vx[i] = vxp[xoff];
+  };
+  // 4 bits: tiles of neighbouring rows (all but the list's last one and that with the end of the sinks) are addressed by the
+  // tile's place, the same for the wave, and fixed offsets; an address per row is two products of 64 bits, and there are eight
+  // of them to a tile (32 sequences of up to 8192 keys 41.2 -> 39.8 us; 16-bit tiles, four times the bytes, are 2 % slower so,
+  // and in the kernel of many rows it is level, too: that one is bound elsewhere)
+  const bool flat = FP4 && (uint64_t)ksr * kFewRowTile < (1u << 31) && (uint64_t)vsr * kFewRowTile < (1u << 31) &&
+                    (uint64_t)a.kc.xr * kFewRowTile < (1u << 31) && (uint64_t)a.vc.xr * kFewRowTile < (1u << 31);
+  constexpr int KPB = FP4 ? D / 8 : 16;  // bytes of a key that a lane takes at a time
+  uint32_t koff[KB], kxoff[KB], voff[T::VP], vxoff[T::VP];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    koff[kb] = (uint32_t)(kb * 16 + l16) * (uint32_t)ksr + g * KPB;
+    kxoff[kb] = FP4 ? (uint32_t)(kb * 16 + l16) * (uint32_t)a.kc.xr + (D == 128 ? g : g / 2) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < T::VP; ++i) {
+    const int p = i * 64 + lane, r = p / T::VPR, c = p % T::VPR;
+    voff[i] = (uint32_t)r * (uint32_t)vsr + c * 16;
+    vxoff[i] = FP4 ? (uint32_t)r * (uint32_t)a.vc.xr + c : 0;
+  }
   auto fetch = [&](int tile, T& x) __attribute__((always_inline)) {
+    const int li0 = tile * kFewRowTile;
+    if (flat && li0 + kFewRowTile <= kl.n && (kl.gap == 0 || li0 >= kl.sinks)) {  // wave-uniform
+      const int64_t key0 = li0 + kl.gap;
+      const uint8_t *kp = kbase + key0 * ksr, *vp = vbase + key0 * vsr;
+      const uint8_t *kxp = FP4 ? kxbase + key0 * a.kc.xr : nullptr, *vxp = FP4 ? vxbase + key0 * a.vc.xr : nullptr;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) fetch_k(x, kb, kp, kxp, koff[kb], kxoff[kb]);
+#pragma unroll
+      for (int i = 0; i < T::VP; ++i) fetch_v(x, i, vp, vxp, voff[i], vxoff[i]);
+      return;
+    }
     auto key_of = [&](int r) {  // (past the last key: the last one again, whose scores are masked)
-      const int li = min(tile * kFewRowTile + r, kl.n - 1);
+      const int li = min(li0 + r, kl.n - 1);
       return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
     };
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int64_t key = key_of(kb * 16 + l16);
-      const uint8_t* p = kbase + key * ksr;
-      if constexpr (FP4) {
-        if constexpr (D == 128) {
-          x.k[kb][0] = *reinterpret_cast<const uint4v*>(p + g * 16);
-        } else {
-          const uint2v h = *reinterpret_cast<const uint2v*>(p + g * 8);
-          x.k[kb][0] = uint4v{h[0], h[1], 0u, 0u};
-        }
-        x.kx[kb] = kxbase[key * a.kc.xr + (D == 128 ? g : g / 2)];
-      } else {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) x.k[kb][s] = *reinterpret_cast<const uint4v*>(p + s * 64 + g * 16);
-      }
+      fetch_k(x, kb, kbase, kxbase, key * ksr + g * KPB, FP4 ? key * a.kc.xr + (D == 128 ? g : g / 2) : 0);
     }
 #pragma unroll
     for (int i = 0; i < T::VP; ++i) {
       const int p = i * 64 + lane, r = p / T::VPR, c = p % T::VPR;
       const int64_t key = key_of(r);
-      x.v[i] = *reinterpret_cast<const uint4v*>(vbase + key * vsr + c * 16);
-      if constexpr (FP4) x.vx[i] = vxbase[key * a.vc.xr + c];
+      fetch_v(x, i, vbase, vxbase, key * vsr + c * 16, FP4 ? key * a.vc.xr + c : 0);
     }
   };
 
@@ -829,6 +865,11 @@ constexpr int kCacheMaxRuns = 64;
 // 512 / 256 / 1024 workgroups: 32 sequences of 8192 keys 41.0 / 54.6 / 41.1 us, 8 of 4000 11.7 / 13.1 / 14.5; one of 4096, 128 /
 // 64 / 256 keys a run 7.5 / 8.9 / 7.9).
 constexpr int kFewRowWorkgroups = 512, kFewRowKeys = 4 * kFewRowTile;
+// ... but one run where it is so short that the merge takes longer than what the runs spare, and a launch: up to five tiles a
+// wave in 4 bits, three in 16, or eight where the KV heads alone are half a round of workgroups (8 KV heads, one run / several,
+// one sequence in 4 bits of 512 keys 6.5 / 7.0, 768 7.9 / 7.2, in 16 bits of 384 7.3 / 7.5, 512 8.5 / 7.3; sixteen of 768 8.7 / 9.0 and
+// 11.9 / 12.2, of 1500 13.0 / 10.3 and 18.7 / 18.4; graph replays, eager calls gain another 2.7 us of host time).
+constexpr int kFewRowAlone4 = 5, kFewRowAlone16 = 3, kFewRowAloneMany = 8, kFewRowManyHeads = 128;
 // Many rows: what a call takes in us, fitted over sixteen calls of 71 to 65536 rows in 1 to 64 runs: a tile alone on its CU and
 // beside another workgroup's, fixed costs with and without the merge, and the partial results' way to memory and back
 // (8 KV heads, 64 tokens against 2000 keys in 4 / 8 / 16 / 32 runs 21.1 / 18.5 / 21.7 / 30.5 us; 512 against 16512 in 2 / 4 / 8
@@ -841,7 +882,7 @@ struct CachePlan {
   int runs;
   int64_t nwg;  // workgroups per run
 };
-static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks) {
+static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit) {
   const int group = Hq / Hkv, rows = S * group;
   const int64_t heads = (int64_t)B * Hkv;
   CachePlan p;
@@ -854,6 +895,8 @@ static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, in
   if (p.nt > 0) {
     int64_t runs = kFewRowWorkgroups / p.nwg;
     if (runs > keys / kFewRowKeys) runs = keys / kFewRowKeys;
+    const int alone = p.nwg >= kFewRowManyHeads ? kFewRowAloneMany : (four_bit ? kFewRowAlone4 : kFewRowAlone16);
+    if (keys <= alone * kFewRowKeys) runs = 1;
     p.runs = (int)(runs < 1 ? 1 : (runs > kCacheMaxRuns ? kCacheMaxRuns : runs));
     return p;
   }
@@ -876,8 +919,8 @@ static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, in
 
 static int64_t run_bytes(int B, int S, int Hq, int D) { return (int64_t)B * S * Hq * (D + 2) * 4; }
 
-int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool /*four_bit*/) {
-  const int runs = cache_plan(B, S, Hq, Hkv, D, kv_len, window, sinks).runs;
+int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit) {
+  const int runs = cache_plan(B, S, Hq, Hkv, D, kv_len, window, sinks, four_bit).runs;
   return runs > 1 ? runs * run_bytes(B, S, Hq, D) : 0;
 }
 
@@ -906,7 +949,7 @@ static CacheDiv cache_div(int d) {
 
 int launch_cache_attention(const CacheAttnArgs& args, hipStream_t stream) {
   CacheAttnArgs a = args;
-  const CachePlan p = cache_plan(a.B, a.S, a.Hq, a.Hkv, a.D, a.kv_len, a.window, a.sinks);
+  const CachePlan p = cache_plan(a.B, a.S, a.Hq, a.Hkv, a.D, a.kv_len, a.window, a.sinks, a.kc.scales != nullptr);
   const int64_t fit = a.ws != nullptr ? a.ws_bytes / run_bytes(a.B, a.S, a.Hq, a.D) : 0;
   a.runs = (int)(fit < p.runs ? (fit < 1 ? 1 : fit) : p.runs);
   a.group = a.Hq / a.Hkv;
