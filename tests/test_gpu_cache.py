@@ -6,9 +6,11 @@ import math
 import pytest
 import torch
 
+import oracle
 from cache_util import assert_within, attention_tolerance, make_caches, values
 from oracle import cache as oc
 from trinity_amd import blocks, ext
+from util import assert_close, attn_inputs
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -133,6 +135,9 @@ ATTN = [
     (1, 7, 12, 2, 64, 3000, 2900, None, True, 0, 0),
     (1, 8, 8, 2, 128, 5000, 5000, None, False, 0, 0),
     (1, 512, 4, 1, 64, 1500, 1500, None, True, 0, 0),
+    (1, 1, 8, 2, 128, 640, 640, None, True, 0, 0),             # few rows: one run in 4 bits, several in 16
+    (33, 1, 4, 4, 64, 1300, 1300, [1300 - 40 * i for i in range(33)], True, 0, 0),  # many heads: 1024 keys and fewer in one run
+    (33, 1, 4, 4, 64, 900, 900, [900 - 27 * i for i in range(33)], True, 0, 0),
 ]
 
 
@@ -302,6 +307,61 @@ def test_prompt_then_tokens(dev, four_bit, window, sinks):
         want, wlse, mag = oc.cache_attention(q, hist[0], hist[1], n, n_q_heads=Hq, window=window, sinks=sinks)
         tol, tol_lse = attention_tolerance(q, hist[0], hist[1], n, mag, want, dtype, n_q_heads=Hq, scale=D ** -0.5)
         _check(got, lse, want, wlse, tol, tol_lse)
+
+
+@pytest.mark.parametrize("S,P,prenorm,qknorm", [(48, 0, False, False), (1, 300, True, False), (7, 90, True, True), (130, 60, False, True)])
+def test_plan_is_the_block(dev, S, P, prenorm, qknorm):
+    """One sequence, 16-bit, no window: the block of tri_qkv_attention (blocks.AttentionPlan) and its oracle.  The plans
+    round the same values (q, k, v, the normalised x) to 16 bits and differ in the order of their sums: 1e-2 as for the block."""
+    N, Hq, Hkv, D = 256, 4, 2, 128
+    t = attn_inputs(S, N, Hq, Hkv, D, P=P, w_std=0.06, with_cache=True)
+    want = oracle.qkv_attention(t["x"], t["wq"], t["wk"], t["wv"], n_q_heads=Hq, n_kv_heads=Hkv, head_dim=D, scale=D ** -0.5,
+                                causal=True, kv_prefix=P, k_cache=t["k_cache"], v_cache=t["v_cache"], prenorm=prenorm,
+                                prenorm_weight=t["norm_w"] if prenorm else None, qknorm=qknorm, rms_eps=1e-5, want_lse=True)
+    d = {k: v.to(dev) for k, v in t.items()}
+    kc, vc = d["k_cache"].clone()[None], d["v_cache"].clone()[None]
+    plan = blocks.CachedAttentionPlan(Hq, Hkv, D, prenorm=prenorm, qknorm=qknorm, eps=1e-5)
+    out = torch.full((S, Hq * D), math.nan, dtype=F16, device=dev)
+    got, lse = plan.run(d["x"], d["wq"], d["wk"], d["wv"], out, kc, vc, kv_len=P + S, norm_w=d["norm_w"] if prenorm else None,
+                        want_lse=True)
+    assert got is out
+    assert_close(out, want["O2"], 1e-2, 1e-2, "O2")
+    assert_close(lse[0], want["lse"], 1e-2, 1e-2, "lse")
+    assert_close(kc[0, :, P:P + S], want["k_new"], 1e-2, 1e-2, "appended k")
+    assert_close(vc[0, :, P:P + S], want["v_new"], 1e-2, 1e-2, "appended v")
+    assert torch.equal(kc[0, :, :P], d["k_cache"][:, :P])
+    other = torch.empty_like(out)
+    blocks.AttentionPlan("vanilla", D=D, H=Hq, P=P, prenorm=prenorm, qknorm=qknorm, scale=D ** -0.5, causal=True, n_kv_heads=Hkv,
+                         eps=1e-5).run(d["x"], d["wq"], d["wk"], d["wv"], other, d["k_cache"], d["v_cache"],
+                                       norm_w=d["norm_w"] if prenorm else None)
+    assert_close(out, other.cpu(), 1e-2, 1e-2, "the two blocks")
+
+
+def test_plan_over_ragged_four_bit_caches(dev):
+    """The block for three conversations, padded, in bf16 and a window: its attention is that over the cache it leaves behind."""
+    B, S, N, Hq, Hkv, D, rows = 3, 40, 192, 6, 2, 64, 90
+    lens = [90, 33, 5]
+    t = attn_inputs(B * S, N, Hq, Hkv, D, w_std=0.07)
+    t = {k: v.to(BF16) for k, v in t.items()}
+    d = {k: v.to(dev) for k, v in t.items()}
+    plan = blocks.CachedAttentionPlan(Hq, Hkv, D, window=25, sinks=2)
+    (kc, kx), (vc, vx) = (plan.attention.make_cache(B, Hkv, rows, D, dev) for _ in range(2))
+    before = make_caches(4, 1, Hkv, 50, D, BF16, True)
+    for new, old in zip((kc, vc, kx, vx), before):
+        new[0, :, :50] = old[0].to(dev)
+    out = plan.run(d["x"], d["wq"], d["wk"], d["wv"], torch.empty(B * S, Hq * D, dtype=BF16, device=dev), kc, vc, kx, vx,
+                   lens=_lens(lens, dev))
+    k, v = values(kc.cpu(), kx.cpu()), values(vc.cpu(), vx.cpu())
+    assert torch.equal(kc[0, :, :50].cpu(), before[0][0])
+    # the rows written: of k = x.wk in 16 bits, within a step of 4 bits of the exact product (its rounding may move a code)
+    exact = (t["x"].double() @ t["wk"].double()).view(B, S, Hkv, D).transpose(1, 2)
+    for b, n in enumerate(lens):
+        m = min(S, n)
+        unit = torch.ldexp(torch.ones(Hkv, m, D // 32, dtype=torch.float64), kx[b, :, n - m:n].cpu().long() - 127).repeat_interleave(32, -1)
+        assert bool(((k[b, :, n - m:n] - exact[b, :, S - m:]).abs() <= 1.1 * unit).all())
+    q = (t["x"].float() @ t["wq"].float()).to(BF16)
+    want, lse, mag = oc.cache_attention(q, k, v, lens, n_q_heads=Hq, window=25, sinks=2)
+    assert_close(out, want, 2e-2, 2e-2, "out")
 
 
 @pytest.mark.parametrize("four_bit", [False, True])
