@@ -159,6 +159,18 @@ def test_class_refuses():
         blocks.CachedAttention(Hq, Hkv, 96).attend(_h(B * S, Hq * 96), _h(B, Hkv, L, 96), _h(B, Hkv, L, 96))
     with pytest.raises(ext.TrinityError):
         blocks.CachedAttention(Hq, Hkv, D, causal=False, window=8).attend(_h(B * S, Hq * D), _h(B, Hkv, L, D), _h(B, Hkv, L, D))
+    for call in (lambda: op.attend(_h(B * S, Hq * D), _h(B, Hkv, L, D), _h(B, Hkv, L, D)),             # host memory
+                 lambda: op.append(_h(B * S, Hkv * D), _h(B * S, Hkv * D), _h(B, Hkv, L, D), _h(B, Hkv, L, D)),
+                 lambda: op.read(_h(B, Hkv, L, D), _h(B, Hkv, L, D)),
+                 lambda: ext.cache_append(_h(B * S, Hkv * D), _h(B * S, Hkv * D), _h(B, Hkv, L, D), None, _h(B, Hkv, L, D), None,
+                                          None, _params()),
+                 lambda: op.attend(_h(B * S, Hq * D), _h(B, Hkv, L, D), _h(B, Hkv, L, D), kv_len=1 << 40)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        op.attend(None, _h(B, Hkv, L, D), _h(B, Hkv, L, D))
+    with pytest.raises(TypeError):
+        op.append(_h(B * S, Hkv * D), _h(B * S, Hkv * D), None, None)
     with pytest.raises(ValueError):
         op.read(_h(B, Hkv, L, D), _h(B, Hkv, L, D), dtype=torch.bfloat16)
     c, x = _four()

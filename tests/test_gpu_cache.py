@@ -390,7 +390,7 @@ def test_graph_of_a_decode_step(dev, four_bit):
         step(op, out)
         step(win, out2)
     stream.synchronize()
-    win._scratch = op._scratch
+    win._scratch = op._scratch  # (the larger one: no window)
     lens.copy_(torch.tensor(start))
     for x, y in zip(c, caches):
         if x is not None:

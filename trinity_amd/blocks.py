@@ -105,9 +105,11 @@ class CachedAttention:
     with fewer has its first rows as padding.  `kv_len` (None: all rows of the cache) bounds the lengths."""
 
     def __init__(self, n_q_heads, n_kv_heads, head_dim, scale=None, causal=True, window=0, sinks=0):
-        self.n_q_heads, self.n_kv_heads, self.head_dim = n_q_heads, n_kv_heads, head_dim
-        self.scale, self.causal, self.window, self.sinks = scale, causal, window, sinks
-        self._last = {}
+        self.head_dim = head_dim
+        # (the sizes of a call are read off its tensors)
+        self._p = ext.cache_params(0, n_kv_heads, head_dim, 0, 0, n_q_heads=n_q_heads, scale=scale, causal=causal, window=window,
+                                   sinks=sinks)
+        self._native = ext.native()
         self._scratch = None
 
     @staticmethod
@@ -116,51 +118,41 @@ class CachedAttention:
         return (torch.zeros(batch, n_kv_heads, rows, head_dim // 2, dtype=torch.uint8, device=device),
                 torch.ones(batch, n_kv_heads, rows, head_dim // 32, dtype=torch.uint8, device=device))
 
-    def _params(self, what, k_cache, rows, kv_len, four_bit=False):
-        """Parameters and scratch size of a call with `rows` rows; the last ones of a kind are kept, since most callers repeat a
-        shape."""
-        key = (k_cache.shape, rows, kv_len, four_bit, self.scale, self.causal, self.window, self.sinks)
-        last = self._last.get(what)
-        if last is None or last[0] != key:
-            batch = k_cache.shape[0] if k_cache.dim() == 4 else 1
-            if what != "read":  # (`read`: rows of each sequence)
-                if batch and rows % batch:
-                    raise ValueError("%d rows are not as many for each of %d sequences" % (rows, batch))
-                rows = rows // batch if batch else 0
-            p = ext.cache_params(batch, self.n_kv_heads, self.head_dim, rows, k_cache.shape[-2] if kv_len is None else kv_len,
-                                 n_q_heads=self.n_q_heads, scale=self.scale, causal=self.causal, window=self.window,
-                                 sinks=self.sinks)
-            need = ext.cache_scratch_bytes(p, four_bit) if what == "attend" else 0
-            self._last[what] = last = (key, p, need)
-        return last[1], last[2]
-
     def append(self, K, V, k_cache, v_cache, k_scales=None, v_scales=None, lens=None, kv_len=None):
         """K, V [batch * tokens, KV heads * head_dim] to the last rows of their sequences."""
-        p, _ = self._params("append", k_cache, K.shape[0], kv_len)
-        ext.cache_append(K, V, k_cache, k_scales, v_cache, v_scales, lens, p)
+        st = self._native.cache_append_rows(K, V, k_cache, k_scales, v_cache, v_scales, lens, kv_len, self._p, ext._stream_or_none(K))
+        if st:
+            ext._check("tri_cache_append", st)
 
     def read(self, k_cache, v_cache, k_scales=None, v_scales=None, dtype=None, rows=None, lens=None, kv_len=None):
         """The last `rows` rows of every sequence (None: `kv_len`) as k, v [batch, KV heads, rows, head_dim]; zeros where a
-        sequence has fewer."""
+        sequence has fewer.  From 4 bits in float16 (None) or bfloat16."""
         if k_scales is None:
             if dtype is not None and dtype != k_cache.dtype:
                 raise ValueError("rows of a 16-bit cache are read as they are, %s" % k_cache.dtype)
             dtype = k_cache.dtype
         elif dtype not in (None, torch.float16, torch.bfloat16):
             raise ValueError("rows are read as float16 or bfloat16")
-        if rows is None:
-            rows = k_cache.shape[-2] if kv_len is None else kv_len
-        p, _ = self._params("read", k_cache, rows, kv_len)
-        return ext.cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, dtype is torch.bfloat16, p)
+        r = self._native.cache_read_rows(k_cache, k_scales, v_cache, v_scales, lens, rows, dtype is torch.bfloat16, kv_len,
+                                         self._p, ext._stream_or_none(k_cache))
+        if type(r) is int:
+            ext._check("tri_cache_read", r)
+        return r
 
     def attend(self, Q, k_cache, v_cache, k_scales=None, v_scales=None, lens=None, kv_len=None, out=None, want_lse=False):
         """Q [batch * tokens, query heads * head_dim] over the caches, which hold the tokens' own keys already.  Returns
         the output like Q, and with `want_lse` the log-sum-exp [batch, query heads, tokens] beside it."""
-        p, need = self._params("attend", k_cache, Q.shape[0], kv_len, k_scales is not None)
-        scratch = self._scratch if need else None
-        if need and (scratch is None or scratch.numel() < need or scratch.device != Q.device):
-            self._scratch = scratch = torch.empty(need, dtype=torch.uint8, device=Q.device)
-        return ext.cache_attention_new(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, p)
+        stream = ext._stream_or_none(Q)
+        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, self._scratch, out, want_lse, kv_len, self._p,
+                                      stream)
+        if type(r) is int:
+            if r > 0:  # bytes of scratch: the first call of its size
+                self._scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
+                r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, self._scratch, out, want_lse, kv_len,
+                                              self._p, stream)
+            if type(r) is int:
+                ext._check("tri_cache_attention", r)
+        return r
 
 
 class CachedAttentionPlan:

@@ -79,8 +79,8 @@ bool marshal(PyObject* const* args, Py_ssize_t nargs, int ntensors, int nscalars
   return true;
 }
 
-// The tensors of a call are on one device (a length or a scale read from host memory would fault the GPU), which is the
-// current one while the call launches.
+// The tensors of a call are on one GPU (a length or a scale read from host memory would fault it), which is the current one
+// while the call launches.
 struct OneDevice {
   c10::OptionalDeviceGuard guard;
   bool ok = true;
@@ -90,10 +90,10 @@ struct OneDevice {
       if (!THPVariable_Check(args[i])) continue;
       const at::Tensor& t = THPVariable_Unpack(args[i]);
       if (first == nullptr) first = &t;
-      ok = t.device() == first->device();
+      ok = t.is_cuda() && t.device() == first->device();
     }
-    if (!ok) PyErr_SetString(PyExc_ValueError, "the tensors of a call have to be on one device");
-    else if (first != nullptr && first->is_cuda()) guard.reset_device(first->device());
+    if (!ok) PyErr_SetString(PyExc_ValueError, "the tensors of a call have to be on one GPU");
+    else if (first != nullptr) guard.reset_device(first->device());
   }
 };
 
@@ -275,10 +275,59 @@ TRI_BIND(cache_attention) {
 }
 #undef TRI_BIND
 
-// The two calls of blocks.CachedAttention that return new tensors make them here: torch.empty from Python takes as long as the
-// rest of a call without its launch.  They return what they made, or the status as an integer.
+// ---- blocks.CachedAttention: the sizes of a call are read off its tensors here, and what it returns is made here - from
+// Python that takes as long as the rest of a call without its launch.  Each takes the heads and the mask as TriCacheParams,
+// its tensors, kv_len (None: all rows of the cache) and the stream; a status other than 0 is returned as an integer.
+struct CacheCall {
+  tri_cache_params p{};
+  bool ok = false;
+  // rows: of all sequences together, or (each) of every one
+  CacheCall(PyObject* params, PyObject* cache, int64_t rows, bool each, PyObject* kv_len) {
+    const CacheParams given(params);
+    if (PyErr_Occurred() != nullptr) return;
+    if (!THPVariable_Check(cache)) {
+      PyErr_Format(PyExc_TypeError, "the cache has to be a tensor, not %.100s", Py_TYPE(cache)->tp_name);
+      return;
+    }
+    const at::Tensor& c = THPVariable_Unpack(cache);
+    const int64_t batch = c.dim() == 4 ? c.size(0) : 1;
+    const int64_t len = kv_len != Py_None ? PyLong_AsLongLong(kv_len) : (c.dim() >= 2 ? c.size(-2) : 0);
+    if (PyErr_Occurred() != nullptr) return;
+    if (!each && batch > 0 && rows % batch != 0) {
+      PyErr_Format(PyExc_ValueError, "%lld rows are not as many for each of %lld sequences", (long long)rows, (long long)batch);
+      return;
+    }
+    const int64_t seq = each ? rows : (batch > 0 ? rows / batch : 0);
+    if (batch > INT32_MAX || seq > INT32_MAX || len > INT32_MAX || seq < INT32_MIN || len < INT32_MIN) {
+      PyErr_SetString(PyExc_ValueError, "sizes beyond 32 bits");
+      return;
+    }
+    p = *given.p;
+    p.batch = (int32_t)batch;
+    p.seq = (int32_t)seq;
+    p.kv_len = (int32_t)len;
+    ok = true;
+  }
+};
+
 at::Tensor new_tensor(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
   return at::empty(sizes, like.options().dtype(type));
+}
+tri_tensor describe(const at::Tensor& t, int32_t dtype) {
+  tri_tensor d{};
+  d.ptr = t.data_ptr();
+  d.ndim = (int32_t)t.dim();
+  d.dtype = dtype;
+  for (int i = 0; i < d.ndim; ++i) {
+    d.shape[i] = t.size(i);
+    d.stride[i] = t.stride(i);
+  }
+  return d;
+}
+const at::Tensor* tensor_of(PyObject* o, const char* what) {
+  if (THPVariable_Check(o)) return &THPVariable_Unpack(o);
+  PyErr_Format(PyExc_TypeError, "%s has to be a tensor, not %.100s", what, Py_TYPE(o)->tp_name);
+  return nullptr;
 }
 template <class F>
 PyObject* run_new(F f) {
@@ -290,32 +339,48 @@ PyObject* run_new(F f) {
   }
 }
 
-// (k_cache, k_scales, v_cache, v_scales, lens, whether in bfloat16, parameters, stream) -> (k, v)
-PyObject* cache_read_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// (k, v, k_cache, k_scales, v_cache, v_scales, lens, kv_len, parameters, stream) -> 0
+PyObject* cache_append_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return run_new([&]() -> PyObject* {
     Tensors t;
-    if (!marshal(a, n, 5, 2, t)) return nullptr;
-    const OneDevice device(a, 5);
-    const CacheParams p(a[6]);
-    void* s = stream_of(a[7]);
-    const int bf16 = PyObject_IsTrue(a[5]);
+    if (!marshal(a, n, 7, 2, t)) return nullptr;
+    const at::Tensor* const k = tensor_of(a[0], "k");
+    if (k == nullptr) return nullptr;
+    const CacheCall c(a[8], a[2], k->dim() > 0 ? k->size(0) : 0, false, a[7]);
+    if (!c.ok) return nullptr;
+    const OneDevice device(a, 7);
+    void* s = stream_of(a[9]);
     if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
-    if (!THPVariable_Check(a[0])) return PyErr_Format(PyExc_TypeError, "the cache has to be a tensor");
-    const at::Tensor& c = THPVariable_Unpack(a[0]);
-    const int64_t sizes[4] = {p.p->batch, p.p->n_kv_heads, p.p->seq, p.p->head_dim};
+    return PyLong_FromLong(call([&] { return tri_cache_append(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], &c.p, s); }));
+  });
+}
+
+// (k_cache, k_scales, v_cache, v_scales, lens, rows (None: kv_len), whether in bfloat16, kv_len, parameters, stream) -> (k, v)
+PyObject* cache_read_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 5, 4, t)) return nullptr;
+    const at::Tensor* const cache = tensor_of(a[0], "the cache");
+    if (cache == nullptr) return nullptr;
+    CacheCall c(a[8], a[0], a[5] != Py_None ? PyLong_AsLongLong(a[5]) : 0, true, a[7]);
+    if (!c.ok) return nullptr;
+    if (a[5] == Py_None) c.p.seq = c.p.kv_len;
+    const bool bf16 = PyObject_IsTrue(a[6]) == 1;
+    const OneDevice device(a, 5);
+    void* s = stream_of(a[9]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    // one allocation, the two halves of it as tensors (taking and returning memory costs a microsecond and a half a tensor)
+    const int64_t sizes[5] = {2, c.p.batch, c.p.n_kv_heads, c.p.seq < 0 ? 0 : c.p.seq, c.p.head_dim};
+    const at::Tensor both = new_tensor(*cache, sizes, bf16 ? at::kBFloat16 : at::kHalf);
     at::Tensor out[2];
     tri_tensor d[2];
     for (int i = 0; i < 2; ++i) {
-      out[i] = new_tensor(c, sizes, bf16 != 0 ? at::kBFloat16 : at::kHalf);
-      d[i].ptr = out[i].data_ptr();
-      d[i].ndim = 4;
-      d[i].dtype = bf16 != 0 ? TRI_BF16 : TRI_F16;
-      for (int j = 0; j < 4; ++j) {
-        d[i].shape[j] = sizes[j];
-        d[i].stride[j] = out[i].stride(j);
-      }
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), both.dtype());
+      out[i].unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(sizes + 1, 4));
+      out[i].unsafeGetTensorImpl()->set_storage_offset(i * (both.numel() / 2));
+      d[i] = describe(out[i], bf16 ? TRI_BF16 : TRI_F16);
     }
-    const int st = call([&] { return tri_cache_read(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], &d[0], &d[1], p.p, s); });
+    const int st = call([&] { return tri_cache_read(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], &d[0], &d[1], &c.p, s); });
     if (st != 0) return PyLong_FromLong(st);
     PyObject *const k = THPVariable_Wrap(out[0]), *const v = THPVariable_Wrap(out[1]);
     PyObject* const r = k != nullptr && v != nullptr ? PyTuple_Pack(2, k, v) : nullptr;
@@ -325,49 +390,47 @@ PyObject* cache_read_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// (q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out or None, want_lse, parameters, stream) -> out, or (out, lse)
-PyObject* cache_attention_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// (q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out or None, want_lse, kv_len, parameters, stream) -> out, or (out, lse);
+// or, where the scratch is smaller than the call's best plan wants or on another device, the bytes that it wants (nothing is
+// launched then)
+PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return run_new([&]() -> PyObject* {
     Tensors t;
-    if (!marshal(a, n, 8, 2, t)) return nullptr;
-    const OneDevice device(a, 8);
-    const CacheParams p(a[9]);
-    void* s = stream_of(a[10]);
-    const int want_lse = PyObject_IsTrue(a[8]);
-    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
-    if (!THPVariable_Check(a[0])) return PyErr_Format(PyExc_TypeError, "q has to be a tensor");
-    const at::Tensor& q = THPVariable_Unpack(a[0]);
+    if (!marshal(a, n, 8, 3, t)) return nullptr;
+    const at::Tensor* const q = tensor_of(a[0], "q");
+    if (q == nullptr) return nullptr;
+    const CacheCall c(a[10], a[1], q->dim() > 0 ? q->size(0) : 0, false, a[9]);
+    const bool want_lse = PyObject_IsTrue(a[8]) == 1;
+    void* s = stream_of(a[11]);
+    if (!c.ok || PyErr_Occurred() != nullptr) return nullptr;
+    const int64_t need = tri_cache_scratch_bytes(&c.p, t.p[2] != nullptr);
+    if (need < 0) return PyLong_FromLongLong(need);
+    if (need > 0 && (t.p[6] == nullptr || t.p[6]->shape[0] < need || THPVariable_Unpack(a[6]).device() != q->device()))
+      return PyLong_FromLongLong(need);
+    PyObject* with[8];
+    for (int i = 0; i < 8; ++i) with[i] = i == 6 && need == 0 ? Py_None : a[i];  // (a scratch that the call does without may be anywhere)
+    const OneDevice device(with, 8);
+    if (!device.ok) return nullptr;
     at::Tensor made, lse;
     tri_tensor o, l;
     tri_tensor *out = t.p[7], *lp = nullptr;
     if (out == nullptr) {
-      const int64_t cols = (int64_t)p.p->n_q_heads * p.p->head_dim;
-      made = new_tensor(q, {q.size(0), cols}, q.scalar_type());
-      o.ptr = made.data_ptr();
-      o.ndim = 2;
-      o.dtype = t.p[0]->dtype;
-      o.shape[0] = q.size(0); o.shape[1] = cols; o.stride[0] = cols; o.stride[1] = 1;
+      made = new_tensor(*q, {q->dim() > 0 ? q->size(0) : 0, (int64_t)c.p.n_q_heads * c.p.head_dim}, q->scalar_type());
+      o = describe(made, t.p[0]->dtype);
       out = &o;
     }
-    if (want_lse != 0) {
-      const int64_t sizes[3] = {p.p->batch, p.p->n_q_heads, p.p->seq};
-      lse = new_tensor(q, sizes, at::kFloat);
-      l.ptr = lse.data_ptr();
-      l.ndim = 3;
-      l.dtype = TRI_F32;
-      for (int j = 0; j < 3; ++j) {
-        l.shape[j] = sizes[j];
-        l.stride[j] = lse.stride(j);
-      }
+    if (want_lse) {
+      lse = new_tensor(*q, {c.p.batch, c.p.n_q_heads, c.p.seq}, at::kFloat);
+      l = describe(lse, TRI_F32);
       lp = &l;
     }
     const int st = call([&] {
-      return tri_cache_attention(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], lp, out, p.p, s);
+      return tri_cache_attention(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], need > 0 ? t.p[6] : nullptr, lp, out, &c.p, s);
     });
     if (st != 0) return PyLong_FromLong(st);
     PyObject* r = made.defined() ? THPVariable_Wrap(made) : a[7];
     if (!made.defined()) Py_INCREF(r);
-    if (r == nullptr || want_lse == 0) return r;
+    if (r == nullptr || !want_lse) return r;
     PyObject* const x = THPVariable_Wrap(lse);
     PyObject* const both = x != nullptr ? PyTuple_Pack(2, r, x) : nullptr;
     Py_DECREF(r);
@@ -407,8 +470,8 @@ PyMethodDef methods[] = {
     TRI_METHOD("gemm_workspace_bytes", workspace_bytes<tri_gemm_workspace_bytes>),
     TRI_METHOD("ffn_workspace_bytes", workspace_bytes<tri_ffn_workspace_bytes>),
     TRI_METHOD("cache_append", cache_append), TRI_METHOD("cache_read", cache_read),
-    TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_read_new", cache_read_new),
-    TRI_METHOD("cache_attention_new", cache_attention_new), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
+    TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_append_rows", cache_append_rows),
+    TRI_METHOD("cache_read_rows", cache_read_rows), TRI_METHOD("cache_attend", cache_attend), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -331,10 +331,15 @@ def cache_params(batch, n_kv_heads, head_dim, seq, kv_len, n_q_heads=None, scale
     return p
 
 
+def _stream_or_none(t):
+    """_stream_ptr, or 0 for a host tensor, which the binding of the cache calls refuses after its other checks."""
+    return _stream_ptr(t) if t is not None and t.is_cuda else 0
+
+
 def cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, validate_only=False):
     if validate_only:
         return _call("tri_validate_cache_append", [k, v, k_cache, k_scales, v_cache, v_scales, lens, ctypes.byref(params)], True)
-    st = native().cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, _stream_ptr(k))
+    st = native().cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, _stream_or_none(k))
     if st:
         _check("tri_cache_append", st)
     return st
@@ -343,7 +348,7 @@ def cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, valid
 def cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, validate_only=False):
     if validate_only:
         return _call("tri_validate_cache_read", [k_cache, k_scales, v_cache, v_scales, lens, k, v, ctypes.byref(params)], True)
-    st = native().cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, _stream_ptr(k))
+    st = native().cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, _stream_or_none(k))
     if st:
         _check("tri_cache_read", st)
     return st
@@ -361,26 +366,10 @@ def cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse,
     if validate_only:
         return _call("tri_validate_cache_attention", [q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out,
                                                       ctypes.byref(params)], True)
-    st = native().cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, _stream_ptr(q))
+    st = native().cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, _stream_or_none(q))
     if st:
         _check("tri_cache_attention", st)
     return st
-
-
-def cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, bf16, params):
-    """cache_read into new tensors [batch, KV heads, seq, head_dim]."""
-    r = native().cache_read_new(k_cache, k_scales, v_cache, v_scales, lens, bf16, params, _stream_ptr(k_cache))
-    if type(r) is int:
-        _check("tri_cache_read", r)
-    return r
-
-
-def cache_attention_new(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, params):
-    """cache_attention into a new tensor where `out` is None: returns the output, and a new log-sum-exp beside it if wanted."""
-    r = native().cache_attention_new(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, params, _stream_ptr(q))
-    if type(r) is int:
-        _check("tri_cache_attention", r)
-    return r
 
 
 def issue_probe(with_mfma, n_valu, n_trans, waves_per_simd, iters=4096, workgroups=256, device="cuda:0"):
