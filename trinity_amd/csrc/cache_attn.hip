@@ -115,6 +115,9 @@ __device__ __forceinline__ void cache_wg_map(const CacheAttnArgs& a, int id, int
 // Step t reads K(t + 1) and V(t), so K tiles travel two steps ahead and V tiles one; each has two buffers.  16-bit tiles go
 // from memory to LDS directly.  4-bit tiles are a 16-byte block per thread: it travels through registers, a step longer,
 // and is turned into 16 bits in the slots of O^T, which have little else to do.
+//
+// KW = 2: eight waves, the four row groups twice, on every other tile each with buffers of their own; they merge through
+// LDS at the end.  For calls with one workgroup a CU at most, whose time is the chain of its tiles.
 template <int D>
 struct TilePipe {
   static constexpr int KSTEPS = D / 16, DT = D / 32;
@@ -123,16 +126,18 @@ struct TilePipe {
   static constexpr int PD = 3, RING = 4;
 };
 
-template <int D, bool FP4>
-__device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, half_t* lds, const half_t* __restrict__ qglob) {
+template <int D, bool FP4, int KW>
+__device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, half_t* lds_all, const half_t* __restrict__ qglob) {
   // (qglob = a.q.  Inlined, every LDS access of this function carries "does not alias q", and an LDS read with alias
   // information is not made to wait for the loads to LDS in flight; barriers and explicit waits order those here.)
   using L = CacheLds<D>;
   using P = TilePipe<D>;
   constexpr int KSTEPS = P::KSTEPS, DT = P::DT, NKF = P::NKF, NVF = P::NVF, GPS = P::GPS, EPS = P::EPS, PD = P::PD, RING = P::RING;
   constexpr int CPR = L::CPR;
-  const int t = threadIdx.x, lane = t & 63;
+  const int t = threadIdx.x & 255, lane = t & 63;  // of the way's four waves
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kway = KW == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  half_t* const lds = lds_all + kway * 4 * L::HALFS;
   const int l32 = lane & 31, g = lane >> 5;
   const int group = a.group, rows = a.rows;
   int b, hk, rb, run;
@@ -141,7 +146,8 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   const KeyList kl = key_list(a, b, row_token(a, r0), row_token(a, min(r0 + kCacheRows, rows) - 1));
   const int ntiles = (kl.n + kCacheTile - 1) / kCacheTile;
   const int per = div_by(ntiles + a.runs - 1, a.by_runs), tile0 = min(run * per, ntiles);
-  const int nsteps = min(per, ntiles - tile0);
+  const int tile1 = min(tile0 + per, ntiles), nsteps = (tile1 - tile0 + KW - 1) / KW;
+  auto tile_of = [&](int step) { return tile0 + step * KW + kway; };  // (may lie past the last one)
 
   const int row = w0 + l32, rowc = min(row, rows - 1);
   const int tok = row_token(a, rowc), head = hk * group + rowc - tok * group;
@@ -150,7 +156,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   const int pos0 = kl.len - a.S + row_token(a, min(w0, rows - 1)), pos1 = kl.len - a.S + row_token(a, min(w0 + 31, rows - 1));
   // the steps that hold a key some row of the wave sees are [0, nact)
   const int seen = a.causal ? min(kl.n, pos1 + 1 - kl.gap) : kl.n;  // ... of the list
-  const int nact = w0 >= rows ? 0 : max(0, min(nsteps, (seen + kCacheTile - 1) / kCacheTile - tile0));
+  const int nact = w0 >= rows ? 0 : max(0, (min(tile1, (seen + kCacheTile - 1) / kCacheTile) - tile0 - kway + KW - 1) / KW);
 
   half8v qf[KSTEPS];
   const half_t* qp = qglob + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)head * D + g * 8;
@@ -171,7 +177,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   half_t *const kt = lds, *const vt = lds + 2 * L::HALFS;
   // key of row r of a tile (past the last key: the last one again, whose scores are masked)
   auto key_of = [&](int step, int r) {
-    const int li = min((tile0 + step) * kCacheTile + r, kl.n - 1);
+    const int li = min(tile_of(step) * kCacheTile + r, kl.n - 1);
     return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
   };
   auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
@@ -246,18 +252,18 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   // front of a gap all of these are sinks).  `last` differs between the wave's rows by less than 32, `from` as much.
   const int last = pos < 0 ? -1 : (a.causal ? pos - kl.gap : kl.n - 1), from = a.window > 0 ? pos - a.window + 1 - kl.gap : 0;
   auto need_mask = [&](int step) {
-    const int li0 = (tile0 + step) * kCacheTile, li1 = li0 + kCacheTile - 1;
+    const int li0 = tile_of(step) * kCacheTile, li1 = li0 + kCacheTile - 1;
     return li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0) || (a.window > 0 && li0 + kl.gap <= pos1 - a.window && li1 >= a.sinks);
   };
   auto apply_mask = [&](float16v (&s)[2], int step) {
-    const int base = (tile0 + step) * kCacheTile + g * 4;  // the lane's scores are of indices base + (0 to 3) + 8 i
+    const int base = tile_of(step) * kCacheTile + g * 4;  // the lane's scores are of indices base + (0 to 3) + 8 i
     const int end = min(last, kl.n - 1) - base;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (mt * 32 + (r >> 2) * 8 + (r & 3) > end) s[mt][r] = -INFINITY;
-    const int li0 = (tile0 + step) * kCacheTile;
+    const int li0 = tile_of(step) * kCacheTile;
     if (a.window > 0 && li0 + kl.gap <= pos1 - a.window) {  // wave-uniform: the window of some row begins in the tile, or behind it
       asm volatile("");
       const int begin = from - base, sinks = a.sinks - base;
@@ -437,13 +443,39 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
     }
   }
 
+  // ---- two ways: the second hands its state over, lane for lane, and leaves
+  constexpr int REG = DT * 16 + 2;
+  float* const mg = reinterpret_cast<float*>(lds_all) + wave * REG * 64 + lane;
+  if constexpr (KW == 2) {
+    __syncthreads();  // (every wave is done with the tiles)
+    if (kway == 1) {
+      mg[0] = m;
+      mg[64] = l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mg[(2 + dt * 16 + e) * 64] = o[dt][e];
+    }
+    __syncthreads();
+    if (kway == 1) return;
+    const float m1 = mg[0], mn = fmaxf(m, m1);
+    const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mn);
+    m = mn;
+    l = l * a0 + mg[64] * a1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * a0 + mg[(2 + dt * 16 + e) * 64] * a1;
+  }
+
   l = pair_sum(l);
   if (a.runs == 1) {
     // ---- a lane has sixteen pieces of 8 bytes of its row: stored as they are, every store instruction touches 32 lines, so
     // each wave turns its rows around in LDS and stores whole ones, 16 bytes a lane
     constexpr int LDO = D + 8;
-    half_t* const stage = lds + wave * 32 * LDO;
-    __syncthreads();  // (every wave is done with the tiles)
+    static_assert(32 * LDO * 2 <= REG * 64 * 4, "two ways: in the place of the state that only this wave has read");
+    half_t* const stage = KW == 2 ? reinterpret_cast<half_t*>(mg - lane) : lds + wave * 32 * LDO;
+    if (KW == 1) __syncthreads();  // (every wave is done with the tiles)
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -477,10 +509,10 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
                     float4v{o[dt][rq * 4], o[dt][rq * 4 + 1], o[dt][rq * 4 + 2], o[dt][rq * 4 + 3]});
 }
 
-template <int D, bool FP4>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_tile_kernel(CacheAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) half_t lds[4 * CacheLds<D>::HALFS];
-  cache_attn_tile_body<D, FP4>(a, lds, a.q);
+template <int D, bool FP4, int KW>
+__global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_tile_kernel(CacheAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) half_t lds[KW * 4 * CacheLds<D>::HALFS];
+  cache_attn_tile_body<D, FP4, KW>(a, lds, a.q);
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows
@@ -870,15 +902,26 @@ constexpr int kFewRowWorkgroups = 512, kFewRowKeys = 4 * kFewRowTile;
 // one sequence in 4 bits of 512 keys 6.5 / 7.0, 768 7.9 / 7.2, in 16 bits of 384 7.3 / 7.5, 512 8.5 / 7.3; sixteen of 768 8.7 / 9.0 and
 // 11.9 / 12.2, of 1500 13.0 / 10.3 and 18.7 / 18.4; graph replays, eager calls gain another 2.7 us of host time).
 constexpr int kFewRowAlone4 = 5, kFewRowAlone16 = 3, kFewRowAloneMany = 8, kFewRowManyHeads = 128;
-// Many rows: what a call takes in us, fitted over sixteen calls of 71 to 65536 rows in 1 to 64 runs: a tile alone on its CU and
-// beside another workgroup's, fixed costs with and without the merge, and the partial results' way to memory and back
-// (8 KV heads, 64 tokens against 2000 keys in 4 / 8 / 16 / 32 runs 21.1 / 18.5 / 21.7 / 30.5 us; 512 against 16512 in 2 / 4 / 8
-// 202 / 164 / 175; 71 heads on one, one token against 8000 in 16 / 32 / 64 15.6 / 11.8 / 10.3).
-constexpr float kTileAloneUs = 1.2f, kTileBesideUs = 2.0f, kTileFixedUs = 5.0f, kTileMergeUs = 7.8f, kTilePartBytesPerUs = 4.1e6f;
+// Many rows: what a call takes in us, fitted over sixteen calls of 71 to 65536 rows in 1 to 64 runs, for 64- and 128-wide heads:
+// a tile alone on its CU, beside another workgroup's, and a pair of them in two key ways (128-wide in 4 bits a little more: there
+// the conversion of both is in the chain); fixed costs with and without the merge, and of the two ways; the partial results'
+// way to memory and back.  (8 KV heads of 128 in 4 bits: 64 tokens against 2000 keys in 4 / 8 / 16 / 32 runs 21.1 / 18.5 / 21.7 /
+// 30.5 us, two ways in eight 19.4; 512 against 16512 in 2 / 4 / 8 202 / 164 / 175, two ways in two 165; 128 against 8000 in sixteen
+// 39.6, two ways in eight 37.6; a prompt of 1024, one way / two 27.0 / 24.7, in 16 bits 28.3 / 23.6; two of 400 against 3000 keys 58.3
+// in two runs / 53.7.  71 heads of 64 on one: one token against 8000 in 16 / 32 / 64 15.6 / 11.8 / 10.3, 100 in eight 39.0, two
+// ways in four 36.8.)
+struct TileUs {
+  float alone, beside, pair;
+};
+constexpr TileUs tile_us(int D, bool four_bit) {
+  return D == 64 ? TileUs{1.0f, 1.5f, 1.55f} : TileUs{1.2f, 2.0f, four_bit ? 2.25f : 1.95f};
+}
+constexpr float kTileFixedUs = 5.0f, kTileMergeUs = 7.8f, kTilePairFixedUs = 1.0f, kTilePartBytesPerUs = 4.1e6f;
 constexpr int kTileRound = 512;  // workgroups at a time, two a CU
 
 struct CachePlan {
   int nt;       // few rows: column tiles of 16 rows (0: the kernel of many rows)
+  int ways;     // many rows: ... with one or two key ways
   int runs;
   int64_t nwg;  // workgroups per run
 };
@@ -903,15 +946,25 @@ static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, in
   const int64_t tiles = (keys + kCacheTile - 1) / kCacheTile;
   const int64_t most = tiles < kCacheMaxRuns ? tiles : kCacheMaxRuns;
   const float part_us = (float)(heads * rows) * (float)D * 8.f / kTilePartBytesPerUs;
+  const TileUs tile = tile_us(D, four_bit);
   float best = 0.f;
   p.runs = 1;
+  p.ways = 1;
   for (int r = 1; r <= most && (r == 1 || p.nwg * r <= 4 * kTileRound); ++r) {
     const int64_t wgs = p.nwg * r, per = (tiles + r - 1) / r;
-    const float steps = wgs <= kTileRound / 2 ? kTileAloneUs : kTileBesideUs * (float)((wgs + kTileRound - 1) / kTileRound);
+    const float steps = wgs <= kTileRound / 2 ? tile.alone : tile.beside * (float)((wgs + kTileRound - 1) / kTileRound);
     const float us = (float)per * steps + (r == 1 ? kTileFixedUs : kTileMergeUs + (float)r * part_us);
     if (r == 1 || us < best) {
       best = us;
       p.runs = r;
+      p.ways = 1;
+    }
+    if (wgs > kTileRound / 2) continue;
+    const float two_us = (float)((per + 1) / 2) * tile.pair + kTilePairFixedUs + (r == 1 ? kTileFixedUs : kTileMergeUs + (float)r * part_us);
+    if (two_us < best) {
+      best = two_us;
+      p.runs = r;
+      p.ways = 2;
     }
   }
   return p;
@@ -925,10 +978,11 @@ int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_
 }
 
 template <int D, bool FP4>
-static void launch_t(const CacheAttnArgs& a, int nt, unsigned nwg, hipStream_t stream) {
+static void launch_t(const CacheAttnArgs& a, int nt, int ways, unsigned nwg, hipStream_t stream) {
   if (nt == 1) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
   else if (nt == 2) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 2>), dim3(nwg), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4>), dim3(nwg), dim3(256), 0, stream, a);
+  else if (ways == 2) hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4, 2>), dim3(nwg), dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
 }
 
 template <int D>
@@ -962,8 +1016,8 @@ int launch_cache_attention(const CacheAttnArgs& args, hipStream_t stream) {
   a.by_heads = cache_div(heads % 8 == 0 ? heads / 8 : heads);
   const unsigned nwg = (unsigned)(p.nwg * a.runs);
   const bool fp4 = a.kc.scales != nullptr;
-  if (a.D == 128) fp4 ? launch_t<128, true>(a, p.nt, nwg, stream) : launch_t<128, false>(a, p.nt, nwg, stream);
-  else fp4 ? launch_t<64, true>(a, p.nt, nwg, stream) : launch_t<64, false>(a, p.nt, nwg, stream);
+  if (a.D == 128) fp4 ? launch_t<128, true>(a, p.nt, p.ways, nwg, stream) : launch_t<128, false>(a, p.nt, p.ways, nwg, stream);
+  else fp4 ? launch_t<64, true>(a, p.nt, p.ways, nwg, stream) : launch_t<64, false>(a, p.nt, p.ways, nwg, stream);
   if (hipGetLastError() != hipSuccess) return -1;
   if (a.runs == 1) return 0;
   if (a.D == 128) launch_merge<128>(a, stream);
