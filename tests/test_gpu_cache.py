@@ -138,6 +138,15 @@ ATTN = [
     (1, 1, 8, 2, 128, 640, 640, None, True, 0, 0),             # few rows: one run in 4 bits, several in 16
     (33, 1, 4, 4, 64, 1300, 1300, [1300 - 40 * i for i in range(33)], True, 0, 0),  # many heads: 1024 keys and fewer in one run
     (33, 1, 4, 4, 64, 900, 900, [900 - 27 * i for i in range(33)], True, 0, 0),
+    (1, 8, 16, 4, 64, 2000, 1990, None, True, 0, 0),           # column tiles of 16 rows: two of them
+    (2, 8, 16, 4, 64, 200, 200, [200, 91], True, 60, 4),
+    (1, 8, 16, 4, 128, 200, 200, None, True, 0, 0),
+    # two key ways: in one run and in several
+    (1, 48, 48, 48, 64, 329, 329, None, True, 0, 0),
+    (2, 155, 8, 8, 64, 340, 339, [339, 150], True, 200, 3),
+    (3, 48, 32, 32, 64, 660, 653, [653, 640, 20], True, 0, 0),
+    (3, 20, 96, 48, 128, 840, 840, [840, 100, 19], True, 0, 0),
+    (3, 133, 16, 16, 128, 1672, 1672, [1672, 1500, 130], False, 0, 0),
 ]
 
 

@@ -919,16 +919,11 @@ constexpr TileUs tile_us(int D, bool four_bit) {
 constexpr float kTileFixedUs = 5.0f, kTileMergeUs = 7.8f, kTilePairFixedUs = 1.0f, kTilePartBytesPerUs = 4.1e6f;
 constexpr int kTileRound = 512;  // workgroups at a time, two a CU
 
-struct CachePlan {
-  int nt;       // few rows: column tiles of 16 rows (0: the kernel of many rows)
-  int ways;     // many rows: ... with one or two key ways
-  int runs;
-  int64_t nwg;  // workgroups per run
-};
-static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit) {
+CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit) {
   const int group = Hq / Hkv, rows = S * group;
   const int64_t heads = (int64_t)B * Hkv;
-  CachePlan p;
+  CachePlan p{};
+  p.ways = 1;
   p.nt = rows <= kFewRowsMost ? (rows + 15) / 16 : 0;
   p.nwg = p.nt > 0 ? heads : (rows + kCacheRows - 1) / kCacheRows * heads;
   // most keys of a row block
@@ -949,7 +944,6 @@ static CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, in
   const TileUs tile = tile_us(D, four_bit);
   float best = 0.f;
   p.runs = 1;
-  p.ways = 1;
   for (int r = 1; r <= most && (r == 1 || p.nwg * r <= 4 * kTileRound); ++r) {
     const int64_t wgs = p.nwg * r, per = (tiles + r - 1) / r;
     const float steps = wgs <= kTileRound / 2 ? tile.alone : tile.beside * (float)((wgs + kTileRound - 1) / kTileRound);

@@ -302,6 +302,13 @@ struct CacheAttnArgs {
   CacheDiv by_group, by_runs, by_hkv, by_heads;  // (by_heads: KV heads of all sequences, or an eighth of them)
 };
 int launch_cache_attention(const CacheAttnArgs& a, hipStream_t stream);
+struct CachePlan {
+  int nt;       // few rows: column tiles of 16 rows (0: the kernel of many rows)
+  int ways;     // many rows: ... with one or two key ways
+  int runs;     // parts that the keys are cut into
+  int64_t nwg;  // workgroups per run
+};
+CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
 int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
 
 }  // namespace tri
