@@ -376,14 +376,14 @@ def test_plan_over_ragged_four_bit_caches(dev):
 @pytest.mark.parametrize("four_bit", [False, True])
 def test_graph_of_a_decode_step(dev, four_bit):
     """A step captured once, on a stream of its own, and replayed as the lengths grow on the device; eager calls of the same
-    objects and of another shape between the replays; two graphs in turn that share their scratch."""
+    objects and of another shape between the replays, on the graph's stream too; two graphs of one object."""
     B, Hq, Hkv, D, rows, dtype = 3, 16, 4, 128, 3000, F16
     caches = make_caches(5, B, Hkv, rows, D, dtype, four_bit)
     c = [None if x is None else x.to(dev) for x in caches]
     start = [2900, 700, 0]
     g = torch.Generator().manual_seed(6)
     op = blocks.CachedAttention(Hq, Hkv, D)
-    win = blocks.CachedAttention(Hq, Hkv, D, window=500, sinks=4)
+    win = blocks.CachedAttention(Hq, Hkv, D, window=2500, sinks=4)
     lens = _lens(start, dev)
     q, k, v = (torch.zeros(B, h * D, dtype=dtype, device=dev) for h in (Hq, Hkv, Hkv))
     out, out2 = (torch.zeros(B, Hq * D, dtype=dtype, device=dev) for _ in range(2))
@@ -399,7 +399,8 @@ def test_graph_of_a_decode_step(dev, four_bit):
         step(op, out)
         step(win, out2)
     stream.synchronize()
-    win._scratch = op._scratch  # (the larger one: no window)
+    kept = {id(o): dict(o._scratch) for o in (op, win)}
+    assert all(len(x) == 1 for x in kept.values())
     lens.copy_(torch.tensor(start))
     for x, y in zip(c, caches):
         if x is not None:
@@ -410,6 +411,7 @@ def test_graph_of_a_decode_step(dev, four_bit):
         with torch.cuda.graph(graph, stream=stream):
             step(o, dst)
         graphs.append(graph)
+    assert all(dict(o._scratch) == kept[id(o)] for o in (op, win))  # the graphs have scratch of their own
     n = list(start)
     hist = [values(caches[0], caches[2]).clone(), values(caches[1], caches[3]).clone()]
     for rep in range(6):
@@ -426,15 +428,54 @@ def test_graph_of_a_decode_step(dev, four_bit):
             val = oc.fp4_decode(*oc.fp4_encode(new[1 + i])) if four_bit else new[1 + i].double()
             for b in range(B):
                 hist[i][b, :, n[b] - 1] = val.view(B, Hkv, D)[b]
-        kw = dict(window=500, sinks=4) if which else {}
+        kw = dict(window=2500, sinks=4) if which else {}
         want, lse, mag = oc.cache_attention(new[0], hist[0], hist[1], n, n_q_heads=Hq, **kw)
         tol, _ = attention_tolerance(new[0], hist[0], hist[1], n, mag, want, dtype, n_q_heads=Hq, scale=D ** -0.5)
         got = (out, out2)[which]
         assert_within(got, want, tol, "replay %d" % rep)
         eager = (op, win)[which].attend(q, c[0], c[1], c[2], c[3], **kv)
         assert torch.equal(eager, got)
-        op.attend(q[:1].repeat(B * 3, 1), c[0], c[1], c[2], c[3], **kv)
+        with torch.cuda.stream(stream):
+            for other in (op, win):
+                other.attend(q[:1].repeat(B * 3, 1), c[0], c[1], c[2], c[3], **kv)
         torch.cuda.synchronize()
+
+
+def test_two_streams_and_a_captured_first_call(dev):
+    """One object on two streams at a time, and captured before it has ever run: every one of them with scratch of its own."""
+    q, c, ln, *ref = _case(dev, 1, 1, 32, 8, 128, 4000, 4000, None, True, 0, 0, F16, True)
+    op = blocks.CachedAttention(32, 8, 128)
+    graph = torch.cuda.CUDAGraph()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        captured = op.attend(q, c[0], c[1], c[2], c[3])
+    assert not op._scratch
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            if i % 3 == 2:
+                graph.replay()
+            else:
+                outs.append(op.attend(q, c[0], c[1], c[2], c[3]))
+    torch.cuda.synchronize()
+    assert len(op._scratch) == 2
+    _check(outs[0], None, *ref)
+    assert all(torch.equal(x, outs[0]) for x in outs + [captured])
+
+
+def test_under_inference_mode(dev):
+    q, c, ln, *ref = _case(dev, 2, 3, 4, 2, 64, 90, 90, [90, 20], True, 0, 0, F16, True)
+    op = blocks.CachedAttention(4, 2, 64)
+    with torch.inference_mode():
+        out, lse = op.attend(q, c[0], c[1], c[2], c[3], lens=ln, want_lse=True)
+        k, v = op.read(c[0], c[1], c[2], c[3], lens=ln)
+        _check(out.clone(), lse + 0, *ref)
+        assert (k + v).shape == (2, 2, 90, 64) and k.clone().is_contiguous()
+    k, v = op.read(c[0], c[1], c[2], c[3], lens=ln)
+    k += 1  # the results are tensors like others, also in place
+    assert _same(v, op.read(c[0], c[1], c[2], c[3], lens=ln)[1])
 
 
 def test_other_devices_tensors_are_refused(dev):

@@ -102,7 +102,10 @@ class CachedAttention:
 
     Caches are [batch, KV heads, rows, head_dim], or `make_cache`'s 4-bit pair of codes and scales.  `lens` (int32 on the
     device, None: all `kv_len`) holds the lengths with the call's tokens, which are the last ones of each sequence; a sequence
-    with fewer has its first rows as padding.  `kv_len` (None: all rows of the cache) bounds the lengths."""
+    with fewer has its first rows as padding.  `kv_len` (None: all rows of the cache) bounds the lengths.
+
+    An object keeps a scratch buffer for every stream it attends on; a call under graph capture takes one of the graph's own, so
+    that graphs share none."""
 
     def __init__(self, n_q_heads, n_kv_heads, head_dim, scale=None, causal=True, window=0, sinks=0):
         self.head_dim = head_dim
@@ -110,7 +113,7 @@ class CachedAttention:
         self._p = ext.cache_params(0, n_kv_heads, head_dim, 0, 0, n_q_heads=n_q_heads, scale=scale, causal=causal, window=window,
                                    sinks=sinks)
         self._native = ext.native()
-        self._scratch = None
+        self._scratch = {}
 
     @staticmethod
     def make_cache(batch, n_kv_heads, rows, head_dim, device):
@@ -143,13 +146,17 @@ class CachedAttention:
         """Q [batch * tokens, query heads * head_dim] over the caches, which hold the tokens' own keys already.  Returns
         the output like Q, and with `want_lse` the log-sum-exp [batch, query heads, tokens] beside it."""
         stream = ext._stream_or_none(Q)
-        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, self._scratch, out, want_lse, kv_len, self._p,
-                                      stream)
+        scratch = self._scratch.get(stream)
+        capturing = scratch is not None and torch.cuda.is_current_stream_capturing()
+        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, None if capturing else scratch, out, want_lse,
+                                      kv_len, self._p, stream)
         if type(r) is int:
-            if r > 0:  # bytes of scratch: the first call of its size
-                self._scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
-                r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, self._scratch, out, want_lse, kv_len,
-                                              self._p, stream)
+            if r > 0:  # bytes of scratch: the first call of its size, or a captured one
+                scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
+                if not torch.cuda.is_current_stream_capturing():
+                    self._scratch[stream] = scratch
+                r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, self._p,
+                                              stream)
             if type(r) is int:
                 ext._check("tri_cache_attention", r)
         return r
@@ -157,7 +164,8 @@ class CachedAttention:
 
 class CachedAttentionPlan:
     """AttentionPlan's block - [PreNorm,] Q/K/V projection, [QKNorm,] append, attention - for the next tokens of several
-    sequences over the caches of `CachedAttention`: X [batch * tokens, N], and what its methods take."""
+    sequences over the caches of `CachedAttention`: X [batch * tokens, N], and what its methods take.  The projections' buffers
+    are the plan's own: calls of one plan, and graphs captured from it, run one after the other."""
 
     def __init__(self, n_q_heads, n_kv_heads, head_dim, scale=None, causal=True, window=0, sinks=0, prenorm=False, qknorm=False,
                  eps=0.0):
