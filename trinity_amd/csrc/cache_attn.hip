@@ -118,6 +118,15 @@ __device__ __forceinline__ void cache_wg_map(const CacheAttnArgs& a, int id, int
 //
 // KW = 2: eight waves, the four row groups twice, on every other tile each with buffers of their own; they merge through
 // LDS at the end.  For calls with one workgroup a CU at most, whose time is the chain of its tiles.
+//
+// What bounds it.  128-wide heads: the board's power limit, as the other attention kernels (a prompt of 4096 tokens over a
+// 4-bit cache 133 us, 1.03 PFLOP/s, level with 16-bit rows: the conversion is hidden; matrix pipe busy 45 % of the time at the
+// clock that the limit leaves), and beside it some 9 us a round of workgroups for their first loads, the first tile's scores and
+// the stores (8192 tokens in a window of 1024, four rounds of 17 tiles, 160 us).  64-wide heads: the chain of a step, two waves
+// a SIMD that wait for LDS, matrix and exponential results a third of the time (two prompts of 1000 tokens, 71 heads, in 256:
+// 24 us, vector pipe 40 % busy, matrix pipe 12 %).  Measured and level: fixed offsets in place of an address per row, cheaper
+// masks, workgroups that start apart; slower: three buffers with loads two steps ahead (64-wide, 5 %), three waves a SIMD (they
+// spill, 12 %).
 template <int D>
 struct TilePipe {
   static constexpr int KSTEPS = D / 16, DT = D / 32;
@@ -521,6 +530,12 @@ __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // from memory straight into the registers that the matrix instructions want: a lane holds D / 4 channels of one key, in
 // 4 bits one block with one scale (the order of the channels in the product is free, as long as q has the same).  V goes
 // through a tile of LDS that only its wave touches, for the transpose.
+//
+// Long lists run at the rate of memory: 32 sequences of up to 8192 keys in 4 bits 36 us of kernel for 217 MB (6.0 TB/s, half of
+// it out of the last-level cache where the call is repeated), 16 in a window of 4096 in 16 bits 41 us for 268 MB (6.5).  Short
+// ones are latency: one sequence of 4096 keys 5.2 us and 3.4 of merge.  48 and 64 rows this way, with four waves on a CU, are
+// slower than the kernel of many rows (64 rows of 8 KV heads against 16000 keys 23.7 us, 21.9 there; 71 of 64-wide against 8000
+// 10.8 and 9.8).
 constexpr int kFewRowTile = 32;   // keys
 
 template <int D>
