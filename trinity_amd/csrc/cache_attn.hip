@@ -406,18 +406,32 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   if (nsteps > 0) {
     // ---- prologue: K(0), K(1), V(0); S^T of tile 0
     if constexpr (FP4) {
+      // (all five on their way at once: one trip to memory)
       fetch4(0, false);
+      const uint4v k0 = kraw;
+      const uint32_t kx0 = kxraw;
       fetch4(0, true);
+      const uint4v v0 = vraw;
+      const uint32_t vx0 = vxraw;
+      fetch4(1, false);
+      const uint4v k1 = kraw;
+      const uint32_t kx1 = kxraw;
+      fetch4(2, false);
+      const uint4v k2 = kraw;
+      const uint32_t kx2 = kxraw;
+      fetch4(1, true);
+      const uint4v v1 = vraw;
+      const uint32_t vx1 = vxraw;
+      kraw = k0; kxraw = kx0; vraw = v0; vxraw = vx0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         commit4(0, false, j);
         commit4(0, true, j);
       }
-      fetch4(1, false);
+      kraw = k1; kxraw = kx1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) commit4(1, false, j);
-      fetch4(2, false);
-      fetch4(1, true);
+      kraw = k2; kxraw = kx2; vraw = v1; vxraw = vx1;
     } else {
       load16(0, false, 0);
       load16(0, true, 0);
