@@ -136,6 +136,19 @@ def test_append_tensors():
     assert _append(k_cache=c[:, :, :1].expand(B, Hkv, L, D // 2)) == STRIDE
 
 
+def test_written_rows_that_share_memory():
+    """No two dimensions step over one another's rows, whatever their order."""
+    some = _h(2 * B * Hkv * L * D)
+    lay = lambda *strides: _append(k_cache=some.as_strided((B, Hkv, L, D), strides + (1,)), v_cache=_h(B, Hkv, L, D), k_scales=None,
+                                   v_scales=None)
+    assert lay(Hkv * L * D, L * D, D) == lay(D, B * D, B * Hkv * D) == lay(L * Hkv * D, D, Hkv * D) == 0
+    assert lay(D, D, D) == lay(Hkv * L * D, (L - 1) * D, D) == lay((Hkv * L - 1) * D, L * D, D) == STRIDE
+    assert lay(D, B * D - 8, B * Hkv * D) == lay(L * D, L * D, D) == STRIDE
+    both = _h(B, L, Hkv, 2, D)  # k and v side by side
+    k, v = (both[:, :, :, i].transpose(1, 2) for i in range(2))
+    assert _append(k_cache=k, v_cache=v, k_scales=None, v_scales=None) == 0
+
+
 def test_read_tensors():
     assert _read(k=None) == _read(v=None) == NULL
     assert _read(k=_h(B, Hkv, S + 1, D)) == _read(v=_h(B, Hkv, L, D)) == SHAPE

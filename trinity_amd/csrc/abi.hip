@@ -1,5 +1,7 @@
 // C ABI of libtrinity_amd.so: argument validation (pure host code, usable
 // without a GPU) and the launch sequences behind each entry point.
+#include <algorithm>
+
 #include "../../include/trinity_amd.h"
 
 #include "launch.h"  // fp16 kernels: namespace tri
@@ -365,8 +367,7 @@ int check_cache_params(const tri_cache_params* p, bool attention) {
 }
 
 // [B, H, >= rows, n] (or [H, rows, n] where B is 1) with contiguous rows; `unit`: what its strides are multiples of.  `write`:
-// rows must not share memory (their order is free, and a stride larger than another's extent is not asked for: a
-// transposed view interleaves heads and rows).
+// rows must not share memory (the order of the dimensions is free).
 int check_cache4(const tri_tensor* t, int64_t B, int64_t H, int64_t rows, bool exact_rows, int64_t n, int64_t unit, int align,
                  int dtype, bool write) {
   if (t == nullptr) return TRI_ERR_NULL;
@@ -383,7 +384,18 @@ int check_cache4(const tri_tensor* t, int64_t B, int64_t H, int64_t rows, bool e
   const int64_t sb = t->ndim == 4 ? t->stride[0] : 0;
   if ((B > 1 && sb % unit != 0) || (H > 1 && st[0] % unit != 0) || (sh[1] > 1 && st[1] % unit != 0)) return TRI_ERR_STRIDE;
   if ((B > 1 && sb < 0) || (H > 1 && st[0] < 0) || (sh[1] > 1 && st[1] < 0)) return TRI_ERR_STRIDE;
-  if (write && ((B > 1 && sb < n) || (H > 1 && st[0] < n) || (sh[1] > 1 && st[1] < n))) return TRI_ERR_STRIDE;
+  if (write) {  // from the smallest stride on, each steps over all that those before it reach
+    struct Dim {
+      int64_t size, stride;
+    } d[3] = {{B, sb}, {H, st[0]}, {sh[1], st[1]}};
+    std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    uint64_t extent = (uint64_t)n;
+    for (const Dim& x : d) {
+      if (x.size <= 1) continue;
+      if ((uint64_t)x.stride < extent) return TRI_ERR_STRIDE;
+      extent += (uint64_t)x.stride * (uint64_t)(x.size - 1);
+    }
+  }
   if (((uintptr_t)t->ptr & (uintptr_t)(align - 1)) != 0) return TRI_ERR_ALIGN;
   return TRI_OK;
 }
