@@ -90,6 +90,13 @@ def test_parameters():
         ext.native().cache_scratch_bytes(ext.attn_params(2, 2, 64, 1), 0)
 
 
+def test_more_heads_than_a_launch_has_workgroups():
+    many = _params(batch=1 << 23, n_kv_heads=2, n_q_heads=2, seq=1)
+    assert _attend(many) == UNSUPPORTED
+    assert ext.lib().tri_cache_scratch_bytes(ctypes.byref(many), 0) == UNSUPPORTED
+    assert _attend(_params(batch=(1 << 23) - 1, n_kv_heads=2, n_q_heads=2, seq=1)) == SHAPE
+
+
 def test_attention_tensors():
     c, x = _four()
     assert _attend(q=None) == _attend(k_cache=None) == _attend(v_cache=None) == _attend(out=None) == NULL

@@ -358,6 +358,7 @@ int check_cache_params(const tri_cache_params* p, bool attention) {
     return TRI_ERR_UNSUPPORTED;
   if (p->kv_len >= (1 << 30) || p->seq >= (1 << 30)) return TRI_ERR_UNSUPPORTED;
   if (!attention) return TRI_OK;
+  if ((int64_t)p->batch * p->n_kv_heads >= (1 << 24)) return TRI_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
   if (p->n_q_heads <= 0 || p->n_q_heads % p->n_kv_heads != 0) return TRI_ERR_SHAPE;
   if ((int64_t)p->batch * p->seq * p->n_q_heads * (p->head_dim / 8) >= kInt32End - 4096) return TRI_ERR_UNSUPPORTED;
   if (!(p->scale > 0.f) || !(p->scale < INFINITY)) return TRI_ERR_UNSUPPORTED;
