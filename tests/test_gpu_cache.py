@@ -252,6 +252,28 @@ def test_numbers_that_are_none_stay_where_they_are_seen(dev):
         assert_within(others, want.view(B, -1)[[0, 2]], tol.view(B, -1)[[0, 2]], "other sequences")
 
 
+@pytest.mark.parametrize("S,Hq,D", [(1, 4, 128), (9, 2, 64), (40, 4, 128), (70, 2, 64)])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_runs_that_see_no_number(dev, S, Hq, D, four_bit):
+    """Parts of the keys whose scores are NaN one and all, and a query that is one, are not lost in the merge of the parts."""
+    Hkv, n = 1, 4096
+    q, c, ln, want, lse, tol, tol_lse = _case(dev, 1, S, Hq, Hkv, D, n, n, None, False, 0, 0, BF16, four_bit)
+    assert ext.cache_scratch_bytes(ext.cache_params(1, Hkv, D, S, n, n_q_heads=Hq, causal=False), four_bit) > 0
+    op = blocks.CachedAttention(Hq, Hkv, D, causal=False)
+    row = (S // 2, Hq - 1)  # token, head
+    bad = q.clone().view(S, Hq, D)
+    bad[row] = math.nan
+    got, got_lse = op.attend(bad.view(S, -1), *c, want_lse=True)
+    got, got_lse = got.cpu().view(S, Hq, D), got_lse.cpu()[0]
+    assert torch.isnan(got[row]).all() and torch.isnan(got_lse[row[1], row[0]])
+    rest = torch.ones(S, Hq, dtype=torch.bool)
+    rest[row] = False
+    assert_within(got[rest], want.view(S, Hq, D)[rest], tol.view(S, Hq, D)[rest], "other rows")
+    (c[2] if four_bit else c[0])[:, :, 1024:2560] = 255 if four_bit else math.nan  # K of whole parts
+    got, got_lse = op.attend(q, *c, want_lse=True)
+    assert torch.isnan(got).all() and torch.isnan(got_lse).all()
+
+
 @pytest.mark.parametrize("four_bit", [False, True])
 def test_offsets_beyond_32_bits(dev, four_bit):
     """A cache whose rows lie so far apart that their offsets do not fit 32 bits (in elements, and in bytes)."""

@@ -873,20 +873,28 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     for (int j = 0; j < UNROLL; ++j) {
       const int i = min(i0 + j * WAYS, a.runs - 1);
       mi[j] = i0 + j * WAYS < a.runs ? ps[i * 2] : -INFINITY;
-      li[j] = ps[i * 2 + 1];
+      li[j] = i0 + j * WAYS < a.runs ? ps[i * 2 + 1] : 0.f;
       v[j] = *reinterpret_cast<const float4v*>(po + (int64_t)i * D);
     }
     float mn = m;
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) mn = fmaxf(mn, mi[j]);
-    if (mn == -INFINITY) continue;  // (runs without a visible key)
+    // (a run whose maximum is -inf sees no key, and its sum is 0, or it sees NaN alone, and its sum is one)
+    if (mn == -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) l += li[j];
+      continue;
+    }
     const float keep = fast_exp2(m - mn);
     l *= keep;
     acc = acc * keep;
     m = mn;
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
-      if (mi[j] == -INFINITY) continue;
+      if (mi[j] == -INFINITY) {
+        l += li[j];
+        continue;
+      }
       const float w = fast_exp2(mi[j] - m);
       l = fmaf(li[j], w, l);
 #pragma unroll
