@@ -463,6 +463,41 @@ def test_graph_of_a_decode_step(dev, four_bit):
         torch.cuda.synchronize()
 
 
+def test_plan_keeps_no_buffer_that_a_graph_uses(dev):
+    """A captured step of single tokens is replayed after eager prompts of the same plan, whose memory others have filled since,
+    and beside another stream's step."""
+    B, N, Hq, Hkv, D, rows = 4, 256, 8, 2, 128, 600
+    t = {k: v.to(dev) for k, v in attn_inputs(40 * B, N, Hq, Hkv, D, w_std=0.06).items()}
+    w = (t["wq"], t["wk"], t["wv"])
+    plan = blocks.CachedAttentionPlan(Hq, Hkv, D, prenorm=True, qknorm=True, eps=1e-5)
+    caches = [x.to(dev) for x in make_caches(8, B, Hkv, rows, D, F16, False)[:2]]
+    lens = _lens([600, 41, 300, 77], dev)
+    out, want = torch.zeros(B, Hq * D, dtype=F16, device=dev), torch.zeros(B, Hq * D, dtype=F16, device=dev)
+    x = t["x"][:B].clone()
+    run = lambda x, out, c: plan.run(x, *w, out, *c, lens=lens)
+    run(x, out, caches)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(x, out, caches)
+    side = torch.cuda.Stream()
+    for rep in range(5):
+        x.copy_(t["x"][rep * B:(rep + 1) * B])
+        c = [y.clone() for y in caches]
+        prompt = torch.empty(40 * B, Hq * D, dtype=F16, device=dev)
+        run(t["x"], prompt, [y.clone() for y in caches])
+        fill = [torch.full((n,), 0x7E, dtype=torch.uint8, device=dev) for n in (B * N * 2, B * Hq * D * 2, B * Hkv * D * 2, 1 << 18, 1 << 21)]
+        run(x, want, c)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = run(t["x"], torch.empty_like(prompt), [y.clone() for y in c])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), rep
+        assert all(torch.equal(y, z) for y, z in zip(c, caches))
+        assert all(bool((f == 0x7E).all()) for f in fill)
+        del beside
+
+
 def test_two_streams_and_a_captured_first_call(dev):
     """One object on two streams at a time, and captured before it has ever run: every one of them with scratch of its own."""
     q, c, ln, *ref = _case(dev, 1, 1, 32, 8, 128, 4000, 4000, None, True, 0, 0, F16, True)

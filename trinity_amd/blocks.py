@@ -164,33 +164,23 @@ class CachedAttention:
 
 class CachedAttentionPlan:
     """AttentionPlan's block - [PreNorm,] Q/K/V projection, [QKNorm,] append, attention - for the next tokens of several
-    sequences over the caches of `CachedAttention`: X [batch * tokens, N], and what its methods take.  The projections' buffers
-    are the plan's own: calls of one plan, and graphs captured from it, run one after the other."""
+    sequences over the caches of `CachedAttention`: X [batch * tokens, N], and what its methods take.  A call's buffers come
+    from the allocator: prompts, single tokens and captured graphs of one plan share none."""
 
     def __init__(self, n_q_heads, n_kv_heads, head_dim, scale=None, causal=True, window=0, sinks=0, prenorm=False, qknorm=False,
                  eps=0.0):
         self.attention = CachedAttention(n_q_heads, n_kv_heads, head_dim, scale=scale, causal=causal, window=window, sinks=sinks)
         self.prenorm, self.qknorm, self.eps = prenorm, qknorm, eps
-        self._cache = {}
 
-    def _buf(self, key, rows, cols, like):
-        b = self._cache.get(key)
-        if b is None or b.shape != (rows, cols) or b.dtype != like.dtype or b.device != like.device:
-            self._cache[key] = b = torch.empty(rows, cols, dtype=like.dtype, device=like.device)
-        return b
-
-    def _project(self, name, X, W, norm):
+    def _project(self, X, W, norm):
         rows, cols = X.shape[0], W.shape[1]
         need = ext.gemm_workspace_bytes(rows, X.shape[1], cols)
-        ws = self._cache.get("ws")
-        if need and (ws is None or ws.numel() < need or ws.device != X.device):
-            self._cache["ws"] = ws = torch.empty(need, dtype=torch.uint8, device=X.device)
-        y = self._buf(name, rows, cols, X)
-        ext.matmul(X, W, None, y, ws if need else None)
+        y = X.new_empty(rows, cols)
+        ext.matmul(X, W, None, y, X.new_empty(need, dtype=torch.uint8) if need else None)
         if not norm:
             return y
         D = self.attention.head_dim
-        z = self._buf(name + "_norm", rows, cols, X)
+        z = torch.empty_like(y)
         ext.rmsnorm(y.view(-1, D), None, z.view(-1, D), self.eps)
         return z
 
@@ -199,13 +189,13 @@ class CachedAttentionPlan:
         if norm_w is not None and not self.prenorm:
             raise ValueError("a norm weight without PreNorm")
         if self.prenorm:
-            xn = self._buf("xn", X.shape[0], X.shape[1], X)
+            xn = X.new_empty(X.shape)
             ext.rmsnorm(X, norm_w, xn, self.eps)
             X = xn
-        K = self._project("k", X, WK, self.qknorm)
-        V = self._project("v", X, WV, False)
+        K = self._project(X, WK, self.qknorm)
+        V = self._project(X, WV, False)
         self.attention.append(K, V, k_cache, v_cache, k_scales, v_scales, lens=lens, kv_len=kv_len)
-        Q = self._project("q", X, WQ, self.qknorm)
+        Q = self._project(X, WQ, self.qknorm)
         return self.attention.attend(Q, k_cache, v_cache, k_scales, v_scales, lens=lens, kv_len=kv_len, out=O2, want_lse=want_lse)
 
 
