@@ -147,6 +147,9 @@ ATTN = [
     (3, 48, 32, 32, 64, 660, 653, [653, 640, 20], True, 0, 0),
     (3, 20, 96, 48, 128, 840, 840, [840, 100, 19], True, 0, 0),
     (3, 133, 16, 16, 128, 1672, 1672, [1672, 1500, 130], False, 0, 0),
+    (1, 100, 71, 1, 64, 1500, 1500, None, True, 0, 0),
+    (2, 66, 71, 1, 64, 420, 411, [411, 350], True, 97, 33),    # lists that end in either half of a tile, sinks into the second
+    (3, 129, 2, 1, 64, 290, 289, [289, 161, 130], True, 0, 0),
 ]
 
 

@@ -108,7 +108,7 @@ __device__ __forceinline__ void cache_wg_map(const CacheAttnArgs& a, int id, int
   hk = bh - b * a.Hkv;
 }
 
-// ---------------------------------------------------------------------------------------------------- many rows
+// ---------------------------------------------------------------------------------------------------- many rows, 128-wide heads
 // Four waves of 32 rows walk tiles of 64 keys.  Inside each wave the matrix pipe works on S^T of tile t + 1 while the
 // probabilities of tile t are computed, and on O^T of tile t while the maximum of tile t + 1 is found; a slot below holds
 // the MFMAs of one K or V fragment, the LDS read of a fragment PD slots ahead, and its share of the vector arithmetic.
@@ -119,28 +119,101 @@ __device__ __forceinline__ void cache_wg_map(const CacheAttnArgs& a, int id, int
 // KW = 2: eight waves, the four row groups twice, on every other tile each with buffers of their own; they merge through
 // LDS at the end.  For calls with one workgroup a CU at most, whose time is the chain of its tiles.
 //
-// What bounds it.  128-wide heads: the board's power limit, as the other attention kernels (a prompt of 4096 tokens over a
+// For 128-wide heads.  What bounds it: the board's power limit, as the other attention kernels (a prompt of 4096 tokens over a
 // 4-bit cache 133 us, 1.03 PFLOP/s, level with 16-bit rows: the conversion is hidden; matrix pipe busy 45 % of the time at the
 // clock that the limit leaves), and beside it some 9 us a round of workgroups for their first loads, the first tile's scores and
-// the stores (8192 tokens in a window of 1024, four rounds of 17 tiles, 160 us).  64-wide heads: the chain of a step, two waves
-// a SIMD that wait for LDS, matrix and exponential results a third of the time (two prompts of 1000 tokens, 71 heads, in 256:
-// 24 us, vector pipe 40 % busy, matrix pipe 12 %).  Measured and level: fixed offsets in place of an address per row, cheaper
-// masks, workgroups that start apart; slower: three buffers with loads two steps ahead (64-wide, 5 %), three waves a SIMD (they
-// spill, 12 %).
-template <int D>
+// the stores (8192 tokens in a window of 1024, four rounds of 17 tiles, 160 us).  Measured and level: fixed offsets in place of
+// an address per row, cheaper masks, workgroups that start apart.  Slower: a second copy of the step without the product after
+// the last tile (the registers spill, 33 to 57 %), a branch around each of its instructions (level, 4-bit 2 to 11 %), three waves
+// a SIMD on tiles of 32 keys as below for 64-wide heads (11 % to 30 %; 1.6 % faster for the window of 1024 in 16 bits).
 struct TilePipe {
+  static constexpr int D = 128;
   static constexpr int KSTEPS = D / 16, DT = D / 32;
   static constexpr int NKF = 2 * KSTEPS, NVF = 4 * DT;  // K / V fragments (MFMAs) per tile
   static constexpr int GPS = 16 / NKF, EPS = 32 / NVF;  // pairs of probabilities per S^T slot; scores per O^T slot
   static constexpr int PD = 3, RING = 4;
 };
 
-template <int D, bool FP4, int KW>
+// The end of a workgroup's rows: the states of the key ways merged, and the result stored.
+template <int D, int KW>
+__device__ __forceinline__ void tile_finish(const CacheAttnArgs& a, half_t* lds_all, int b, int hk, int run, int w0, int wave, int lane,
+                                            int kway, float m, float l, float16v (&o)[D / 32]) {
+  constexpr int DT = D / 32, CPR = D / 8;
+  const int l32 = lane & 31, g = lane >> 5, group = a.group, rows = a.rows;
+  const int row = w0 + l32, rowc = min(row, rows - 1), tok = row_token(a, rowc), head = hk * group + rowc - tok * group;
+  // ---- more ways: the others hand their state over, lane for lane, and leave
+  constexpr int REG = DT * 16 + 2;
+  float* const mg = reinterpret_cast<float*>(lds_all) + wave * REG * 64 + lane;
+  if constexpr (KW == 2) {
+    __syncthreads();  // (every wave is done with the tiles)
+    if (kway == 1) {
+      mg[0] = m;
+      mg[64] = l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mg[(2 + dt * 16 + e) * 64] = o[dt][e];
+    }
+    __syncthreads();
+    if (kway == 1) return;
+    const float m1 = mg[0], mn = fmaxf(m, m1);
+    const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mn);
+    m = mn;
+    l = l * a0 + mg[64] * a1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * a0 + mg[(2 + dt * 16 + e) * 64] * a1;
+  }
+
+  l = pair_sum(l);
+  if (a.runs == 1) {
+    // ---- a lane has sixteen pieces of 8 bytes of its row: stored as they are, every store instruction touches 32 lines, so
+    // each wave turns its rows around in LDS and stores whole ones, 16 bytes a lane
+    constexpr int LDO = D + 8;
+    static_assert(32 * LDO * 2 <= REG * 64 * 4, "two ways: in the place of the state that only this wave has read");
+    half_t* const stage = KW == 2 ? reinterpret_cast<half_t*>(mg - lane) : lds_all + wave * 32 * LDO;
+    if (KW == 1) __syncthreads();  // (every wave is done with the tiles)
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        half4v hv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hv[e] = (half_t)(o[dt][rq * 4 + e] * inv);
+        *reinterpret_cast<half4v*>(stage + l32 * LDO + dt * 32 + rq * 8 + g * 4) = hv;
+      }
+    if (a.lse != nullptr && g == 0 && row < rows)
+      a.lse[((int64_t)b * a.Hq + head) * a.S + tok] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    constexpr int RPI = 64 / CPR;  // rows per store instruction
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int r = i * RPI + lane / CPR, c = lane % CPR;
+      const half8v v = *reinterpret_cast<const half8v*>(stage + r * LDO + c * 8);
+      if (w0 + r < rows) {
+        const int tk = row_token(a, w0 + r), hd = hk * group + w0 + r - tk * group;
+        *reinterpret_cast<half8v*>(a.out + ((int64_t)b * a.S + tk) * a.ldo + (int64_t)hd * D + c * 8) = v;
+      }
+    }
+    return;
+  }
+  if (row >= rows) return;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq)
+      finish_row<D>(a, b, hk, row, run, dt * 8 + rq * 2 + g, m, l,
+                    float4v{o[dt][rq * 4], o[dt][rq * 4 + 1], o[dt][rq * 4 + 2], o[dt][rq * 4 + 3]});
+}
+
+template <bool FP4, int KW>
 __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, half_t* lds_all, const half_t* __restrict__ qglob) {
   // (qglob = a.q.  Inlined, every LDS access of this function carries "does not alias q", and an LDS read with alias
   // information is not made to wait for the loads to LDS in flight; barriers and explicit waits order those here.)
+  using P = TilePipe;
+  constexpr int D = P::D;
   using L = CacheLds<D>;
-  using P = TilePipe<D>;
   constexpr int KSTEPS = P::KSTEPS, DT = P::DT, NKF = P::NKF, NVF = P::NVF, GPS = P::GPS, EPS = P::EPS, PD = P::PD, RING = P::RING;
   constexpr int CPR = L::CPR;
   const int t = threadIdx.x & 255, lane = t & 63;  // of the way's four waves
@@ -174,9 +247,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
 
   // ---- tiles: a thread's pieces of 16 bytes (16-bit: chunks, 4-bit: blocks) and the row of the tile each is of
   constexpr int PPR = FP4 ? D / 32 : CPR;              // pieces per row
-  constexpr int NP = kCacheTile * PPR / 256;           // per thread (4-bit, D = 64: half the threads have one)
-  constexpr bool HALF = NP == 0;
-  constexpr int NPA = HALF ? 1 : NP;
+  constexpr int NP = kCacheTile * PPR / 256;           // per thread
   constexpr int ES = FP4 ? 1 : 2;
   const uint8_t* const kbase = static_cast<const uint8_t*>(a.kc.p) + (b * a.kc.sb + hk * a.kc.sh) * ES;
   const uint8_t* const vbase = static_cast<const uint8_t*>(a.vc.p) + (b * a.vc.sb + hk * a.vc.sh) * ES;
@@ -192,7 +263,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
     half_t* const dst = (isv ? vt : kt) + buf * L::HALFS;
 #pragma unroll
-    for (int i = 0; i < NPA; ++i) {
+    for (int i = 0; i < NP; ++i) {
       const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
       const uint8_t* src = (isv ? vbase : kbase) + key_of(step, r) * (isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src,
@@ -201,8 +272,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   };
   uint4v kraw, vraw;
   uint32_t kxraw = 0, vxraw = 0;
-  const int pr = (HALF ? t % 128 : t) / PPR, pc = (HALF ? t % 128 : t) % PPR;  // 4-bit: the thread's row and block (HALF: K for the first 128 threads, V for the others)
-  const bool has_k = !HALF || t < 128, has_v = !HALF || t >= 128;
+  const int pr = t / PPR, pc = t % PPR;  // 4-bit: the thread's row and block
   auto fetch4 = [&](int step, bool isv) {
     const int64_t key = key_of(step, pr);
     if (isv) {
@@ -215,9 +285,8 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   };
   auto commit4 = [&](int step, bool isv, int j) {  // chunk j of the block
     half_t* const dst = (isv ? vt : kt) + (step & 1) * L::HALFS;
-    if (isv ? has_v : has_k)
-      *reinterpret_cast<half8v*>(dst + pr * D + (((pc * 4 + j) ^ (isv ? L::fv(pr) : L::fk(pr))) << 3)) =
-          fp4x8_to_half8(isv ? vraw[j] : kraw[j], fp4_scale(isv ? vxraw : kxraw));
+    *reinterpret_cast<half8v*>(dst + pr * D + (((pc * 4 + j) ^ (isv ? L::fv(pr) : L::fk(pr))) << 3)) =
+        fp4x8_to_half8(isv ? vraw[j] : kraw[j], fp4_scale(isv ? vxraw : kxraw));
   };
 
   // ---- fragments: K fragment j = (16 channels j / 2, key half j % 2), V fragment v = (key half, key quarter, 32 channels)
@@ -441,7 +510,7 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
       meet();
     } else {  // K(0) is there, V(0) and K(1) may still be on their way
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * NPA));
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * NP));
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
@@ -466,76 +535,238 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
     }
   }
 
-  // ---- two ways: the second hands its state over, lane for lane, and leaves
-  constexpr int REG = DT * 16 + 2;
-  float* const mg = reinterpret_cast<float*>(lds_all) + wave * REG * 64 + lane;
-  if constexpr (KW == 2) {
-    __syncthreads();  // (every wave is done with the tiles)
-    if (kway == 1) {
-      mg[0] = m;
-      mg[64] = l;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mg[(2 + dt * 16 + e) * 64] = o[dt][e];
-    }
-    __syncthreads();
-    if (kway == 1) return;
-    const float m1 = mg[0], mn = fmaxf(m, m1);
-    const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mn);
-    m = mn;
-    l = l * a0 + mg[64] * a1;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * a0 + mg[(2 + dt * 16 + e) * 64] * a1;
-  }
+  tile_finish<D, KW>(a, lds_all, b, hk, run, w0, wave, lane, kway, m, l, o);
+}
 
-  l = pair_sum(l);
-  if (a.runs == 1) {
-    // ---- a lane has sixteen pieces of 8 bytes of its row: stored as they are, every store instruction touches 32 lines, so
-    // each wave turns its rows around in LDS and stores whole ones, 16 bytes a lane
-    constexpr int LDO = D + 8;
-    static_assert(32 * LDO * 2 <= REG * 64 * 4, "two ways: in the place of the state that only this wave has read");
-    half_t* const stage = KW == 2 ? reinterpret_cast<half_t*>(mg - lane) : lds + wave * 32 * LDO;
-    if (KW == 1) __syncthreads();  // (every wave is done with the tiles)
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+template <bool FP4, int KW>
+__global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_tile_kernel(CacheAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) half_t lds[KW * 4 * CacheLds<TilePipe::D>::HALFS];
+  cache_attn_tile_body<FP4, KW>(a, lds, a.q);
+}
+
+// ---------------------------------------------------------------------------------------------------- many rows, 64-wide heads
+// The same tiles, two buffers of each, K and V one step ahead, and a step without overlap inside a wave: scores of 32 keys, their
+// probabilities, their product with V.  A 64-wide head has half the matrix work per probability, so that what a SIMD lacks is not a
+// schedule but other waves: at 32 keys at a time a wave takes 103 registers (4-bit 111), and four of them, of four workgroups, share
+// a SIMD.  Halves of a tile that no row of the wave sees are skipped.  Against the pipelined step above with two waves a SIMD: two
+// prompts of 1000 tokens, 71 heads, in a window of 256 25.3 -> 20.1 us, 4096 in one of 1024 109.3 -> 96.8, one token against 8000 keys 9.6
+// -> 9.0; 64 keys at a time (119 registers) 22.8; three waves a SIMD 24.5.  4-bit tiles: a thread has one block, of K or of V.
+//
+// KW = 2: as above.
+template <bool FP4, int KW>
+__device__ __forceinline__ void cache_attn_waves_body(const CacheAttnArgs& a, half_t* lds_all, const half_t* __restrict__ qglob) {
+  constexpr int D = 64;
+  using L = CacheLds<D>;  // (qglob = a.q, as above)
+  constexpr int KSTEPS = D / 16, DT = D / 32, CPR = D / 8;
+  constexpr int HALFS = L::HALFS;
+  const int t = threadIdx.x & 255, lane = t & 63;  // of the way's four waves
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kway = KW == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  half_t* const lds = lds_all + kway * 4 * HALFS;
+  const int l32 = lane & 31, g = lane >> 5;
+  const int group = a.group, rows = a.rows;
+  int b, hk, rb, run;
+  cache_wg_map(a, (int)blockIdx.x, b, hk, rb, run);
+  const int r0 = rb * kCacheRows, w0 = r0 + wave * 32;
+  const KeyList kl = key_list(a, b, row_token(a, r0), row_token(a, min(r0 + kCacheRows, rows) - 1));
+  const int ntiles = (kl.n + kCacheTile - 1) / kCacheTile;
+  const int per = div_by(ntiles + a.runs - 1, a.by_runs), tile0 = min(run * per, ntiles);
+  const int tile1 = min(tile0 + per, ntiles), nsteps = (tile1 - tile0 + KW - 1) / KW;
+  auto tile_of = [&](int step) { return tile0 + step * KW + kway; };  // (may lie past the last one)
+
+  const int row = w0 + l32, rowc = min(row, rows - 1);
+  const int tok = row_token(a, rowc), head = hk * group + rowc - tok * group;
+  const int pos = kl.len - a.S + tok;
+  // positions of the wave's rows (it may have none)
+  const int pos0 = kl.len - a.S + row_token(a, min(w0, rows - 1)), pos1 = kl.len - a.S + row_token(a, min(w0 + 31, rows - 1));
+  // the wave's rows see list indices below this
+  const int seen = w0 >= rows ? 0 : min(tile1 * kCacheTile, a.causal ? min(kl.n, pos1 + 1 - kl.gap) : kl.n);
+
+  half8v qf[KSTEPS];
+  const half_t* qp = qglob + ((int64_t)b * a.S + tok) * a.ldq + (int64_t)head * D + g * 8;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+  for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *reinterpret_cast<const half8v*>(qp + ks * 16);
+
+  constexpr int ES = FP4 ? 1 : 2;
+  const uint8_t* const kbase = static_cast<const uint8_t*>(a.kc.p) + (b * a.kc.sb + hk * a.kc.sh) * ES;
+  const uint8_t* const vbase = static_cast<const uint8_t*>(a.vc.p) + (b * a.vc.sb + hk * a.vc.sh) * ES;
+  const int64_t ksr = a.kc.sr * ES, vsr = a.vc.sr * ES;
+  half_t *const kt = lds, *const vt = lds + 2 * HALFS;
+  // key of row r of a tile (past the last key: the last one again, whose scores are masked)
+  auto key_of = [&](int step, int r) {
+    const int li = min(tile_of(step) * kCacheTile + r, kl.n - 1);
+    return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
+  };
+  auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
+    half_t* const dst = (isv ? vt : kt) + buf * HALFS;
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        half4v hv;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) hv[e] = (half_t)(o[dt][rq * 4 + e] * inv);
-        *reinterpret_cast<half4v*>(stage + l32 * LDO + dt * 32 + rq * 8 + g * 4) = hv;
-      }
-    if (a.lse != nullptr && g == 0 && row < rows)
-      a.lse[((int64_t)b * a.Hq + head) * a.S + tok] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
-    constexpr int RPI = 64 / CPR;  // rows per store instruction
-#pragma unroll
-    for (int i = 0; i < 32 / RPI; ++i) {
-      const int r = i * RPI + lane / CPR, c = lane % CPR;
-      const half8v v = *reinterpret_cast<const half8v*>(stage + r * LDO + c * 8);
-      if (w0 + r < rows) {
-        const int tk = row_token(a, w0 + r), hd = hk * group + w0 + r - tk * group;
-        *reinterpret_cast<half8v*>(a.out + ((int64_t)b * a.S + tk) * a.ldo + (int64_t)hd * D + c * 8) = v;
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
+      const uint8_t* src = (isv ? vbase : kbase) + key_of(step, r) * (isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src,
+                                       (TRI_LDS void*)(dst + (i * 4 + wave) * 512), 16, 0, 0);
     }
-    return;
+  };
+  // 4-bit: a block per thread, of K in the first two waves, of V in the others
+  constexpr int BPR = D / 32;
+  const bool own_v = wave >= 2;
+  const int pr = t % 128 / BPR, pc = t % BPR;
+  const uint8_t* const own = own_v ? vbase : kbase;
+  const uint8_t* const own_x = FP4 ? (own_v ? a.vc.scales + b * a.vc.xb + hk * a.vc.xh : a.kc.scales + b * a.kc.xb + hk * a.kc.xh) : nullptr;
+  const int64_t own_sr = own_v ? vsr : ksr, own_xr = own_v ? a.vc.xr : a.kc.xr;
+  const int own_at = (own_v ? 2 * HALFS : 0) + pr * D, own_f = own_v ? L::fv(pr) : L::fk(pr);
+  uint4v raw;
+  uint32_t xraw = 0;
+  auto fetch4 = [&](int step) {
+    const int64_t key = key_of(step, pr);
+    raw = *reinterpret_cast<const uint4v*>(own + key * own_sr + pc * 16);
+    xraw = own_x[key * own_xr + pc];
+  };
+  auto commit4 = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<half8v*>(lds + own_at + buf * HALFS + (((pc * 4 + j) ^ own_f) << 3)) = fp4x8_to_half8(raw[j], fp4_scale(xraw));
+  };
+
+  int kbyte[KSTEPS], vbyte[DT];
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ++ks) {
+    kbyte[ks] = (l32 * D + (((ks * 2 + g) ^ L::fk(l32)) << 3)) * 2;
+    asm volatile("" : "+v"(kbyte[ks]));
   }
-  if (row >= rows) return;
+  const int j4 = (lane & 15) >> 2;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    vbyte[dt] = (int)(uint32_t)(uintptr_t)lds + (2 * HALFS + (4 * g + j4) * D + ((chunk ^ L::fv(j4)) << 3) + (lane & 1) * 4) * 2;
+    asm volatile("" : "+v"(vbyte[dt]));
+  }
+  const char* const ldsb = reinterpret_cast<const char*>(lds);
+  auto read_kf = [&](int par, int hf, int ks) {
+    return *reinterpret_cast<const half8v*>(ldsb + kbyte[ks] + (par * HALFS + hf * 32 * D) * 2);
+  };
+  auto read_vf = [&](int par, int hf, int v) {  // 16 keys v / DT, 32 channels v % DT
+    TRI_LDS char* vp = (TRI_LDS char*)(uintptr_t)(uint32_t)vbyte[v % DT] + (par * HALFS + (hf * 32 + (v / DT) * 16) * D) * 2;
+    const short4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TRI_LDS short4s*)vp);
+    const short4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TRI_LDS short4s*)(vp + 8 * D * 2));
+    half4v hl, hh;
+    __builtin_memcpy(&hl, &lo, 8);
+    __builtin_memcpy(&hh, &hi, 8);
+    return cat8(hl, hh);
+  };
+
+  const float c2 = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  float16v o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int rq = 0; rq < 4; ++rq)
-      finish_row<D>(a, b, hk, row, run, dt * 8 + rq * 2 + g, m, l,
-                    float4v{o[dt][rq * 4], o[dt][rq * 4 + 1], o[dt][rq * 4 + 2], o[dt][rq * 4 + 3]});
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  // Masks in terms of list indices: visible are those up to `last`, and of them those from `from` on or below a.sinks (in
+  // front of a gap all of these are sinks).
+  const int last = pos < 0 ? -1 : (a.causal ? min(pos - kl.gap, kl.n - 1) : kl.n - 1), from = a.window > 0 ? pos - a.window + 1 - kl.gap : 0;
+
+  auto step = [&](int st, auto parc) __attribute__((always_inline)) {
+    constexpr int PAR = decltype(parc)::value;
+    // this wave's share of the tiles is in LDS - 4-bit: written, lgkmcnt(0); 16-bit: landed, vmcnt(0) - and everybody's
+    asm volatile("" ::: "memory");
+    if constexpr (FP4) __builtin_amdgcn_s_waitcnt(0xC07F);
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if constexpr (!FP4) {
+      if (st + 1 < nsteps) {
+        load16(st + 1, false, PAR ^ 1);
+        load16(st + 1, true, PAR ^ 1);
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int li0 = tile_of(st) * kCacheTile + hf * 32, li1 = li0 + 31;
+      if (li0 >= seen) break;  // wave-uniform
+      float16v s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      half8v kf[KSTEPS];
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j) kf[j] = read_kf(PAR, hf, j);
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j) s = mfma32(kf[j], qf[j], s);
+      const int base = li0 + g * 4;  // the lane's scores are of indices base + (0 to 3) + 8 i
+      if (li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0)) {  // wave-uniform
+        asm volatile("");
+        const int end = last - base;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if ((r >> 2) * 8 + (r & 3) > end) s[r] = -INFINITY;
+      }
+      if (a.window > 0 && li0 + kl.gap <= pos1 - a.window && li1 >= a.sinks) {  // ... the window of some row begins here, or behind it
+        asm volatile("");
+        const int begin = from - base, sinks = a.sinks - base;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int c = (r >> 2) * 8 + (r & 3);
+          if (c < begin && c >= sinks) s[r] = -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      mx = pair_max(mx) * c2;
+      if (__builtin_amdgcn_ballot_w64(mx > m + kCacheLazyMax) != 0) {  // wave-uniform
+        const float mnew = fmaxf(m, mx);
+        const float alpha = mnew == -INFINITY ? 1.0f : fast_exp2(m - mnew);
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * alpha;
+      }
+      const float nm = m == -INFINITY ? 0.f : -m;
+      half8v pf[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = fast_exp2(fmaf(s[r], c2, nm));
+        sum += p;
+        pf[r / 8][r % 8] = (half_t)p;
+      }
+      l += sum;
+#pragma unroll
+      for (int v = 0; v < 2 * DT; ++v) o[v % DT] = mfma32(read_vf(PAR, hf, v), pf[v / DT], o[v % DT]);
+    }
+    if constexpr (FP4) {
+      commit4(PAR ^ 1);
+      fetch4(st + 2);  // (past the last step: its last keys again)
+    }
+  };
+
+  if (nsteps > 0) {
+    if constexpr (FP4) {
+      fetch4(0);
+      const uint4v r0v = raw;
+      const uint32_t x0 = xraw;
+      fetch4(1);
+      const uint4v r1v = raw;
+      const uint32_t x1 = xraw;
+      raw = r0v; xraw = x0;
+      commit4(0);
+      raw = r1v; xraw = x1;
+    } else {
+      load16(0, false, 0);
+      load16(0, true, 0);
+    }
+    for (int st = 0; st < nsteps; st += 2) {
+      step(st, std::integral_constant<int, 0>{});
+      if (st + 1 < nsteps) step(st + 1, std::integral_constant<int, 1>{});
+    }
+  }
+  tile_finish<D, KW>(a, lds_all, b, hk, run, w0, wave, lane, kway, m, l, o);
 }
 
-template <int D, bool FP4, int KW>
-__global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_tile_kernel(CacheAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) half_t lds[KW * 4 * CacheLds<D>::HALFS];
-  cache_attn_tile_body<D, FP4, KW>(a, lds, a.q);
+template <bool FP4, int KW>
+__global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(4, 4))) void cache_attn_waves_kernel(CacheAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) half_t lds[KW * 4 * CacheLds<64>::HALFS];
+  cache_attn_waves_body<FP4, KW>(a, lds, a.q);
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows
@@ -549,7 +780,7 @@ __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // it out of the last-level cache where the call is repeated), 16 in a window of 4096 in 16 bits 41 us for 268 MB (6.5).  Short
 // ones are latency: one sequence of 4096 keys 5.2 us and 3.4 of merge.  48 and 64 rows this way, with four waves on a CU, are
 // slower than the kernel of many rows (64 rows of 8 KV heads against 16000 keys 23.7 us, 21.9 there; 71 of 64-wide against 8000
-// 10.8 and 9.8).
+// 10.8 and 9.0).
 constexpr int kFewRowTile = 32;   // keys
 
 template <int D>
@@ -945,13 +1176,13 @@ constexpr int kFewRowAlone4 = 5, kFewRowAlone16 = 3, kFewRowAloneMany = 8, kFewR
 // way to memory and back.  (8 KV heads of 128 in 4 bits: 64 tokens against 2000 keys in 4 / 8 / 16 / 32 runs 21.1 / 18.5 / 21.7 /
 // 30.5 us, two ways in eight 19.4; 512 against 16512 in 2 / 4 / 8 202 / 164 / 175, two ways in two 165; 128 against 8000 in sixteen
 // 39.6, two ways in eight 37.6; a prompt of 1024, one way / two 27.0 / 24.7, in 16 bits 28.3 / 23.6; two of 400 against 3000 keys 58.3
-// in two runs / 53.7.  71 heads of 64 on one: one token against 8000 in 16 / 32 / 64 15.6 / 11.8 / 10.3, 100 in eight 39.0, two
-// ways in four 36.8.)
+// in two runs / 53.7.  71 heads of 64 on one in 16 bits: one token against 8000 in 24 / 32 / 48 / 64 12.2 / 10.3 / 9.5 / 8.6, 33 in
+// 24 22.7, two ways in twelve 20.3, 100 in eight 35.3, two ways in four 33.2.)
 struct TileUs {
   float alone, beside, pair;
 };
 constexpr TileUs tile_us(int D, bool four_bit) {
-  return D == 64 ? TileUs{1.0f, 1.5f, 1.55f} : TileUs{1.2f, 2.0f, four_bit ? 2.25f : 1.95f};
+  return D == 64 ? TileUs{0.9f, 1.25f, 1.3f} : TileUs{1.2f, 2.0f, four_bit ? 2.25f : 1.95f};
 }
 constexpr float kTileFixedUs = 5.0f, kTileMergeUs = 7.8f, kTilePairFixedUs = 1.0f, kTilePartBytesPerUs = 4.1e6f;
 constexpr int kTileRound = 512;  // workgroups at a time, two a CU
@@ -1012,8 +1243,13 @@ template <int D, bool FP4>
 static void launch_t(const CacheAttnArgs& a, int nt, int ways, unsigned nwg, hipStream_t stream) {
   if (nt == 1) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
   else if (nt == 2) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 2>), dim3(nwg), dim3(256), 0, stream, a);
-  else if (ways == 2) hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4, 2>), dim3(nwg), dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((cache_attn_tile_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
+  else if constexpr (D == 64) {
+    if (ways == 2) hipLaunchKernelGGL((cache_attn_waves_kernel<FP4, 2>), dim3(nwg), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((cache_attn_waves_kernel<FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
+  } else {
+    if (ways == 2) hipLaunchKernelGGL((cache_attn_tile_kernel<FP4, 2>), dim3(nwg), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((cache_attn_tile_kernel<FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
+  }
 }
 
 template <int D>
