@@ -690,8 +690,13 @@ __device__ __forceinline__ void cache_attn_waves_body(const CacheAttnArgs& a, ha
       half8v kf[KSTEPS];
 #pragma unroll
       for (int j = 0; j < KSTEPS; ++j) kf[j] = read_kf(PAR, hf, j);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < KSTEPS; ++j) s = mfma32(kf[j], qf[j], s);
+      half8v vf[2 * DT];
+#pragma unroll
+      for (int v = 0; v < 2 * DT; ++v) vf[v] = read_vf(PAR, hf, v);
+      __builtin_amdgcn_sched_barrier(0);
       const int base = li0 + g * 4;  // the lane's scores are of indices base + (0 to 3) + 8 i
       if (li1 >= kl.n || pos0 < 0 || (a.causal && li1 + kl.gap > pos0)) {  // wave-uniform
         asm volatile("");
@@ -732,7 +737,7 @@ __device__ __forceinline__ void cache_attn_waves_body(const CacheAttnArgs& a, ha
       }
       l += sum;
 #pragma unroll
-      for (int v = 0; v < 2 * DT; ++v) o[v % DT] = mfma32(read_vf(PAR, hf, v), pf[v / DT], o[v % DT]);
+      for (int v = 0; v < 2 * DT; ++v) o[v % DT] = mfma32(vf[v], pf[v / DT], o[v % DT]);
     }
     if constexpr (FP4) {
       commit4(PAR ^ 1);
