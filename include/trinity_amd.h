@@ -287,7 +287,7 @@ int tri_validate_roco(const tri_tensor* x, const tri_tensor* norm_w, const tri_t
  * Tensors:
  *   16-bit caches  [batch, n_kv_heads, rows >= kv_len, D] (or without the first dimension where batch is 1), of the call's
  *                  element type; scales NULL.  Any strides that are multiples of 8, the innermost 1 (a [batch, rows,
- *                  heads, D] cache is passed as its transposed view).
+ *                  heads, D] cache is passed as its transposed view), those of rows under 2^30 here and below.
  *   4-bit caches   TRI_U8 [batch, n_kv_heads, rows, D / 2], strides multiples of 16, with scales TRI_U8 [batch, n_kv_heads,
  *                  rows, D / 32], strides multiples of D / 32.  The OCP microscaling format: 32 consecutive channels share
  *                  a power of two 2^e, stored as the byte e + 127 (255: the block is NaN; bytes 1 to 254 are read as they

@@ -90,6 +90,18 @@ def test_parameters():
         ext.native().cache_scratch_bytes(ext.attn_params(2, 2, 64, 1), 0)
 
 
+def test_row_strides_of_2_30():
+    p, q = _params(batch=1, n_kv_heads=1, n_q_heads=1, seq=1, kv_len=1), _h(1, D)
+    for rows, want in ((1, 0), (2, UNSUPPORTED)):  # one row has none
+        near = _h(1, 1, rows, D)
+        far = ext.as_tri(near)
+        far.stride[2] = 1 << 30
+        assert _attend(p, q=q, out=q, k_cache=near, v_cache=near) == 0
+        assert _attend(p, q=q, out=q, k_cache=far, v_cache=near) == _attend(p, q=q, out=q, k_cache=near, v_cache=far) == want
+        far.stride[2] = (1 << 30) - 8
+        assert _attend(p, q=q, out=q, k_cache=far, v_cache=near) == 0
+
+
 def test_more_heads_than_a_launch_has_workgroups():
     many = _params(batch=1 << 23, n_kv_heads=2, n_q_heads=2, seq=1)
     assert _attend(many) == UNSUPPORTED

@@ -378,7 +378,7 @@ int check_cache4(const tri_tensor* t, int64_t B, int64_t H, int64_t rows, bool e
   const int64_t* st = t->stride + (t->ndim - 3);
   if ((t->ndim == 4 && t->shape[0] != B) || sh[0] != H || sh[2] != n) return TRI_ERR_SHAPE;
   if (exact_rows ? sh[1] != rows : sh[1] < rows) return TRI_ERR_SHAPE;
-  if (sh[1] >= kInt32End) return TRI_ERR_UNSUPPORTED;
+  if (sh[1] >= kInt32End || (sh[1] > 1 && st[1] >= (1 << 30))) return TRI_ERR_UNSUPPORTED;
   if (B == 0 || sh[1] == 0) return TRI_OK;  // no elements: no storage
   if (t->ptr == nullptr) return TRI_ERR_NULL;
   if (st[2] != 1) return TRI_ERR_STRIDE;

@@ -31,6 +31,9 @@ constexpr float kCacheLazyMax = 8.0f;
 __device__ __forceinline__ int div_by(int n, CacheDiv d) { return (int)(__umulhi((uint32_t)n << 4, d.mul) >> d.sh); }
 __device__ __forceinline__ int row_token(const CacheAttnArgs& a, int row) { return div_by(row, a.by_group); }
 
+// offset of a key's row: row strides are less than 2^31 bytes, so that this is one product of 32 bits and not three
+__device__ __forceinline__ uint64_t row_at(int key, int64_t stride) { return (uint64_t)(uint32_t)key * (uint32_t)stride; }
+
 // what a row block of a sequence sees
 struct KeyList {
   int len;        // keys of the sequence
@@ -258,14 +261,14 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   // key of row r of a tile (past the last key: the last one again, whose scores are masked)
   auto key_of = [&](int step, int r) {
     const int li = min(tile_of(step) * kCacheTile + r, kl.n - 1);
-    return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
+    return li + (li < kl.sinks ? 0 : kl.gap);
   };
   auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
     half_t* const dst = (isv ? vt : kt) + buf * L::HALFS;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
-      const uint8_t* src = (isv ? vbase : kbase) + key_of(step, r) * (isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
+      const uint8_t* src = (isv ? vbase : kbase) + row_at(key_of(step, r), isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src,
                                        (TRI_LDS void*)(dst + (i * 4 + wave) * 512), 16, 0, 0);
     }
@@ -274,13 +277,13 @@ __device__ __forceinline__ void cache_attn_tile_body(const CacheAttnArgs& a, hal
   uint32_t kxraw = 0, vxraw = 0;
   const int pr = t / PPR, pc = t % PPR;  // 4-bit: the thread's row and block
   auto fetch4 = [&](int step, bool isv) {
-    const int64_t key = key_of(step, pr);
+    const int key = key_of(step, pr);
     if (isv) {
-      vraw = *reinterpret_cast<const uint4v*>(vbase + key * vsr + pc * 16);
-      vxraw = vxbase[key * a.vc.xr + pc];
+      vraw = *reinterpret_cast<const uint4v*>(vbase + row_at(key, vsr) + pc * 16);
+      vxraw = vxbase[row_at(key, a.vc.xr) + pc];
     } else {
-      kraw = *reinterpret_cast<const uint4v*>(kbase + key * ksr + pc * 16);
-      kxraw = kxbase[key * a.kc.xr + pc];
+      kraw = *reinterpret_cast<const uint4v*>(kbase + row_at(key, ksr) + pc * 16);
+      kxraw = kxbase[row_at(key, a.kc.xr) + pc];
     }
   };
   auto commit4 = [&](int step, bool isv, int j) {  // chunk j of the block
@@ -595,14 +598,14 @@ __device__ __forceinline__ void cache_attn_waves_body(const CacheAttnArgs& a, ha
   // key of row r of a tile (past the last key: the last one again, whose scores are masked)
   auto key_of = [&](int step, int r) {
     const int li = min(tile_of(step) * kCacheTile + r, kl.n - 1);
-    return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
+    return li + (li < kl.sinks ? 0 : kl.gap);
   };
   auto load16 = [&](int step, bool isv, int buf) {  // 16-bit: to LDS, 1 KB an instruction
     half_t* const dst = (isv ? vt : kt) + buf * HALFS;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int p = i * 256 + t, r = p / CPR, slot = p % CPR;
-      const uint8_t* src = (isv ? vbase : kbase) + key_of(step, r) * (isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
+      const uint8_t* src = (isv ? vbase : kbase) + row_at(key_of(step, r), isv ? vsr : ksr) + (slot ^ (isv ? L::fv(r) : L::fk(r))) * 16;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)src,
                                        (TRI_LDS void*)(dst + (i * 4 + wave) * 512), 16, 0, 0);
     }
@@ -618,9 +621,9 @@ __device__ __forceinline__ void cache_attn_waves_body(const CacheAttnArgs& a, ha
   uint4v raw;
   uint32_t xraw = 0;
   auto fetch4 = [&](int step) {
-    const int64_t key = key_of(step, pr);
-    raw = *reinterpret_cast<const uint4v*>(own + key * own_sr + pc * 16);
-    xraw = own_x[key * own_xr + pc];
+    const int key = key_of(step, pr);
+    raw = *reinterpret_cast<const uint4v*>(own + row_at(key, own_sr) + pc * 16);
+    xraw = own_x[row_at(key, own_xr) + pc];
   };
   auto commit4 = [&](int buf) {
 #pragma unroll
@@ -886,18 +889,18 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
     }
     auto key_of = [&](int r) {  // (past the last key: the last one again, whose scores are masked)
       const int li = min(li0 + r, kl.n - 1);
-      return (int64_t)(li + (li < kl.sinks ? 0 : kl.gap));
+      return li + (li < kl.sinks ? 0 : kl.gap);
     };
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const int64_t key = key_of(kb * 16 + l16);
-      fetch_k(x, kb, kbase, kxbase, key * ksr + g * KPB, FP4 ? key * a.kc.xr + (D == 128 ? g : g / 2) : 0);
+      const int key = key_of(kb * 16 + l16);
+      fetch_k(x, kb, kbase, kxbase, row_at(key, ksr) + g * KPB, FP4 ? row_at(key, a.kc.xr) + (D == 128 ? g : g / 2) : 0);
     }
 #pragma unroll
     for (int i = 0; i < T::VP; ++i) {
       const int p = i * 64 + lane, r = p / T::VPR, c = p % T::VPR;
-      const int64_t key = key_of(r);
-      fetch_v(x, i, vbase, vxbase, key * vsr + c * 16, FP4 ? key * a.vc.xr + c : 0);
+      const int key = key_of(r);
+      fetch_v(x, i, vbase, vxbase, row_at(key, vsr) + c * 16, FP4 ? row_at(key, a.vc.xr) + c : 0);
     }
   };
 
