@@ -550,10 +550,11 @@ __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ---------------------------------------------------------------------------------------------------- many rows, 64-wide heads
 // The same tiles, two buffers of each, K and V one step ahead, and a step without overlap inside a wave: scores of 32 keys, their
 // probabilities, their product with V.  A 64-wide head has half the matrix work per probability, so that what a SIMD lacks is not a
-// schedule but other waves: at 32 keys at a time a wave takes 103 registers (4-bit 111), and four of them, of four workgroups, share
+// schedule but other waves: at 32 keys at a time a wave takes 114 registers (4-bit 122), and four of them, of four workgroups, share
 // a SIMD.  Halves of a tile that no row of the wave sees are skipped.  Against the pipelined step above with two waves a SIMD: two
-// prompts of 1000 tokens, 71 heads, in a window of 256 25.3 -> 20.1 us, 4096 in one of 1024 109.3 -> 96.8, one token against 8000 keys 9.6
-// -> 9.0; 64 keys at a time (119 registers) 22.8; three waves a SIMD 24.5.  4-bit tiles: a thread has one block, of K or of V.
+// prompts of 1000 tokens, 71 heads, in a window of 256 25.3 -> 20.0 us, 4096 in one of 1024 109.3 -> 95.8, one token against 8000 keys 9.6
+// -> 8.9; 64 keys at a time (119 registers) 22.8; three waves a SIMD 24.5; five spill.  Level: the waves' priority raised for the
+// products.  4-bit tiles: a thread has one block, of K or of V.
 //
 // KW = 2: as above.
 template <bool FP4, int KW>
@@ -857,9 +858,9 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
     if constexpr (FP4) x.vx[i] = vxp[xoff];
   };
   // 4 bits: tiles of neighbouring rows (all but the list's last one and that with the end of the sinks) are addressed by the
-  // tile's place, the same for the wave, and fixed offsets; an address per row is two products of 64 bits, and there are eight
-  // of them to a tile (32 sequences of up to 8192 keys 41.2 -> 39.8 us; 16-bit tiles, four times the bytes, are 2 % slower so,
-  // and in the kernel of many rows it is level, too: that one is bound elsewhere)
+  // tile's place, the same for the wave, and fixed offsets in place of an address per row, eight of them a tile (32 sequences of
+  // up to 8192 keys 41.2 -> 40.2 us; 16-bit tiles, four times the bytes, are 2 % slower so, and in the kernel of many rows it is
+  // level, too: that one is bound elsewhere)
   const bool flat = FP4 && (uint64_t)ksr * kFewRowTile < (1u << 31) && (uint64_t)vsr * kFewRowTile < (1u << 31) &&
                     (uint64_t)a.kc.xr * kFewRowTile < (1u << 31) && (uint64_t)a.vc.xr * kFewRowTile < (1u << 31);
   constexpr int KPB = FP4 ? D / 8 : 16;  // bytes of a key that a lane takes at a time
