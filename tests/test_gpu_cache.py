@@ -138,9 +138,14 @@ ATTN = [
     (1, 1, 8, 2, 128, 640, 640, None, True, 0, 0),             # few rows: one run in 4 bits, several in 16
     (33, 1, 4, 4, 64, 1300, 1300, [1300 - 40 * i for i in range(33)], True, 0, 0),  # many heads: 1024 keys and fewer in one run
     (33, 1, 4, 4, 64, 900, 900, [900 - 27 * i for i in range(33)], True, 0, 0),
-    (1, 8, 16, 4, 64, 2000, 1990, None, True, 0, 0),           # column tiles of 16 rows: two of them
+    (1, 8, 16, 4, 64, 2000, 1990, None, True, 0, 0),
     (2, 8, 16, 4, 64, 200, 200, [200, 91], True, 60, 4),
     (1, 8, 16, 4, 128, 200, 200, None, True, 0, 0),
+    # column tiles of 16 rows, two of them (4 bits, many keys of all KV heads together), in one run and in several
+    (43, 8, 18, 6, 64, 520, 513, [513 - 11 * i for i in range(43)], True, 0, 0),
+    (33, 5, 32, 8, 128, 500, 498, [498 - 15 * i for i in range(33)], True, 0, 0),
+    (2, 3, 16, 2, 64, 33100, 33000, [33000, 20001], True, 0, 0),
+    (1, 8, 6, 2, 128, 65700, 65667, None, True, 0, 0),
     # two key ways: in one run and in several
     (1, 48, 48, 48, 64, 329, 329, None, True, 0, 0),
     (2, 155, 8, 8, 64, 340, 339, [339, 150], True, 200, 3),

@@ -1168,7 +1168,13 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
 }
 
 // ---- which kernel, and in how many runs
-constexpr int kFewRowsMost = 32;  // stacked rows of a KV head, up to which the kernel of few rows runs
+// The kernel of few rows runs up to 16 stacked rows of a KV head (16 rows, tile kernels / few rows: 8 KV heads of 128 against 16000
+// keys in 4 bits 12.3 / 9.5 us, in 16 12.7 / 11.2), and up to 32 in 4 bits where there is enough to read that its rate counts, and not
+// its latency, KV heads times keys (32 rows of 128 in 4 bits: 64 x 1024 12.7 / 15.2, 8 x 16000 17.8 / 18.9, 64 x 2048 17.8 / 18.9, 256 x
+// 512 14.1 / 12.0, 128 x 1024 18.5 / 16.2, 32 x 8000 22.7 / 20.9, 256 x 2000 34.6 / 24.7; 64-wide 9.6 / 10.4, 12.2 / 11.9, 12.2 / 11.6, 10.1 / 8.5,
+// 12.2 / 10.9, 16.2 / 14.2, 26.8 / 16.9; in 16 bits 64 x 1024 13.0 / 15.9, 64 x 4000 27.9 / 29.3, 256 x 2000 44.3 / 45.8).
+constexpr int kFewRowsMost = 16, kFewRowsMost4 = 32;
+constexpr int64_t kFewRowsMost4Keys = 1 << 17;
 constexpr int kCacheMaxRuns = 64;
 // Few rows: as many runs as give 512 workgroups (eight waves a CU), of at least four tiles, one a wave (8 KV heads in 4 bits,
 // 512 / 256 / 1024 workgroups: 32 sequences of 8192 keys 41.0 / 54.6 / 41.1 us, 8 of 4000 11.7 / 13.1 / 14.5; one of 4096, 128 /
@@ -1201,7 +1207,9 @@ CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int windo
   const int64_t heads = (int64_t)B * Hkv;
   CachePlan p{};
   p.ways = 1;
-  p.nt = rows <= kFewRowsMost ? (rows + 15) / 16 : 0;
+  const int64_t few_keys = window > 0 && (int64_t)S + window + sinks < kv_len ? (int64_t)S + window + sinks : kv_len;
+  const bool most4 = four_bit && heads * few_keys >= kFewRowsMost4Keys;
+  p.nt = rows <= (most4 ? kFewRowsMost4 : kFewRowsMost) ? (rows + 15) / 16 : 0;
   p.nwg = p.nt > 0 ? heads : (rows + kCacheRows - 1) / kCacheRows * heads;
   // most keys of a row block
   const int64_t toks = p.nt > 0 ? S : (kCacheRows + group - 1) / group + 1;
@@ -1250,9 +1258,17 @@ int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_
 
 template <int D, bool FP4>
 static void launch_t(const CacheAttnArgs& a, int nt, int ways, unsigned nwg, hipStream_t stream) {
-  if (nt == 1) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
-  else if (nt == 2) hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 2>), dim3(nwg), dim3(256), 0, stream, a);
-  else if constexpr (D == 64) {
+  if (nt == 1) {
+    hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
+    return;
+  }
+  if constexpr (FP4) {
+    if (nt == 2) {
+      hipLaunchKernelGGL((cache_attn_few_kernel<D, FP4, 2>), dim3(nwg), dim3(256), 0, stream, a);
+      return;
+    }
+  }
+  if constexpr (D == 64) {
     if (ways == 2) hipLaunchKernelGGL((cache_attn_waves_kernel<FP4, 2>), dim3(nwg), dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((cache_attn_waves_kernel<FP4, 1>), dim3(nwg), dim3(256), 0, stream, a);
   } else {
