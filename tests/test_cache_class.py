@@ -1,0 +1,56 @@
+"""blocks.CachedAttention on the CPU: what it owns, and what it hands to the compiled binding (a stand-in of it here, as
+nothing may be launched)."""
+import threading
+
+import torch
+
+from trinity_amd import blocks, ext
+
+
+class _Binding:
+    """cache_attend as the binding has it, without the launches; `meet`: calls wait for one another while they hold their scratch."""
+
+    def __init__(self):
+        self.meet, self.held = None, []
+
+    def cache_attend(self, q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, params, stream):
+        if scratch is None or scratch.numel() < 64:
+            return 64
+        if self.meet is not None:
+            self.meet.wait(timeout=30)
+            self.held.append(scratch.data_ptr())
+            self.meet.wait(timeout=30)
+        return q
+
+
+def test_calls_in_flight_never_hold_one_buffer(monkeypatch):
+    """The binding gives up the interpreter lock between the two launches of a call: what the first leaves in its scratch is
+    that call's until the second is behind it."""
+    binding = _Binding()
+    monkeypatch.setattr(ext, "native", lambda: binding)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    op = blocks.CachedAttention(2, 2, 64)
+    q, c = torch.zeros(1, 128), torch.zeros(1, 2, 4, 64)
+    op.attend(q, c, c)
+    assert len(op._scratch) == 1
+    binding.meet = threading.Barrier(3)
+    failed = []
+
+    def call():
+        try:
+            op.attend(q, c, c)
+        except Exception as e:  # (a broken barrier, for instance)
+            failed.append(e)
+
+    threads = [threading.Thread(target=call) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    assert len(set(binding.held)) == 3
+    assert len(op._scratch) == 1  # one of them is kept
+    binding.meet = None
+    kept = next(iter(op._scratch.values()))
+    op.attend(q, c, c)
+    assert next(iter(op._scratch.values())) is kept

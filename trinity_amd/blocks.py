@@ -105,7 +105,7 @@ class CachedAttention:
     with fewer has its first rows as padding.  `kv_len` (None: all rows of the cache) bounds the lengths.
 
     An object keeps a scratch buffer for every stream it attends on; a call under graph capture takes one of the graph's own, so
-    that graphs share none."""
+    that graphs share none, and calls of several threads on one stream take one each."""
 
     def __init__(self, n_q_heads, n_kv_heads, head_dim, scale=None, causal=True, window=0, sinks=0):
         self.head_dim = head_dim
@@ -146,19 +146,22 @@ class CachedAttention:
         """Q [batch * tokens, query heads * head_dim] over the caches, which hold the tokens' own keys already.  Returns
         the output like Q, and with `want_lse` the log-sum-exp [batch, query heads, tokens] beside it."""
         stream = ext._stream_or_none(Q)
-        scratch = self._scratch.get(stream)
-        capturing = scratch is not None and torch.cuda.is_current_stream_capturing()
-        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, None if capturing else scratch, out, want_lse,
+        # The buffer leaves the object for the time of a call: its two launches (parts of the keys, their merge) are enqueued
+        # without the interpreter lock, and another thread's call on the stream, which may enqueue its own between them, finds none.
+        kept = self._scratch.pop(stream, None)
+        capturing = kept is not None and torch.cuda.is_current_stream_capturing()
+        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, None if capturing else kept, out, want_lse,
                                       kv_len, self._p, stream)
+        if type(r) is int and r > 0:  # bytes of scratch: the first call of its size, or a captured one
+            scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
+            if not torch.cuda.is_current_stream_capturing():
+                kept = scratch
+            r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, self._p,
+                                          stream)
+        if kept is not None:
+            self._scratch[stream] = kept
         if type(r) is int:
-            if r > 0:  # bytes of scratch: the first call of its size, or a captured one
-                scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
-                if not torch.cuda.is_current_stream_capturing():
-                    self._scratch[stream] = scratch
-                r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, self._p,
-                                              stream)
-            if type(r) is int:
-                ext._check("tri_cache_attention", r)
+            ext._check("tri_cache_attention", r)
         return r
 
 
