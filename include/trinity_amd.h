@@ -334,9 +334,10 @@ int tri_validate_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scale
 
 /* out = softmax(scale * q.K^T over the keys that each token sees).V, from caches that hold the call's tokens already.
  *   q, out [batch * seq, n_q_heads * D]; lse fp32 [batch, n_q_heads, seq] contiguous or NULL: the natural log-sum-exp.
- * A row without a visible key (padding) gets zeros, and -inf as its lse.  scratch: 1-D TRI_U8, 256-byte aligned, or NULL;
- * with tri_cache_scratch_bytes the call runs its fastest plan, with less (or none) it cuts the key axis into
- * fewer parts - same results to rounding.  The size does not depend on the lengths below kv_len. */
+ * A row without a visible key (padding) gets zeros, and -inf as its lse, whatever the values that other rows see.
+ * scratch: 1-D TRI_U8, 256-byte aligned, or NULL; with tri_cache_scratch_bytes the call runs its fastest plan, with less
+ * (or none) it cuts the key axis into fewer parts - same results to rounding.  The size does not depend on the lengths
+ * below kv_len. */
 int64_t tri_cache_scratch_bytes(const tri_cache_params* p, int32_t four_bit);
 int tri_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales /* nullable */,
                         const tri_tensor* v_cache, const tri_tensor* v_scales /* nullable */,
