@@ -2,6 +2,7 @@
 nothing may be launched)."""
 import threading
 
+import pytest
 import torch
 
 from trinity_amd import blocks, ext
@@ -54,3 +55,24 @@ def test_calls_in_flight_never_hold_one_buffer(monkeypatch):
     kept = next(iter(op._scratch.values()))
     op.attend(q, c, c)
     assert next(iter(op._scratch.values())) is kept
+
+
+def test_int32_tensors_are_lengths_alone():
+    """They came with the lengths of sequences; every other place of every call refuses them as it did before."""
+    i32, h = torch.zeros(0, 64, dtype=torch.int32), torch.zeros(0, 64, dtype=torch.float16)
+    w = torch.zeros(64, 64, dtype=torch.float16)
+    with pytest.raises(TypeError):
+        ext.as_tri(i32)
+    for call in (lambda x: ext.rmsnorm(x, None, h, validate_only=True), lambda x: ext.native().rmsnorm(x, None, h, 1e-5, 0),
+                 lambda x: ext.native().matmul(x, w, None, h, None, 0), lambda x: ext.native().gateup_swiglu(h, w, w, x, None, 0)):
+        with pytest.raises(TypeError):
+            call(i32)
+    cache, lens = torch.zeros(1, 1, 4, 64, dtype=torch.float16), torch.zeros(1, dtype=torch.int32)
+    p = ext.cache_params(1, 1, 64, 0, 4)
+    args = [h, cache, None, cache, None, lens, None, None, h]
+    assert ext.cache_attention(*args, p, validate_only=True) == 0
+    for i in (0, 1, 3, 6, 7, 8):
+        with pytest.raises(TypeError):
+            ext.cache_attention(*args[:i], i32, *args[i + 1:], p, validate_only=True)
+        with pytest.raises(TypeError):
+            ext.native().cache_attention(*args[:i], i32, *args[i + 1:], p, 0)

@@ -24,8 +24,8 @@ struct Tensors {
   tri_tensor* p[kMaxTensors];
 };
 
-// a[i] = tensor, None, or a tensor's descriptor as ext.as_tri makes it
-bool to_tri(PyObject* o, tri_tensor& v, tri_tensor*& p) {
+// o = tensor, None, or a tensor's descriptor as ext.as_tri makes it; int32 tensors are lengths and nothing else
+bool to_tri(PyObject* o, tri_tensor& v, tri_tensor*& p, bool lengths) {
   if (o == Py_None) {
     p = nullptr;
     return true;
@@ -50,8 +50,13 @@ bool to_tri(PyObject* o, tri_tensor& v, tri_tensor*& p) {
     case at::kFloat: v.dtype = TRI_F32; break;
     case at::kByte: v.dtype = TRI_U8; break;
     case at::kFloat8_e4m3fn: v.dtype = TRI_FP8_E4M3; break;
-    case at::kInt: v.dtype = TRI_I32; break;
-    default: PyErr_Format(PyExc_TypeError, "unsupported dtype %s", at::toString(t.scalar_type())); return false;
+    default:
+      if (lengths && t.scalar_type() == at::kInt) {
+        v.dtype = TRI_I32;
+        break;
+      }
+      PyErr_Format(PyExc_TypeError, "unsupported dtype %s", at::toString(t.scalar_type()));
+      return false;
   }
   const int64_t nd = t.dim();
   if (nd > 4) {
@@ -68,13 +73,14 @@ bool to_tri(PyObject* o, tri_tensor& v, tri_tensor*& p) {
   return true;
 }
 
-bool marshal(PyObject* const* args, Py_ssize_t nargs, int ntensors, int nscalars, Tensors& t) {
+// lens_at: which of the tensors holds lengths of sequences
+bool marshal(PyObject* const* args, Py_ssize_t nargs, int ntensors, int nscalars, Tensors& t, int lens_at = -1) {
   if (nargs != ntensors + nscalars + 1) {
     PyErr_Format(PyExc_TypeError, "expected %d arguments, got %zd", ntensors + nscalars + 1, nargs);
     return false;
   }
   for (int i = 0; i < ntensors; ++i) {
-    if (!to_tri(args[i], t.v[i], t.p[i])) return false;
+    if (!to_tri(args[i], t.v[i], t.p[i], i == lens_at)) return false;
   }
   return true;
 }
@@ -241,7 +247,7 @@ TRI_BIND(roco) {  // (as_mean_var comes before the parameters, as in the C entry
 TRI_BIND(cache_append) {
   return run([&] {
     Tensors t;
-    if (!marshal(a, n, 7, 1, t)) return 0;
+    if (!marshal(a, n, 7, 1, t, 6)) return 0;
     const OneDevice device(a, 7);
     if (!device.ok) return 0;
     const CacheParams p(a[7]);
@@ -252,7 +258,7 @@ TRI_BIND(cache_append) {
 TRI_BIND(cache_read) {
   return run([&] {
     Tensors t;
-    if (!marshal(a, n, 7, 1, t)) return 0;
+    if (!marshal(a, n, 7, 1, t, 4)) return 0;
     const OneDevice device(a, 7);
     if (!device.ok) return 0;
     const CacheParams p(a[7]);
@@ -263,7 +269,7 @@ TRI_BIND(cache_read) {
 TRI_BIND(cache_attention) {
   return run([&] {
     Tensors t;
-    if (!marshal(a, n, 9, 1, t)) return 0;
+    if (!marshal(a, n, 9, 1, t, 5)) return 0;
     const OneDevice device(a, 9);
     if (!device.ok) return 0;
     const CacheParams p(a[9]);
@@ -343,7 +349,7 @@ PyObject* run_new(F f) {
 PyObject* cache_append_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return run_new([&]() -> PyObject* {
     Tensors t;
-    if (!marshal(a, n, 7, 2, t)) return nullptr;
+    if (!marshal(a, n, 7, 2, t, 6)) return nullptr;
     const at::Tensor* const k = tensor_of(a[0], "k");
     if (k == nullptr) return nullptr;
     const CacheCall c(a[8], a[2], k->dim() > 0 ? k->size(0) : 0, false, a[7]);
@@ -359,7 +365,7 @@ PyObject* cache_append_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* cache_read_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return run_new([&]() -> PyObject* {
     Tensors t;
-    if (!marshal(a, n, 5, 4, t)) return nullptr;
+    if (!marshal(a, n, 5, 4, t, 4)) return nullptr;
     const at::Tensor* const cache = tensor_of(a[0], "the cache");
     if (cache == nullptr) return nullptr;
     CacheCall c(a[8], a[0], a[5] != Py_None ? PyLong_AsLongLong(a[5]) : 0, true, a[7]);
@@ -396,7 +402,7 @@ PyObject* cache_read_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return run_new([&]() -> PyObject* {
     Tensors t;
-    if (!marshal(a, n, 8, 3, t)) return nullptr;
+    if (!marshal(a, n, 8, 3, t, 5)) return nullptr;
     const at::Tensor* const q = tensor_of(a[0], "q");
     if (q == nullptr) return nullptr;
     const CacheCall c(a[10], a[1], q->dim() > 0 ? q->size(0) : 0, false, a[9]);

@@ -19,7 +19,7 @@ NATIVE_PATH = os.path.join(_HERE, "_native.so")
 
 TRI_F16, TRI_BF16, TRI_F32, TRI_U8, TRI_FP8_E4M3, TRI_I32 = 0, 1, 2, 3, 4, 5
 _DTYPES = {torch.float16: TRI_F16, torch.bfloat16: TRI_BF16, torch.float32: TRI_F32, torch.uint8: TRI_U8,
-           torch.float8_e4m3fn: TRI_FP8_E4M3, torch.int32: TRI_I32}
+           torch.float8_e4m3fn: TRI_FP8_E4M3}
 
 
 class TriTensor(ctypes.Structure):
@@ -130,11 +130,12 @@ def native():
     return _native
 
 
-def as_tri(t):
-    """torch tensor (or None) -> TriTensor (or None).  No copies are made."""
+def as_tri(t, lengths=False):
+    """torch tensor (or None) -> TriTensor (or None).  No copies are made.  `lengths`: int32 is one of its types."""
     if t is None:
         return None
-    if t.dtype not in _DTYPES:
+    dtype = TRI_I32 if lengths and t.dtype == torch.int32 else _DTYPES.get(t.dtype)
+    if dtype is None:
         raise TypeError("unsupported dtype %s" % t.dtype)
     if t.dim() > 4:
         raise ValueError("at most 4 dimensions")
@@ -144,7 +145,7 @@ def as_tri(t):
         s.shape[i] = t.shape[i]
         s.stride[i] = t.stride(i)
     s.ndim = t.dim()
-    s.dtype = _DTYPES[t.dtype]
+    s.dtype = dtype
     return s
 
 
@@ -336,9 +337,13 @@ def _stream_or_none(t):
     return _stream_ptr(t) if t is not None and t.is_cuda else 0
 
 
+def _lens(t):
+    return as_tri(t, lengths=True) if isinstance(t, torch.Tensor) else t
+
+
 def cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, validate_only=False):
     if validate_only:
-        return _call("tri_validate_cache_append", [k, v, k_cache, k_scales, v_cache, v_scales, lens, ctypes.byref(params)], True)
+        return _call("tri_validate_cache_append", [k, v, k_cache, k_scales, v_cache, v_scales, _lens(lens), ctypes.byref(params)], True)
     st = native().cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, _stream_or_none(k))
     if st:
         _check("tri_cache_append", st)
@@ -347,7 +352,7 @@ def cache_append(k, v, k_cache, k_scales, v_cache, v_scales, lens, params, valid
 
 def cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, validate_only=False):
     if validate_only:
-        return _call("tri_validate_cache_read", [k_cache, k_scales, v_cache, v_scales, lens, k, v, ctypes.byref(params)], True)
+        return _call("tri_validate_cache_read", [k_cache, k_scales, v_cache, v_scales, _lens(lens), k, v, ctypes.byref(params)], True)
     st = native().cache_read(k_cache, k_scales, v_cache, v_scales, lens, k, v, params, _stream_or_none(k))
     if st:
         _check("tri_cache_read", st)
@@ -364,7 +369,7 @@ def cache_scratch_bytes(params, four_bit):
 
 def cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, validate_only=False):
     if validate_only:
-        return _call("tri_validate_cache_attention", [q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out,
+        return _call("tri_validate_cache_attention", [q, k_cache, k_scales, v_cache, v_scales, _lens(lens), scratch, lse, out,
                                                       ctypes.byref(params)], True)
     st = native().cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, _stream_or_none(q))
     if st:
