@@ -1,5 +1,7 @@
 """blocks.CachedAttention on the CPU: what it owns, and what it hands to the compiled binding (a stand-in of it here, as
 nothing may be launched)."""
+import copy
+import pickle
 import threading
 
 import pytest
@@ -76,3 +78,20 @@ def test_int32_tensors_are_lengths_alone():
             ext.cache_attention(*args[:i], i32, *args[i + 1:], p, validate_only=True)
         with pytest.raises(TypeError):
             ext.native().cache_attention(*args[:i], i32, *args[i + 1:], p, 0)
+
+
+@pytest.mark.parametrize("make", [blocks.CachedAttention, blocks.CachedAttentionPlan, lambda *a, **kw: blocks.AttentionPlan(D=64)])
+def test_objects_can_be_copied_and_pickled(make):
+    """As parts of an nn.Module are (the earlier plans can); a copy has the same parameters and no buffer of the first."""
+    op = make(6, 2, 64, window=7, sinks=3)
+    own = getattr(op, "attention", op)
+    if hasattr(own, "_p"):
+        own._scratch[0] = torch.zeros(8)
+    for other in (copy.deepcopy(op), copy.copy(op), pickle.loads(pickle.dumps(op))):
+        its = getattr(other, "attention", other)
+        if hasattr(own, "_p"):
+            assert bytes(its._p) == bytes(own._p)
+            assert not its._scratch or its is own
+            with pytest.raises(ValueError):  # (host memory)
+                its.append(torch.zeros(1, 128).half(), torch.zeros(1, 128).half(), *[torch.zeros(1, 2, 4, 64).half()] * 2)
+    assert not hasattr(own, "_p") or own._scratch

@@ -112,8 +112,12 @@ class CachedAttention:
         # (the sizes of a call are read off its tensors)
         self._p = ext.cache_params(0, n_kv_heads, head_dim, 0, 0, n_q_heads=n_q_heads, scale=scale, causal=causal, window=window,
                                    sinks=sinks)
-        self._native = ext.native()
+        ext.native()  # (loaded now, not by a call under capture)
         self._scratch = {}
+
+    def __getstate__(self):
+        """Copies start without scratch (and a module cannot be copied: the binding is looked up by each call)."""
+        return dict(self.__dict__, _scratch={})
 
     @staticmethod
     def make_cache(batch, n_kv_heads, rows, head_dim, device):
@@ -123,7 +127,7 @@ class CachedAttention:
 
     def append(self, K, V, k_cache, v_cache, k_scales=None, v_scales=None, lens=None, kv_len=None):
         """K, V [batch * tokens, KV heads * head_dim] to the last rows of their sequences."""
-        st = self._native.cache_append_rows(K, V, k_cache, k_scales, v_cache, v_scales, lens, kv_len, self._p, ext._stream_or_none(K))
+        st = ext.native().cache_append_rows(K, V, k_cache, k_scales, v_cache, v_scales, lens, kv_len, self._p, ext._stream_or_none(K))
         if st:
             ext._check("tri_cache_append", st)
 
@@ -136,7 +140,7 @@ class CachedAttention:
             dtype = k_cache.dtype
         elif dtype not in (None, torch.float16, torch.bfloat16):
             raise ValueError("rows are read as float16 or bfloat16")
-        r = self._native.cache_read_rows(k_cache, k_scales, v_cache, v_scales, lens, rows, dtype is torch.bfloat16, kv_len,
+        r = ext.native().cache_read_rows(k_cache, k_scales, v_cache, v_scales, lens, rows, dtype is torch.bfloat16, kv_len,
                                          self._p, ext._stream_or_none(k_cache))
         if type(r) is int:
             ext._check("tri_cache_read", r)
@@ -150,14 +154,13 @@ class CachedAttention:
         # without the interpreter lock, and another thread's call on the stream, which may enqueue its own between them, finds none.
         kept = self._scratch.pop(stream, None)
         capturing = kept is not None and torch.cuda.is_current_stream_capturing()
-        r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, None if capturing else kept, out, want_lse,
-                                      kv_len, self._p, stream)
+        call = ext.native().cache_attend
+        r = call(Q, k_cache, k_scales, v_cache, v_scales, lens, None if capturing else kept, out, want_lse, kv_len, self._p, stream)
         if type(r) is int and r > 0:  # bytes of scratch: the first call of its size, or a captured one
             scratch = torch.empty(r, dtype=torch.uint8, device=Q.device)
             if not torch.cuda.is_current_stream_capturing():
                 kept = scratch
-            r = self._native.cache_attend(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, self._p,
-                                          stream)
+            r = call(Q, k_cache, k_scales, v_cache, v_scales, lens, scratch, out, want_lse, kv_len, self._p, stream)
         if kept is not None:
             self._scratch[stream] = kept
         if type(r) is int:
