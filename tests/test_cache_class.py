@@ -1,7 +1,9 @@
 """blocks.CachedAttention on the CPU: what it owns, and what it hands to the compiled binding (a stand-in of it here, as
 nothing may be launched)."""
 import copy
+import ctypes
 import pickle
+import random
 import threading
 
 import pytest
@@ -95,3 +97,22 @@ def test_objects_can_be_copied_and_pickled(make):
             with pytest.raises(ValueError):  # (host memory)
                 its.append(torch.zeros(1, 128).half(), torch.zeros(1, 128).half(), *[torch.zeros(1, 2, 4, 64).half()] * 2)
     assert not hasattr(own, "_p") or own._scratch
+
+
+def test_sizes_beyond_what_a_launch_counts():
+    """Products of batch, tokens and heads up to 2^62: refused from the limit on, and sized below it."""
+    size = ext.lib().tri_cache_scratch_bytes
+    size.restype = ctypes.c_int64
+    rng = random.Random(1)
+    cases = [(1 << 15, 1 << 15, 1, 1 << 30, 128), (1, 1 << 29, 1, (1 << 31) - 1, 64), ((1 << 23) - 1, 255, 1, 1 << 23, 128),
+             (1, (1 << 27) - 257, 1, 1, 128), (1, (1 << 27) - 256, 1, 1, 128), (1, (1 << 28) - 513, 1, 1, 64), (1, (1 << 28) - 512, 1, 1, 64)]
+    for _ in range(5000):
+        cases.append((int(2 ** rng.uniform(0, 24)), int(2 ** rng.uniform(0, 30)), int(2 ** rng.uniform(0, 20)), int(2 ** rng.uniform(0, 11)),
+                      rng.choice((64, 128))))
+    fits = 0
+    for B, S, Hkv, group, D in cases:
+        p = ext.cache_params(B, Hkv, D, S, 1000, n_q_heads=Hkv * group)
+        ok = B * S * Hkv * group * (D // 8) < (1 << 31) - 4096 and B * Hkv < 1 << 24
+        assert (size(ctypes.byref(p), 0) >= 0) == ok, (B, S, Hkv, group, D)
+        fits += ok
+    assert 500 < fits < len(cases) - 500

@@ -353,14 +353,15 @@ int check_cache_params(const tri_cache_params* p, bool attention) {
   if (p == nullptr) return TRI_ERR_NULL;
   if (p->head_dim != 64 && p->head_dim != 128) return TRI_ERR_UNSUPPORTED;
   if (p->batch < 0 || p->seq < 0 || p->kv_len < 0 || p->n_kv_heads <= 0) return TRI_ERR_SHAPE;
-  // (threads and workgroups are counted in 32 bits, with room for the largest tile)
-  if ((int64_t)p->batch * p->seq >= kInt32End || (int64_t)p->batch * p->seq * p->n_kv_heads * (p->head_dim / 8) >= kInt32End - 4096)
-    return TRI_ERR_UNSUPPORTED;
+  // (threads and workgroups are counted in 32 bits, with room for the largest tile: this many rows, each with a thread for
+  // eight channels; tokens and heads are both below 2^31, so that their product does not pass 63 bits)
+  const int64_t tokens = (int64_t)p->batch * p->seq, most = (kInt32End - 4096) / (p->head_dim / 8);
+  if (tokens >= kInt32End || tokens * p->n_kv_heads >= most) return TRI_ERR_UNSUPPORTED;
   if (p->kv_len >= (1 << 30) || p->seq >= (1 << 30)) return TRI_ERR_UNSUPPORTED;
   if (!attention) return TRI_OK;
   if ((int64_t)p->batch * p->n_kv_heads >= (1 << 24)) return TRI_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
   if (p->n_q_heads <= 0 || p->n_q_heads % p->n_kv_heads != 0) return TRI_ERR_SHAPE;
-  if ((int64_t)p->batch * p->seq * p->n_q_heads * (p->head_dim / 8) >= kInt32End - 4096) return TRI_ERR_UNSUPPORTED;
+  if (tokens * p->n_q_heads >= most) return TRI_ERR_UNSUPPORTED;
   if (!(p->scale > 0.f) || !(p->scale < INFINITY)) return TRI_ERR_UNSUPPORTED;
   if (p->window < 0 || p->sinks < 0) return TRI_ERR_SHAPE;
   if (p->window > 0 && !p->causal) return TRI_ERR_UNSUPPORTED;
