@@ -133,7 +133,8 @@ class CachedAttention:
 
     def read(self, k_cache, v_cache, k_scales=None, v_scales=None, dtype=None, rows=None, lens=None, kv_len=None):
         """The last `rows` rows of every sequence (None: `kv_len`) as k, v [batch, KV heads, rows, head_dim]; zeros where a
-        sequence has fewer.  From 4 bits in float16 (None) or bfloat16."""
+        sequence has fewer.  From 4 bits in float16 (None) or bfloat16.  k and v are the halves of one allocation: what keeps one
+        keeps the memory of both (`clone` for one alone, also to save it)."""
         if k_scales is None:
             if dtype is not None and dtype != k_cache.dtype:
                 raise ValueError("rows of a 16-bit cache are read as they are, %s" % k_cache.dtype)

@@ -274,7 +274,7 @@ struct CacheRowsArgs {
   int64_t k_sb, k_sh, k_sr, v_sb, v_sh, v_sr;
   CacheView kc, vc;
   const int32_t* lens;
-  int B, S, Hkv, D, kv_len, rows;  // rows: of the caches
+  int B, S, Hkv, D, kv_len;
 };
 int launch_cache_append(const CacheRowsArgs& a, hipStream_t stream);
 int launch_cache_read(const CacheRowsArgs& a, hipStream_t stream);
