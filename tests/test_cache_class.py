@@ -1,10 +1,12 @@
 """blocks.CachedAttention on the CPU: what it owns, and what it hands to the compiled binding (a stand-in of it here, as
 nothing may be launched)."""
 import copy
+import contextlib
 import ctypes
 import pickle
 import random
 import threading
+import types
 
 import pytest
 import torch
@@ -116,3 +118,51 @@ def test_sizes_beyond_what_a_launch_counts():
         assert (size(ctypes.byref(p), 0) >= 0) == ok, (B, S, Hkv, group, D)
         fits += ok
     assert 500 < fits < len(cases) - 500
+
+
+def _plan_of_records(monkeypatch):
+    """A plan whose steps note the current device (`now`) and launch nothing."""
+    now, steps = [0], []
+    note = lambda *a, **kw: steps.append(now[0])
+    for name in ("matmul", "rmsnorm"):
+        monkeypatch.setattr(ext, name, note)
+    plan = blocks.CachedAttentionPlan(4, 2, 64, prenorm=True, qknorm=True)
+    monkeypatch.setattr(plan.attention, "append", note, raising=False)
+    monkeypatch.setattr(plan.attention, "attend", note, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+
+    @contextlib.contextmanager
+    def device(d):
+        before, now[0] = now[0], torch.device(d).index
+        yield
+        now[0] = before
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    return plan, now, steps
+
+
+def _on(device, *shape):
+    """What the plan's own code looks at of a tensor there."""
+    t = torch.zeros(*shape, dtype=torch.float16)
+    return types.SimpleNamespace(shape=t.shape, device=torch.device(device), is_cuda=device != "cpu", new_empty=t.new_empty)
+
+
+def test_plan_refuses_tensors_of_other_devices_before_anything_runs(monkeypatch):
+    plan, now, steps = _plan_of_records(monkeypatch)
+    at = {"X": (8, 128), "WQ": (128, 256), "WK": (128, 128), "WV": (128, 128), "norm_w": (128,)}
+    for device in ("cpu", "cuda:1"):
+        for name in at:
+            t = {k: _on(device if k == name else "cuda:0", *shape) for k, shape in at.items()}
+            with pytest.raises(ValueError):
+                plan.run(t["X"], t["WQ"], t["WK"], t["WV"], None, None, None, norm_w=t["norm_w"])
+    assert not steps
+
+
+def test_plan_runs_on_its_tensors_gpu(monkeypatch):
+    plan, now, steps = _plan_of_records(monkeypatch)
+    now[0] = 0
+    for index in (0, 1):
+        on = lambda *shape: _on("cuda:%d" % index, *shape)
+        del steps[:]
+        plan.run(on(8, 128), on(128, 256), on(128, 128), on(128, 128), None, None, None, norm_w=on(128))
+        assert steps == [index] * 8 and now[0] == 0  # norm, three products, two norms, append, attention

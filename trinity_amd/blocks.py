@@ -195,6 +195,12 @@ class CachedAttentionPlan:
             want_lse=False):
         if norm_w is not None and not self.prenorm:
             raise ValueError("a norm weight without PreNorm")
+        # (the products and norms launch on the current GPU, and would read another's memory, or the host's, as if it were its own)
+        if not X.is_cuda or any(t is not None and t.device != X.device for t in (WQ, WK, WV, norm_w)):
+            raise ValueError("the tensors of a call have to be on one GPU")
+        if X.device.index != torch.cuda.current_device():
+            with torch.cuda.device(X.device):
+                return self.run(X, WQ, WK, WV, O2, k_cache, v_cache, k_scales, v_scales, lens, kv_len, norm_w, want_lse)
         if self.prenorm:
             xn = X.new_empty(X.shape)
             ext.rmsnorm(X, norm_w, xn, self.eps)
