@@ -34,11 +34,6 @@ __device__ __forceinline__ int row_token(const CacheAttnArgs& a, int row) { retu
 // offset of a key's row: row strides are less than 2^31 bytes, so that this is one product of 32 bits and not three
 __device__ __forceinline__ uint64_t row_at(int key, int64_t stride) { return (uint64_t)(uint32_t)key * (uint32_t)stride; }
 
-// keys of a sequence
-__device__ __forceinline__ int seq_keys(const CacheAttnArgs& a, int b) {
-  return a.lens == nullptr ? a.kv_len : min(max(a.lens[b], 0), a.kv_len);
-}
-
 // what a row block of a sequence sees
 struct KeyList {
   int len;        // keys of the sequence
@@ -48,7 +43,7 @@ struct KeyList {
 
 __device__ __forceinline__ KeyList key_list(const CacheAttnArgs& a, int b, int tok0, int tok1) {
   KeyList k;
-  k.len = seq_keys(a, b);
+  k.len = a.lens == nullptr ? a.kv_len : min(max(a.lens[b], 0), a.kv_len);
   const int first = max(k.len - a.S + tok0, 0), last = k.len - a.S + tok1;  // positions of the block's tokens
   const int end = last < 0 ? 0 : (a.causal ? last + 1 : k.len);
   const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
@@ -58,26 +53,27 @@ __device__ __forceinline__ KeyList key_list(const CacheAttnArgs& a, int b, int t
   return k;
 }
 
-// result of a row at position pos: four channels d4 of the finished sum, divided by the softmax's, and its log-sum-exp.  Padding,
-// the rows without a visible key, gets zeros and -inf, chosen and not multiplied: its sum is zero times the rows of V that others
-// of the block see, NaN where one of these holds no number.
+// result of a row: four channels d4 of the finished sum, divided by the softmax's, and its log-sum-exp.  Padding, the rows without
+// a visible key, gets zeros and -inf, chosen and not multiplied: its sum is zero times the rows of V that others of the block see,
+// NaN where one of these holds no number.  (A row whose scores are all -inf has a sum of zero, too: it is NaN.)
 template <int D>
-__device__ __forceinline__ void store_row(const CacheAttnArgs& a, int b, int hk, int row, int pos, int d4, float m, float l, float4v acc) {
+__device__ __forceinline__ void store_row(const CacheAttnArgs& a, int b, int hk, int row, bool padding, int d4, float m, float l, float4v acc) {
   const int tok = row_token(a, row), head = hk * a.group + row - tok * a.group;
   const float inv = 1.0f / l;
   half4v hv;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) hv[e] = pos < 0 ? (half_t)0.f : (half_t)(acc[e] * inv);
-  *reinterpret_cast<half4v*>(a.out + ((int64_t)b * a.S + tok) * a.ldo + (int64_t)head * D + d4 * 4) = hv;
+  for (int e = 0; e < 4; ++e) hv[e] = (half_t)(acc[e] * inv);
+  *reinterpret_cast<half4v*>(a.out + ((int64_t)b * a.S + tok) * a.ldo + (int64_t)head * D + d4 * 4) = padding ? half4v{} : hv;
   if (a.lse != nullptr && d4 == 0)
-    a.lse[((int64_t)b * a.Hq + head) * a.S + tok] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    a.lse[((int64_t)b * a.Hq + head) * a.S + tok] = padding || l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
 }
 
-// ... or, of several runs, its partial result: unnormalised O [b][hk][row][run][D], then (max, sum) [b][hk][row][run][2]
+// ... or, of several runs, its partial result: unnormalised O [b][hk][row][run][D], then (max, sum) [b][hk][row][run][2].  Padding
+// has the sum -1, which the merge knows it by.
 template <int D>
-__device__ __forceinline__ void finish_row(const CacheAttnArgs& a, int b, int hk, int row, int pos, int run, int d4, float m, float l, float4v acc) {
+__device__ __forceinline__ void finish_row(const CacheAttnArgs& a, int b, int hk, int row, bool padding, int run, int d4, float m, float l, float4v acc) {
   if (a.runs == 1) {
-    store_row<D>(a, b, hk, row, pos, d4, m, l, acc);
+    store_row<D>(a, b, hk, row, padding, d4, m, l, acc);
     return;
   }
   const int64_t rows = a.rows, at = (((int64_t)b * a.Hkv + hk) * rows + row) * a.runs + run;
@@ -85,7 +81,7 @@ __device__ __forceinline__ void finish_row(const CacheAttnArgs& a, int b, int hk
   if (d4 == 0) {
     float* ps = a.ws + (int64_t)a.B * a.Hkv * rows * a.runs * D + at * 2;
     ps[0] = m;
-    ps[1] = l;
+    ps[1] = padding ? -1.f : l;
   }
 }
 
@@ -183,14 +179,21 @@ __device__ __forceinline__ void tile_finish(const CacheAttnArgs& a, half_t* lds_
     static_assert(32 * LDO * 2 <= REG * 64 * 4, "two ways: in the place of the state that only this wave has read");
     half_t* const stage = KW == 2 ? reinterpret_cast<half_t*>(mg - lane) : lds_all + wave * 32 * LDO;
     if (KW == 1) __syncthreads();  // (every wave is done with the tiles)
-    const float inv = 1.0f / l;
+    float inv = 1.0f / l;
+    if (__builtin_amdgcn_ballot_w64(pos < 0) != 0) {  // wave-uniform; padding (see store_row), which most calls have none of
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = pos < 0 ? 0.f : o[dt][e];
+      inv = pos < 0 ? 0.f : inv;
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int rq = 0; rq < 4; ++rq) {
         half4v hv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) hv[e] = pos < 0 ? (half_t)0.f : (half_t)(o[dt][rq * 4 + e] * inv);  // (as in store_row)
+        for (int e = 0; e < 4; ++e) hv[e] = (half_t)(o[dt][rq * 4 + e] * inv);
         *reinterpret_cast<half4v*>(stage + l32 * LDO + dt * 32 + rq * 8 + g * 4) = hv;
       }
     if (a.lse != nullptr && g == 0 && row < rows)
@@ -212,7 +215,7 @@ __device__ __forceinline__ void tile_finish(const CacheAttnArgs& a, half_t* lds_
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int rq = 0; rq < 4; ++rq)
-      finish_row<D>(a, b, hk, row, pos, run, dt * 8 + rq * 2 + g, m, l,
+      finish_row<D>(a, b, hk, row, pos < 0, run, dt * 8 + rq * 2 + g, m, l,
                     float4v{o[dt][rq * 4], o[dt][rq * 4 + 1], o[dt][rq * 4 + 2], o[dt][rq * 4 + 3]});
 }
 
@@ -1084,7 +1087,7 @@ __device__ __forceinline__ void cache_attn_few_body(const CacheAttnArgs& a, half
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[e], sc, acc[e]);
     }
-    finish_row<D>(a, b, hk, row, kl.len - a.S + row_token(a, row), run, d4, M, L, acc);
+    finish_row<D>(a, b, hk, row, kl.len - a.S + row_token(a, row) < 0, run, d4, M, L, acc);
   }
 }
 
@@ -1108,8 +1111,6 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
   const int64_t idx = (int64_t)blockIdx.x * LANES + lane;
   const int64_t at = min(idx / LPR, total - 1);
   const int d4 = (int)(idx % LPR);
-  const int bh = (int)(at / rows), row = (int)(at - (int64_t)bh * rows), b = bh / a.Hkv;
-  const int pos = seq_keys(a, b) - a.S + row_token(a, row);
   const float* po = a.ws + at * a.runs * D + d4 * 4;
   const float* ps = a.ws + total * a.runs * D + at * a.runs * 2;
   float m = -INFINITY, l = 0.f;
@@ -1127,7 +1128,7 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     float mn = m;
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) mn = fmaxf(mn, mi[j]);
-    // (a run whose maximum is -inf sees no key, and its sum is 0, or it sees NaN alone, and its sum is one)
+    // (a run whose maximum is -inf sees no key, and its sum is 0, or it sees NaN alone, and its sum is one; that of padding is -1)
     if (mn == -INFINITY) {
 #pragma unroll
       for (int j = 0; j < UNROLL; ++j) l += li[j];
@@ -1165,14 +1166,14 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(CacheAttnArgs a) {
     for (int w = 0; w < WAYS; ++w) {
       const float mw = sm[w * LANES + lane];
       const float sc = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
-      l = fmaf(sl[w * LANES + lane], sc, l);
+      l = mw == -INFINITY ? l + sl[w * LANES + lane] : fmaf(sl[w * LANES + lane], sc, l);
       const float4v v = so[w * LANES + lane];
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[e], sc, acc[e]);
     }
   }
   if (idx / LPR >= total) return;
-  store_row<D>(a, b, bh - b * a.Hkv, row, pos, d4, m, l, acc);
+  store_row<D>(a, (int)(at / rows / a.Hkv), (int)(at / rows % a.Hkv), (int)(at % rows), l < 0.f, d4, m, l, acc);
 }
 
 // ---- which kernel, and in how many runs
