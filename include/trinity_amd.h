@@ -297,7 +297,8 @@ int tri_validate_roco(const tri_tensor* x, const tri_tensor* norm_w, const tri_t
  *                  65504 read as infinities).
  *   lens           TRI_I32 [batch], or NULL: every sequence has kv_len keys.
  * The rows a call reads are those of keys that some token of it sees; no others need hold numbers.  Within a call a NaN or
- * infinity among the values of a key reaches the tokens that see it and may reach others of the same call. */
+ * infinity among the values of a key reaches the tokens that see it and may reach others of the same call, but no
+ * padding. */
 typedef struct tri_cache_params {
   int32_t batch;
   int32_t n_q_heads;  /* (tri_cache_attention only) */
@@ -335,9 +336,9 @@ int tri_validate_cache_read(const tri_tensor* k_cache, const tri_tensor* k_scale
 /* out = softmax(scale * q.K^T over the keys that each token sees).V, from caches that hold the call's tokens already.
  *   q, out [batch * seq, n_q_heads * D]; lse fp32 [batch, n_q_heads, seq] contiguous or NULL: the natural log-sum-exp.
  * A row without a visible key (padding) gets zeros, and -inf as its lse, whatever the values that other rows see.
- * scratch: 1-D TRI_U8, 256-byte aligned, or NULL; with tri_cache_scratch_bytes the call runs its fastest plan, with less
- * (or none) it cuts the key axis into fewer parts - same results to rounding.  The size does not depend on the lengths
- * below kv_len. */
+ * scratch: 1-D TRI_U8, 256-byte aligned, or NULL, and this call's own until it has run (two launches); with
+ * tri_cache_scratch_bytes the call runs its fastest plan, with less (or none) it cuts the key axis into fewer parts - same
+ * results to rounding.  The size does not depend on the lengths below kv_len. */
 int64_t tri_cache_scratch_bytes(const tri_cache_params* p, int32_t four_bit);
 int tri_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tri_tensor* k_scales /* nullable */,
                         const tri_tensor* v_cache, const tri_tensor* v_scales /* nullable */,

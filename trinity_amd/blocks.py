@@ -6,6 +6,8 @@ beyond the caller's tensors, and calls the C ABI on torch's current stream.
 Scratch is allocated on the first call only (the reference's drivers always
 run warm-up calls before capturing a graph, convert_eval_rms.py:253-263), so
 `forward` allocates nothing afterwards and is safe under graph capture.
+Such a plan serves one call at a time (CachedAttention and
+CachedAttentionPlan may be shared by threads and streams).
 
 Reference semantics (baseline/ref_rms.py:28-403) are the defaults: no softmax
 scale, no causal mask, as many KV heads as query heads, RMSNorm without eps
