@@ -166,3 +166,14 @@ def test_plan_runs_on_its_tensors_gpu(monkeypatch):
         del steps[:]
         plan.run(on(8, 128), on(128, 256), on(128, 128), on(128, 128), None, None, None, norm_w=on(128))
         assert steps == [index] * 8 and now[0] == 0  # norm, three products, two norms, append, attention
+
+
+def test_host_memory_is_refused_before_scratch_is_asked_for():
+    """A call that cuts its keys into parts, and one that does not, raise the same."""
+    op = blocks.CachedAttention(4, 2, 64)
+    for rows in (40, 4000):
+        q, c = torch.zeros(1, 256).half(), torch.zeros(1, 2, rows, 64).half()
+        assert (ext.cache_scratch_bytes(ext.cache_params(1, 2, 64, 1, rows, n_q_heads=4), False) > 0) == (rows == 4000)
+        with pytest.raises(ValueError):
+            op.attend(q, c, c)
+        assert not op._scratch

@@ -411,12 +411,12 @@ PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!c.ok || PyErr_Occurred() != nullptr) return nullptr;
     const int64_t need = tri_cache_scratch_bytes(&c.p, t.p[2] != nullptr);
     if (need < 0) return PyLong_FromLongLong(need);
-    if (need > 0 && (t.p[6] == nullptr || t.p[6]->shape[0] < need || THPVariable_Unpack(a[6]).device() != q->device()))
-      return PyLong_FromLongLong(need);
     PyObject* with[8];
-    for (int i = 0; i < 8; ++i) with[i] = i == 6 && need == 0 ? Py_None : a[i];  // (a scratch that the call does without may be anywhere)
+    for (int i = 0; i < 8; ++i) with[i] = i == 6 ? Py_None : a[i];  // (the scratch may be anywhere: another is asked for then)
     const OneDevice device(with, 8);
     if (!device.ok) return nullptr;
+    if (need > 0 && (t.p[6] == nullptr || t.p[6]->shape[0] < need || THPVariable_Unpack(a[6]).device() != q->device()))
+      return PyLong_FromLongLong(need);
     at::Tensor made, lse;
     tri_tensor o, l;
     tri_tensor *out = t.p[7], *lp = nullptr;
