@@ -53,7 +53,7 @@ extern "C" {
  * signatures, a different noise stream for a given seed.
  * 7: tri_diag_issue_probe added; nothing else changed.
  * 8: tri_diag_power_probe added; nothing else changed.
- * (The tri_cache_* entry points came later: nothing that was there changed for them, and a caller finds them by their
+ * (The tri_cache_*, tri_fp4_*, tri_route and tri_experts_* entry points came later: nothing that was there changed for them, and a caller finds them by their
  * symbols.) */
 #define TRI_ABI_VERSION 8
 
@@ -63,7 +63,7 @@ typedef enum tri_dtype {
   TRI_F32 = 2,
   TRI_U8 = 3,
   TRI_FP8_E4M3 = 4, /* OCP e4m3 (no infinities, +-448 largest): KV caches only */
-  TRI_I32 = 5       /* lengths of sequences (tri_cache_*) */
+  TRI_I32 = 5       /* lengths of sequences (tri_cache_*), experts of tokens */
 } tri_dtype;
 
 typedef enum tri_status {
@@ -348,6 +348,74 @@ int tri_validate_cache_attention(const tri_tensor* q, const tri_tensor* k_cache,
                                  const tri_tensor* v_cache, const tri_tensor* v_scales, const tri_tensor* lens,
                                  const tri_tensor* scratch, const tri_tensor* lse, const tri_tensor* out,
                                  const tri_cache_params* p);
+
+/* ------------------------------------------------------------------ 4-bit weights, routed experts
+ * Products over weights in 4 bits, and the SwiGLU FFN of experts that each token chooses for itself (over 16-bit or 4-bit
+ * weights), with the routing that chooses them.  No counterpart in the reference, whose FFNs are dense and in fp16
+ * (baseline/ffn_ref.py:12-52).
+ *
+ * 4-bit matrices are two byte tensors, in the format of the 4-bit caches above with blocks along rows: codes TRI_U8
+ * [rows, K / 2] (two codes a byte, the even column in the low half; rows 16-byte aligned) and scales TRI_U8 [rows, K / 32]
+ * (any alignment and row stride).  Weights of a product are [N, K], a row for each output column - torch.nn.Linear's layout;
+ * of experts [E, N, K], their strides free.  K is a multiple of 32 (at most 2^22), N of 8.  A matrix (of one expert) and the rows that experts
+ * read each span less than 4 GB, rows are less than 16 MB apart.
+ * The element type of a product has to hold its weights' values (fp16: from 2^-24 to 65504; beyond, they count as
+ * zeros and infinities); a block whose scale is 255 is NaN.  Sums are in fp32, results are rounded once. */
+
+/* codes, scales of x [M, K] (fp16 or bf16), as tri_cache_append has them: e is the least exponent >= -110 with max |x| < 7 * 2^e
+ * over the block, x / 2^e goes to the nearest magnitude, ties to the even code; a block that holds an infinity or NaN
+ * gets the byte 255.  And back: x = the values that codes and scales stand for, exactly, where x's type holds them. */
+int tri_fp4_quantize(const tri_tensor* x, tri_tensor* codes, tri_tensor* scales, void* hip_stream);
+int tri_validate_fp4_quantize(const tri_tensor* x, const tri_tensor* codes, const tri_tensor* scales);
+int tri_fp4_dequantize(const tri_tensor* codes, const tri_tensor* scales, tri_tensor* x, void* hip_stream);
+int tri_validate_fp4_dequantize(const tri_tensor* codes, const tri_tensor* scales, const tri_tensor* x);
+
+/* out [M, N] = x . w^T: w, w_scales a 4-bit matrix [N, K]; x [M, K] of out's type, or (x_scales given) a 4-bit matrix, too:
+ * the products are then exact and their sum runs on the 4-bit matrix instructions, whatever out's type.  With a workspace of
+ * tri_fp4_workspace_bytes (1-D TRI_U8, 16-byte aligned, this call's own until it has run) the call runs its fastest plan, with
+ * less (or none) it does not cut K into parts - same results to rounding. */
+int64_t tri_fp4_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t four_bit_x);
+int tri_fp4_matmul(const tri_tensor* x, const tri_tensor* x_scales /* nullable */, const tri_tensor* w, const tri_tensor* w_scales,
+                   tri_tensor* workspace /* nullable */, tri_tensor* out, void* hip_stream);
+int tri_validate_fp4_matmul(const tri_tensor* x, const tri_tensor* x_scales, const tri_tensor* w, const tri_tensor* w_scales,
+                            const tri_tensor* workspace, const tri_tensor* out);
+
+/* Experts of every token and their weights, from a router's logits [T, E] (fp16, bf16 or fp32; E at most 512).
+ * s = softmax(logits), or their sigmoid; c = s + bias (fp32 [E], or NULL: 0).  The top_k experts of the largest c in descending
+ * order, ties to the lowest index; with groups > 1 (dividing E, at most 64) out of the top_groups best groups of E / groups
+ * neighbours, a group counting the sum of its group_top (1 or 2) largest c.  weights = s of the chosen (without the bias), with
+ * renormalize over their sum, times scale.  Computed in 64 bits.  A logit of -inf has s = 0; where no logit is above that, all
+ * weights are 0; a NaN makes weights NaN, and ids still top_k different experts.
+ *   ids TRI_I32 [T, top_k], weights TRI_F32 [T, top_k], contiguous. */
+typedef struct tri_route_params {
+  int32_t top_k; /* 1 to 64, and at most the experts of the groups that stay */
+  int32_t sigmoid;
+  int32_t groups;     /* 1: all experts are in question (top_groups, group_top: 1) */
+  int32_t top_groups;
+  int32_t group_top;
+  int32_t renormalize;
+  float scale; /* finite */
+} tri_route_params;
+int tri_route(const tri_tensor* logits, const tri_tensor* bias /* nullable */, tri_tensor* ids, tri_tensor* weights,
+              const tri_route_params* p, void* hip_stream);
+int tri_validate_route(const tri_tensor* logits, const tri_tensor* bias, const tri_tensor* ids, const tri_tensor* weights,
+                       const tri_route_params* p);
+
+/* out[t] = sum over i of weights[t, i] * (silu(x[t] . gate_e^T) * (x[t] . up_e^T)) . down_e^T, e = ids[t, i].
+ *   x, out [T, N]; ids, weights [T, top_k] as tri_route leaves them (an expert may occur twice; ids outside [0, E) count nothing);
+ *   gate, up [E, F, N], down [E, N, F]: of x's type, or 4-bit (codes and scales of all three).  N and F multiples of 32, E and
+ *   top_k at most 512 and 64.  16-bit weights: rows 16-byte aligned.
+ * The hidden rows are rounded to x's type, the experts' outputs are summed in fp32, in the order of the choices.  workspace: 1-D TRI_U8, 256-byte
+ * aligned, tri_experts_workspace_bytes or more, this call's own until it has run. */
+int64_t tri_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts, int64_t n, int64_t f);
+int tri_experts_ffn(const tri_tensor* x, const tri_tensor* ids, const tri_tensor* weights, const tri_tensor* gate,
+                    const tri_tensor* gate_scales /* nullable */, const tri_tensor* up, const tri_tensor* up_scales /* nullable */,
+                    const tri_tensor* down, const tri_tensor* down_scales /* nullable */, tri_tensor* workspace, tri_tensor* out,
+                    void* hip_stream);
+int tri_validate_experts_ffn(const tri_tensor* x, const tri_tensor* ids, const tri_tensor* weights, const tri_tensor* gate,
+                             const tri_tensor* gate_scales, const tri_tensor* up, const tri_tensor* up_scales,
+                             const tri_tensor* down, const tri_tensor* down_scales, const tri_tensor* workspace,
+                             const tri_tensor* out);
 
 /* Issue probe (measurement only; no counterpart in the reference).  Launches `workgroups` workgroups of
  * 4 * waves_per_simd waves, one workgroup per CU, every wave looping `iters` times (a multiple of 8) over a group

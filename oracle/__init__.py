@@ -24,7 +24,7 @@ path, so the pins are mathematical):
                       prefix (causal and not), the zero-logit closed form
                       softmax(g / tau).sum(queries) for tensor and seeded noise,
                       tau / noise sensitivity, sum_k score = S
-* cache.*           - fp64, see there (no counterpart in the reference)
+* cache.*, experts.* - fp64, see there (no counterpart in the reference)
 * philox4x32        - Random123's published known-answer vectors for seven rounds (what the kernels use) and ten
 * gumbel_noise      - float stage: parity unpinned by any external vector (it is
                       this build's own definition: sixteen bits per key,
@@ -44,5 +44,5 @@ from .blocks import (  # noqa: F401
     qkv_attention,
     attention_stage,
 )
-from . import cache  # noqa: F401
+from . import cache, experts  # noqa: F401
 from .philox import philox4x32, philox4x32_10, gumbel_noise, uniform_from_bits  # noqa: F401

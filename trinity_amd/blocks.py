@@ -6,8 +6,8 @@ beyond the caller's tensors, and calls the C ABI on torch's current stream.
 Scratch is allocated on the first call only (the reference's drivers always
 run warm-up calls before capturing a graph, convert_eval_rms.py:253-263), so
 `forward` allocates nothing afterwards and is safe under graph capture.
-Such a plan serves one call at a time (CachedAttention and
-CachedAttentionPlan may be shared by threads and streams).
+Such a plan serves one call at a time (CachedAttention, CachedAttentionPlan and
+what stands behind them below may be shared by threads and streams).
 
 Reference semantics (baseline/ref_rms.py:28-403) are the defaults: no softmax
 scale, no causal mask, as many KV heads as query heads, RMSNorm without eps
@@ -282,3 +282,112 @@ class FfnPlan:
             ext.ffn_swiglu(X, W1, W_up, W2, self._hidden, out, workspace=ws)
         else:
             ext.ffn_gelu(X, W1, W2, self._hidden, out, workspace=ws)
+
+
+class Fp4Matmul:
+    """Products over weights in 4 bits: y = x . w^T, w as `quantize` makes it of an [N, K] matrix (torch.nn.Linear's layout) -
+    codes [N, K / 2] and scales [N, K / 32]; with `quantize_x`, x goes to 4 bits as well, and the product runs on the 4-bit matrix
+    instructions.  Every call's buffers come from the allocator: an object may be shared by threads, streams and graphs."""
+
+    def __init__(self, quantize_x=False):
+        self.quantize_x = bool(quantize_x)
+        ext.native()  # (loaded now, not by a call under capture)
+
+    @staticmethod
+    def quantize(X):
+        """Codes and scales of the rows of X [M, K], K a multiple of 32."""
+        r = ext.native().fp4_quantize_new(X, ext._stream_or_none(X))
+        if type(r) is int:
+            ext._check("tri_fp4_quantize", r)
+        return r
+
+    @staticmethod
+    def dequantize(codes, scales, dtype=torch.float16):
+        """The values that codes and scales stand for, in float16 or bfloat16."""
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("values are float16 or bfloat16")
+        r = ext.native().fp4_dequantize_new(codes, scales, dtype is torch.bfloat16, ext._stream_or_none(codes))
+        if type(r) is int:
+            ext._check("tri_fp4_dequantize", r)
+        return r
+
+    def run(self, X, W, w_scales, x_scales=None, out=None, dtype=torch.float16):
+        """X [M, K], or its codes with `x_scales` (the result is then of type `dtype`, or `out`'s)."""
+        if x_scales is not None and dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("results are float16 or bfloat16")
+        r = ext.native().fp4_matmul_new(X, x_scales, W, w_scales, out, self.quantize_x and x_scales is None,
+                                        dtype is torch.bfloat16, ext._stream_or_none(X))
+        if type(r) is int:
+            ext._check("tri_fp4_matmul", r)
+        return r
+
+
+class Router:
+    """Experts of every token and their weights from a router's logits: scores are the softmax or sigmoid of the logits, experts
+    are chosen by score + bias, `top_k` of them in descending order (ties: the lowest index), out of the `top_groups` best of
+    `groups` groups of neighbours - a group counts its `group_top` (1 or 2) largest - and weighted with their scores, over the
+    sum of the chosen if `renormalize`, times `scale`."""
+
+    def __init__(self, top_k, scores="softmax", groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0):
+        if scores not in ("softmax", "sigmoid"):
+            raise ValueError("scores must be softmax or sigmoid")
+        self.top_k = top_k
+        self._p = ext.route_params(top_k, sigmoid=scores == "sigmoid", groups=groups, top_groups=top_groups, group_top=group_top,
+                                   renormalize=renormalize, scale=scale)
+        ext.native()
+
+    def route(self, logits, bias=None):
+        """logits [T, E], bias float32 [E]: ids int32 [T, top_k] and weights float32 [T, top_k]."""
+        r = ext.native().route_new(logits, bias, self._p, ext._stream_or_none(logits))
+        if type(r) is int:
+            ext._check("tri_route", r)
+        return r
+
+
+class ExpertsFfn:
+    """The SwiGLU FFN of the experts that each token chose: out[t] = sum over i of weights[t, i] * FFN_ids[t, i](x[t]).  Weights are
+    [E, F, N] (gate, up) and [E, N, F] (down), torch.nn.Linear's layout for each expert, of x's type or in 4 bits (codes, and
+    scales of all three, as `Fp4Matmul.quantize` makes them of an expert's matrix).  ids outside [0, E) count nothing.  Every call's
+    buffers come from the allocator: an object may be shared by threads, streams and graphs."""
+
+    def __init__(self):
+        ext.native()
+
+    def run(self, X, ids, weights, W_gate, W_up, W_down, gate_scales=None, up_scales=None, down_scales=None, out=None):
+        r = ext.native().experts_ffn_new(X, ids, weights, W_gate, gate_scales, W_up, up_scales, W_down, down_scales, out,
+                                         ext._stream_or_none(X))
+        if type(r) is int:
+            ext._check("tri_experts_ffn", r)
+        return r
+
+
+class RoutedFfnPlan:
+    """The FFN half of a layer with experts: [RMSNorm,] the router's product, routing, and the experts' FFN: X [T, N], W_router
+    [N, E], and what `Router` and `ExpertsFfn` take.  A call's buffers come from the allocator."""
+
+    def __init__(self, top_k, scores="softmax", groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0, prenorm=False,
+                 eps=0.0):
+        self.router = Router(top_k, scores=scores, groups=groups, top_groups=top_groups, group_top=group_top,
+                             renormalize=renormalize, scale=scale)
+        self.experts = ExpertsFfn()
+        self.prenorm, self.eps = prenorm, eps
+
+    def run(self, X, W_router, W_gate, W_up, W_down, gate_scales=None, up_scales=None, down_scales=None, bias=None, norm_w=None,
+            out=None):
+        if norm_w is not None and not self.prenorm:
+            raise ValueError("a norm weight without PreNorm")
+        # (the product and the norm launch on the current GPU, and would read another's memory, or the host's, as if it were its own)
+        if not X.is_cuda or any(t is not None and t.device != X.device for t in (W_router, norm_w)):
+            raise ValueError("the tensors of a call have to be on one GPU")
+        if X.device.index != torch.cuda.current_device():
+            with torch.cuda.device(X.device):
+                return self.run(X, W_router, W_gate, W_up, W_down, gate_scales, up_scales, down_scales, bias, norm_w, out)
+        if self.prenorm:
+            xn = X.new_empty(X.shape)
+            ext.rmsnorm(X, norm_w, xn, self.eps)
+            X = xn
+        logits = X.new_empty(X.shape[0], W_router.shape[1])
+        need = ext.gemm_workspace_bytes(X.shape[0], X.shape[1], W_router.shape[1])
+        ext.matmul(X, W_router, None, logits, X.new_empty(need, dtype=torch.uint8) if need else None)
+        ids, weights = self.router.route(logits, bias)
+        return self.experts.run(X, ids, weights, W_gate, W_up, W_down, gate_scales, up_scales, down_scales, out=out)

@@ -431,6 +431,88 @@ int check_caches(const tri_tensor* kc, const tri_tensor* kx, const tri_tensor* v
 
 inline bool cache_is_empty(const tri_cache_params* p) { return p->batch == 0 || p->seq == 0; }
 
+// ---- 4-bit matrices, experts
+constexpr int64_t kSpan = ((int64_t)1 << 32) - 256, kMaxRowStride = (int64_t)1 << 24, kMaxDeep = (int64_t)1 << 22;
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;  // (a launch of 256-thread workgroups has less than 2^32 threads)
+
+// contiguous rows [(E,) rows, n] of `size`-byte elements that start at multiples of `align` bytes (experts may share memory, rows
+// of a matrix do not)
+int check_rows(const tri_tensor* t, int64_t E, int64_t rows, int64_t n, int dtype, int size, int align) {
+  if (t == nullptr) return TRI_ERR_NULL;
+  if (t->dtype != dtype) return TRI_ERR_DTYPE;
+  const int lead = E >= 0 ? 1 : 0;
+  if (t->ndim != 2 + lead || (lead && t->shape[0] != E) || t->shape[lead] != rows || t->shape[lead + 1] != n) return TRI_ERR_SHAPE;
+  if (rows == 0) return TRI_OK;  // no rows: no storage
+  if (t->ptr == nullptr) return TRI_ERR_NULL;
+  const int64_t* st = t->stride + lead;
+  if (n > 1 && st[1] != 1) return TRI_ERR_STRIDE;
+  if (rows > 1 && (st[0] < n || st[0] * size % align != 0)) return TRI_ERR_STRIDE;
+  if (lead && E > 1 && (t->stride[0] < 0 || t->stride[0] * size % align != 0)) return TRI_ERR_STRIDE;
+  if (((uintptr_t)t->ptr & (uintptr_t)(align - 1)) != 0) return TRI_ERR_ALIGN;
+  if (rows > 1 && st[0] * size >= kMaxRowStride) return TRI_ERR_UNSUPPORTED;
+  return TRI_OK;
+}
+inline int64_t row_bytes(const tri_tensor* t, int size) { return t->shape[t->ndim - 2] > 1 ? t->stride[t->ndim - 2] * size : t->shape[t->ndim - 1] * size; }
+inline bool spans_too_much(const tri_tensor* t, int size) { return t->shape[t->ndim - 2] * row_bytes(t, size) >= kSpan; }
+
+int check_fp4(const tri_tensor* codes, const tri_tensor* scales, int64_t E, int64_t rows, int64_t K) {
+  if (codes == nullptr || scales == nullptr) return TRI_ERR_NULL;
+  TRI_TRY(check_rows(codes, E, rows, K / 2, TRI_U8, 1, 16));
+  return check_rows(scales, E, rows, K / 32, TRI_U8, 1, 1);
+}
+// depth of a product: what 4-bit blocks and the kernels' steps are multiples of
+int check_deep(int64_t K) { return K < 32 || K % 32 != 0 || K > kMaxDeep ? TRI_ERR_UNSUPPORTED : TRI_OK; }
+
+int check_fp4_rows(const tri_tensor* x, const tri_tensor* codes, const tri_tensor* scales) {
+  if (x == nullptr || codes == nullptr || scales == nullptr) return TRI_ERR_NULL;
+  if (x->ndim != 2) return TRI_ERR_SHAPE;
+  const int64_t M = x->shape[0], K = x->shape[1];
+  TRI_TRY(check_mat(x, -1, -1, elem_dtype(x)));
+  TRI_TRY(check_deep(K));
+  if (M >= kInt32End) return TRI_ERR_UNSUPPORTED;
+  return check_fp4(codes, scales, -1, M, K);
+}
+
+// contiguous [T, k] of 32-bit values
+int check_choices(const tri_tensor* ids, const tri_tensor* weights, int64_t T, int64_t k) {
+  for (const tri_tensor* t : {ids, weights}) {
+    if (t->ndim != 2 || t->shape[0] != T || t->shape[1] != k) return TRI_ERR_SHAPE;
+    if (T == 0) continue;
+    if (t->ptr == nullptr) return TRI_ERR_NULL;
+    if ((k > 1 && t->stride[1] != 1) || (T > 1 && t->stride[0] != k)) return TRI_ERR_STRIDE;
+    if (((uintptr_t)t->ptr & 3u) != 0) return TRI_ERR_ALIGN;
+  }
+  return TRI_OK;
+}
+
+struct ExpertSizes {
+  int64_t T, k, E, N, F;
+  int64_t n() const { return T * k; }
+};
+// most workgroups of a call: row tiles of 32 by column tiles of 128
+bool too_many_tiles(int64_t row_tiles, int64_t cols) { return row_tiles * ((cols + 127) / 128) > kMaxBlocks; }
+int check_expert_sizes(const ExpertSizes& z) {
+  if (z.T < 0 || z.k < 1 || z.E < 1 || z.N < 1 || z.F < 1) return TRI_ERR_SHAPE;
+  if (z.E > tri::kMaxExperts || z.k > 64) return TRI_ERR_UNSUPPORTED;
+  TRI_TRY(check_deep(z.N));
+  TRI_TRY(check_deep(z.F));
+  if (z.T > (1 << 24) || z.n() > (1 << 24)) return TRI_ERR_UNSUPPORTED;
+  const int64_t tiles = (z.n() + 31) / 32 + z.E;
+  return too_many_tiles(tiles, 2 * z.F) || too_many_tiles(tiles, z.N) ? TRI_ERR_UNSUPPORTED : TRI_OK;
+}
+// where a call's buffers begin
+struct ExpertLayout {
+  int64_t hidden, y, rows, tiles, total;
+  explicit ExpertLayout(const ExpertSizes& z) {
+    const int64_t n = z.n();
+    hidden = 0;
+    y = align256(n * z.F * 2);
+    rows = y + align256(n * z.N * 4);
+    tiles = rows + align256(n * 4);
+    total = tiles + align256(16 * (1 + (n + 31) / 32 + (z.E < n ? z.E : n)));
+  }
+};
+
 }  // namespace
 
 // The launch sequences exist once per element type: the same text, compiled against the fp16 kernels
@@ -748,6 +830,137 @@ int tri_cache_attention(const tri_tensor* q, const tri_tensor* k_cache, const tr
   TRI_TRY(tri_validate_cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, p));
   if (cache_is_empty(p)) return TRI_OK;
   return TRI_DISPATCH(q, impl_cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, p, hip_stream));
+}
+
+// ---------------------------------------------------------------- 4-bit weights, routed experts
+int tri_validate_fp4_quantize(const tri_tensor* x, const tri_tensor* codes, const tri_tensor* scales) {
+  return check_fp4_rows(x, codes, scales);
+}
+int tri_fp4_quantize(const tri_tensor* x, tri_tensor* codes, tri_tensor* scales, void* hip_stream) {
+  TRI_TRY(tri_validate_fp4_quantize(x, codes, scales));
+  if (x->shape[0] == 0) return TRI_OK;
+  return TRI_DISPATCH(x, impl_fp4_quantize(x, codes, scales, hip_stream));
+}
+int tri_validate_fp4_dequantize(const tri_tensor* codes, const tri_tensor* scales, const tri_tensor* x) {
+  return check_fp4_rows(x, codes, scales);
+}
+int tri_fp4_dequantize(const tri_tensor* codes, const tri_tensor* scales, tri_tensor* x, void* hip_stream) {
+  TRI_TRY(tri_validate_fp4_dequantize(codes, scales, x));
+  if (x->shape[0] == 0) return TRI_OK;
+  return TRI_DISPATCH(x, impl_fp4_dequantize(codes, scales, x, hip_stream));
+}
+
+int64_t tri_fp4_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t four_bit_x) {
+  if (m < 0 || n < 0) return TRI_ERR_SHAPE;
+  TRI_TRY(check_deep(k));
+  if (n % 8 != 0 || m >= kInt32End || n >= kInt32End || too_many_tiles((m + 31) / 32, n)) return TRI_ERR_UNSUPPORTED;
+  if (m == 0 || n == 0) return 0;
+  return tri::fp4_matmul_workspace((int)m, (int)k, (int)n, four_bit_x != 0);
+}
+
+int tri_validate_fp4_matmul(const tri_tensor* x, const tri_tensor* x_scales, const tri_tensor* w, const tri_tensor* w_scales,
+                            const tri_tensor* workspace, const tri_tensor* out) {
+  if (x == nullptr || w == nullptr || w_scales == nullptr || out == nullptr) return TRI_ERR_NULL;
+  if (x->ndim != 2 || w->ndim != 2 || out->ndim != 2) return TRI_ERR_SHAPE;
+  const int dt = elem_dtype(out);
+  const int64_t M = x->shape[0], N = w->shape[0], K = w->shape[1] < kMaxDeep ? w->shape[1] * 2 : kMaxDeep + 1;
+  TRI_TRY(check_mat(out, M, N, dt));
+  TRI_TRY(check_deep(K));
+  if (x_scales != nullptr) TRI_TRY(check_fp4(x, x_scales, -1, M, K));
+  else TRI_TRY(check_mat(x, M, K, dt));
+  TRI_TRY(check_fp4(w, w_scales, -1, N, K));
+  TRI_TRY(check_ws(workspace));
+  const int64_t need = tri_fp4_workspace_bytes(M, K, N, x_scales != nullptr);
+  if (need < 0) return (int)need;
+  if (M == 0 || N == 0) return TRI_OK;
+  if (row_bytes(x, x_scales != nullptr ? 1 : 2) >= kMaxRowStride || spans_too_much(w, 1) || spans_too_much(w_scales, 1)) return TRI_ERR_UNSUPPORTED;
+  return TRI_OK;
+}
+int tri_fp4_matmul(const tri_tensor* x, const tri_tensor* x_scales, const tri_tensor* w, const tri_tensor* w_scales,
+                   tri_tensor* workspace, tri_tensor* out, void* hip_stream) {
+  TRI_TRY(tri_validate_fp4_matmul(x, x_scales, w, w_scales, workspace, out));
+  if (x->shape[0] == 0 || w->shape[0] == 0) return TRI_OK;
+  return TRI_DISPATCH(out, impl_fp4_matmul(x, x_scales, w, w_scales, workspace, out, hip_stream));
+}
+
+int tri_validate_route(const tri_tensor* logits, const tri_tensor* bias, const tri_tensor* ids, const tri_tensor* weights,
+                       const tri_route_params* p) {
+  if (logits == nullptr || ids == nullptr || weights == nullptr || p == nullptr) return TRI_ERR_NULL;
+  if (logits->dtype != TRI_F16 && logits->dtype != TRI_BF16 && logits->dtype != TRI_F32) return TRI_ERR_DTYPE;
+  if (logits->ndim != 2 || logits->shape[0] < 0 || logits->shape[1] < 1) return TRI_ERR_SHAPE;
+  const int64_t T = logits->shape[0], E = logits->shape[1];
+  if (E > tri::kMaxExperts) return TRI_ERR_UNSUPPORTED;
+  if (p->top_k < 1 || p->top_k > E || p->groups < 1 || p->top_groups < 1 || p->top_groups > p->groups) return TRI_ERR_SHAPE;
+  if (p->top_k > 64 || p->groups > 64 || (p->group_top != 1 && p->group_top != 2)) return TRI_ERR_UNSUPPORTED;
+  if (E % p->groups != 0 || p->top_groups * (E / p->groups) < p->top_k || p->group_top > E / p->groups) return TRI_ERR_SHAPE;
+  if (p->groups == 1 && p->group_top != 1) return TRI_ERR_SHAPE;
+  if (!(p->scale > -INFINITY) || !(p->scale < INFINITY)) return TRI_ERR_UNSUPPORTED;
+  if (T > (int64_t)1 << 25) return TRI_ERR_UNSUPPORTED;  // (a workgroup has at least four tokens)
+  if (bias != nullptr) {
+    if (bias->dtype != TRI_F32) return TRI_ERR_DTYPE;
+    if (bias->ndim != 1 || bias->shape[0] != E) return TRI_ERR_SHAPE;
+    if (bias->ptr == nullptr) return TRI_ERR_NULL;
+    if (E > 1 && bias->stride[0] != 1) return TRI_ERR_STRIDE;
+    if (((uintptr_t)bias->ptr & 3u) != 0) return TRI_ERR_ALIGN;
+  }
+  if (ids->dtype != TRI_I32 || weights->dtype != TRI_F32) return TRI_ERR_DTYPE;
+  TRI_TRY(check_choices(ids, weights, T, p->top_k));
+  if (T == 0) return TRI_OK;
+  if (logits->ptr == nullptr) return TRI_ERR_NULL;
+  if ((E > 1 && logits->stride[1] != 1) || (T > 1 && logits->stride[0] < E)) return TRI_ERR_STRIDE;
+  if (((uintptr_t)logits->ptr & (logits->dtype == TRI_F32 ? 3u : 1u)) != 0) return TRI_ERR_ALIGN;
+  return TRI_OK;
+}
+int tri_route(const tri_tensor* logits, const tri_tensor* bias, tri_tensor* ids, tri_tensor* weights, const tri_route_params* p,
+              void* hip_stream) {
+  TRI_TRY(tri_validate_route(logits, bias, ids, weights, p));
+  if (logits->shape[0] == 0) return TRI_OK;
+  return f16::impl_route(logits, bias, ids, weights, p, hip_stream);
+}
+
+int64_t tri_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts, int64_t n, int64_t f) {
+  const ExpertSizes z{tokens, top_k, experts, n, f};
+  TRI_TRY(check_expert_sizes(z));
+  return tokens == 0 ? 0 : ExpertLayout(z).total;
+}
+
+int tri_validate_experts_ffn(const tri_tensor* x, const tri_tensor* ids, const tri_tensor* weights, const tri_tensor* gate,
+                             const tri_tensor* gate_scales, const tri_tensor* up, const tri_tensor* up_scales,
+                             const tri_tensor* down, const tri_tensor* down_scales, const tri_tensor* workspace,
+                             const tri_tensor* out) {
+  if (x == nullptr || ids == nullptr || weights == nullptr || gate == nullptr || up == nullptr || down == nullptr || out == nullptr) return TRI_ERR_NULL;
+  if (x->ndim != 2 || ids->ndim != 2 || gate->ndim != 3) return TRI_ERR_SHAPE;
+  const int dt = elem_dtype(x);
+  const ExpertSizes z{x->shape[0], ids->shape[1], gate->shape[0], x->shape[1], gate->shape[1]};
+  TRI_TRY(check_mat(x, -1, -1, dt));
+  TRI_TRY(check_mat(out, z.T, z.N, dt));
+  if (ids->dtype != TRI_I32 || weights->dtype != TRI_F32) return TRI_ERR_DTYPE;
+  TRI_TRY(check_expert_sizes(z));
+  TRI_TRY(check_choices(ids, weights, z.T, z.k));
+  if ((gate_scales == nullptr) != (up_scales == nullptr) || (gate_scales == nullptr) != (down_scales == nullptr)) return TRI_ERR_NULL;  // one format
+  const bool w4 = gate_scales != nullptr;
+  const tri_tensor* const w[3] = {gate, up, down};
+  const tri_tensor* const s[3] = {gate_scales, up_scales, down_scales};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t rows = i < 2 ? z.F : z.N, K = i < 2 ? z.N : z.F;
+    if (w4) TRI_TRY(check_fp4(w[i], s[i], z.E, rows, K));
+    else TRI_TRY(check_rows(w[i], z.E, rows, K, dt, 2, 16));
+    if (spans_too_much(w[i], w4 ? 1 : 2) || (w4 && spans_too_much(s[i], 1))) return TRI_ERR_UNSUPPORTED;
+  }
+  if (z.T == 0) return TRI_OK;
+  if (row_bytes(x, 2) >= kMaxRowStride || spans_too_much(x, 2)) return TRI_ERR_UNSUPPORTED;
+  if (workspace == nullptr) return TRI_ERR_NULL;
+  TRI_TRY(check_ws(workspace));
+  if (workspace->shape[0] < ExpertLayout(z).total) return TRI_ERR_SCRATCH;
+  if (((uintptr_t)workspace->ptr & 255u) != 0) return TRI_ERR_ALIGN;
+  return TRI_OK;
+}
+int tri_experts_ffn(const tri_tensor* x, const tri_tensor* ids, const tri_tensor* weights, const tri_tensor* gate,
+                    const tri_tensor* gate_scales, const tri_tensor* up, const tri_tensor* up_scales, const tri_tensor* down,
+                    const tri_tensor* down_scales, tri_tensor* workspace, tri_tensor* out, void* hip_stream) {
+  TRI_TRY(tri_validate_experts_ffn(x, ids, weights, gate, gate_scales, up, up_scales, down, down_scales, workspace, out));
+  if (x->shape[0] == 0) return TRI_OK;
+  return TRI_DISPATCH(x, impl_experts_ffn(x, ids, weights, gate, gate_scales, up, up_scales, down, down_scales, workspace, out, hip_stream));
 }
 
 }  // extern "C"

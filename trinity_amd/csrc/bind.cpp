@@ -103,21 +103,24 @@ struct OneDevice {
   }
 };
 
-// the bytes of a ctypes structure (tri_attn_params, tri_cache_params)
+// the bytes of a ctypes structure (tri_attn_params, tri_cache_params, tri_route_params)
 template <class T>
 struct ParamsOf {
-  static_assert(sizeof(tri_attn_params) != sizeof(tri_cache_params), "told apart by their sizes");
+  static_assert(sizeof(tri_attn_params) != sizeof(tri_cache_params) && sizeof(tri_route_params) != sizeof(tri_cache_params) &&
+                    sizeof(tri_route_params) != sizeof(tri_attn_params), "told apart by their sizes");
   Py_buffer buf{};
   const T* p = nullptr;
   explicit ParamsOf(PyObject* o) {
     if (PyObject_GetBuffer(o, &buf, PyBUF_SIMPLE) != 0) return;
     if (buf.len == (Py_ssize_t)sizeof(T)) p = static_cast<const T*>(buf.buf);
-    else PyErr_SetString(PyExc_TypeError, sizeof(T) == sizeof(tri_attn_params) ? "expected TriAttnParams" : "expected TriCacheParams");
+    else PyErr_SetString(PyExc_TypeError, sizeof(T) == sizeof(tri_attn_params) ? "expected TriAttnParams"
+                         : sizeof(T) == sizeof(tri_cache_params) ? "expected TriCacheParams" : "expected TriRouteParams");
   }
   ~ParamsOf() { if (buf.obj != nullptr) PyBuffer_Release(&buf); }
 };
 using Params = ParamsOf<tri_attn_params>;
 using CacheParams = ParamsOf<tri_cache_params>;
+using RouteParams = ParamsOf<tri_route_params>;
 
 void* stream_of(PyObject* o) { return PyLong_AsVoidPtr(o); }
 
@@ -276,6 +279,59 @@ TRI_BIND(cache_attention) {
     void* s = stream_of(a[10]);
     return call([&] {
       return tri_cache_attention(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], t.p[7], t.p[8], p.p, s);
+    });
+  });
+}
+TRI_BIND(fp4_quantize) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 3, 0, t)) return 0;
+    const OneDevice device(a, 3);
+    if (!device.ok) return 0;
+    void* s = stream_of(a[3]);
+    return call([&] { return tri_fp4_quantize(t.p[0], t.p[1], t.p[2], s); });
+  });
+}
+TRI_BIND(fp4_dequantize) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 3, 0, t)) return 0;
+    const OneDevice device(a, 3);
+    if (!device.ok) return 0;
+    void* s = stream_of(a[3]);
+    return call([&] { return tri_fp4_dequantize(t.p[0], t.p[1], t.p[2], s); });
+  });
+}
+TRI_BIND(fp4_matmul) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 6, 0, t)) return 0;
+    const OneDevice device(a, 6);
+    if (!device.ok) return 0;
+    void* s = stream_of(a[6]);
+    return call([&] { return tri_fp4_matmul(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], s); });
+  });
+}
+TRI_BIND(route) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 4, 1, t, 2)) return 0;
+    const OneDevice device(a, 4);
+    if (!device.ok) return 0;
+    const RouteParams p(a[4]);
+    void* s = stream_of(a[5]);
+    return call([&] { return tri_route(t.p[0], t.p[1], t.p[2], t.p[3], p.p, s); });
+  });
+}
+TRI_BIND(experts_ffn) {
+  return run([&] {
+    Tensors t;
+    if (!marshal(a, n, 11, 0, t, 1)) return 0;
+    const OneDevice device(a, 11);
+    if (!device.ok) return 0;
+    void* s = stream_of(a[11]);
+    return call([&] {
+      return tri_experts_ffn(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], t.p[7], t.p[8], t.p[9], t.p[10], s);
     });
   });
 }
@@ -445,6 +501,173 @@ PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- blocks.Fp4Matmul, Router, ExpertsFfn: as above, what a call returns and the workspace it needs are made here (from the
+// allocator of the current stream, so that calls share neither).
+tri_tensor bytes_of(const at::Tensor& t) {
+  tri_tensor d{};
+  d.ptr = t.data_ptr();
+  d.ndim = 1;
+  d.dtype = TRI_U8;
+  d.shape[0] = t.numel();
+  d.stride[0] = 1;
+  return d;
+}
+PyObject* pair(at::Tensor&& x, at::Tensor&& y) {
+  PyObject *const a = THPVariable_Wrap(std::move(x)), *const b = THPVariable_Wrap(std::move(y));
+  PyObject* const r = a != nullptr && b != nullptr ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return r;
+}
+
+// (x, stream) -> (codes, scales)
+PyObject* fp4_quantize_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 1, 0, t)) return nullptr;
+    const at::Tensor* const x = tensor_of(a[0], "x");
+    if (x == nullptr) return nullptr;
+    const OneDevice device(a, 1);
+    void* s = stream_of(a[1]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    const int64_t rows = x->dim() > 0 ? x->size(0) : 0, cols = x->dim() > 1 ? x->size(1) : 0;
+    at::Tensor codes = new_tensor(*x, {rows, cols / 2}, at::kByte), scales = new_tensor(*x, {rows, cols / 32}, at::kByte);
+    tri_tensor c = describe(codes, TRI_U8), e = describe(scales, TRI_U8);
+    const int st = call([&] { return tri_fp4_quantize(t.p[0], &c, &e, s); });
+    return st != 0 ? PyLong_FromLong(st) : pair(std::move(codes), std::move(scales));
+  });
+}
+// (codes, scales, whether to bfloat16, stream) -> x
+PyObject* fp4_dequantize_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 2, 1, t)) return nullptr;
+    const at::Tensor* const codes = tensor_of(a[0], "codes");
+    if (codes == nullptr) return nullptr;
+    const bool bf16 = PyObject_IsTrue(a[2]) == 1;
+    const OneDevice device(a, 2);
+    void* s = stream_of(a[3]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    at::Tensor x = new_tensor(*codes, {codes->dim() > 0 ? codes->size(0) : 0, codes->dim() > 1 ? codes->size(1) * 2 : 0}, bf16 ? at::kBFloat16 : at::kHalf);
+    tri_tensor d = describe(x, bf16 ? TRI_BF16 : TRI_F16);
+    const int st = call([&] { return tri_fp4_dequantize(t.p[0], t.p[1], &d, s); });
+    return st != 0 ? PyLong_FromLong(st) : THPVariable_Wrap(std::move(x));
+  });
+}
+// (x, x_scales, w, w_scales, out or None, whether x is quantised here, whether the result is bfloat16 (4-bit x), stream) -> out
+PyObject* fp4_matmul_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 5, 2, t)) return nullptr;
+    const at::Tensor *const x = tensor_of(a[0], "x"), *const w = tensor_of(a[2], "w");
+    if (x == nullptr || w == nullptr) return nullptr;
+    const bool quantize = PyObject_IsTrue(a[5]) == 1, bf16 = PyObject_IsTrue(a[6]) == 1;
+    const OneDevice device(a, 5);
+    void* s = stream_of(a[7]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    const int64_t rows = x->dim() > 0 ? x->size(0) : 0, cols = w->dim() > 0 ? w->size(0) : 0, deep = w->dim() > 1 ? w->size(1) * 2 : 0;
+    const bool four = quantize || t.p[1] != nullptr;
+    const int64_t need = tri_fp4_workspace_bytes(rows, deep, cols, four);
+    if (need < 0) return PyLong_FromLongLong(need);
+    at::Tensor made, codes, scales, room;
+    tri_tensor o, c, e, r;
+    tri_tensor* out = t.p[4];
+    if (out == nullptr) {
+      const at::ScalarType type = t.p[1] != nullptr ? (bf16 ? at::kBFloat16 : at::kHalf) : x->scalar_type();
+      made = new_tensor(*x, {rows, cols}, type);
+      o = describe(made, type == at::kBFloat16 ? TRI_BF16 : (type == at::kHalf ? TRI_F16 : TRI_F32));
+      out = &o;
+    }
+    if (need > 0) {
+      room = new_tensor(*x, {need}, at::kByte);
+      r = bytes_of(room);
+    }
+    tri_tensor *xp = t.p[0], *sp = t.p[1];
+    if (quantize) {
+      if (out->dtype != xp->dtype) return PyLong_FromLong(TRI_ERR_DTYPE);
+      codes = new_tensor(*x, {rows, deep / 2}, at::kByte);
+      scales = new_tensor(*x, {rows, deep / 32}, at::kByte);
+      c = describe(codes, TRI_U8);
+      e = describe(scales, TRI_U8);
+      // (a call that is refused enqueues nothing)
+      int st = tri_validate_fp4_quantize(xp, &c, &e);
+      if (st == 0) st = tri_validate_fp4_matmul(&c, &e, t.p[2], t.p[3], need > 0 ? &r : nullptr, out);
+      if (st == 0) st = call([&] { return tri_fp4_quantize(xp, &c, &e, s); });
+      if (st != 0) return PyLong_FromLong(st);
+      xp = &c;
+      sp = &e;
+    }
+    const int st = call([&] { return tri_fp4_matmul(xp, sp, t.p[2], t.p[3], need > 0 ? &r : nullptr, out, s); });
+    if (st != 0) return PyLong_FromLong(st);
+    if (made.defined()) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(a[4]);
+    return a[4];
+  });
+}
+// (logits, bias, parameters, stream) -> (ids, weights)
+PyObject* route_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 2, 1, t)) return nullptr;
+    const at::Tensor* const logits = tensor_of(a[0], "logits");
+    if (logits == nullptr) return nullptr;
+    const RouteParams p(a[2]);
+    if (PyErr_Occurred() != nullptr) return nullptr;
+    const OneDevice device(a, 2);
+    void* s = stream_of(a[3]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    const int64_t sizes[2] = {logits->dim() > 0 ? logits->size(0) : 0, p.p->top_k > 0 ? p.p->top_k : 0};
+    at::Tensor ids = new_tensor(*logits, sizes, at::kInt), weights = new_tensor(*logits, sizes, at::kFloat);
+    tri_tensor i = describe(ids, TRI_I32), w = describe(weights, TRI_F32);
+    const int st = call([&] { return tri_route(t.p[0], t.p[1], &i, &w, p.p, s); });
+    return st != 0 ? PyLong_FromLong(st) : pair(std::move(ids), std::move(weights));
+  });
+}
+// (x, ids, weights, gate, gate_scales, up, up_scales, down, down_scales, out or None, stream) -> out
+PyObject* experts_ffn_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return run_new([&]() -> PyObject* {
+    Tensors t;
+    if (!marshal(a, n, 10, 0, t, 1)) return nullptr;
+    const at::Tensor *const x = tensor_of(a[0], "x"), *const ids = tensor_of(a[1], "ids"), *const gate = tensor_of(a[3], "the gate's weights");
+    if (x == nullptr || ids == nullptr || gate == nullptr) return nullptr;
+    const OneDevice device(a, 10);
+    void* s = stream_of(a[10]);
+    if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
+    if (x->dim() != 2 || ids->dim() != 2 || gate->dim() != 3) return PyLong_FromLong(TRI_ERR_SHAPE);
+    const int64_t need = tri_experts_workspace_bytes(x->size(0), ids->size(1), gate->size(0), x->size(1), gate->size(1));
+    if (need < 0) return PyLong_FromLongLong(need);
+    at::Tensor made, room = new_tensor(*x, {need}, at::kByte);
+    tri_tensor o, r = bytes_of(room);
+    tri_tensor* out = t.p[9];
+    if (out == nullptr) {
+      made = at::empty(x->sizes(), x->options());
+      o = describe(made, t.p[0]->dtype);
+      out = &o;
+    }
+    const int st = call([&] {
+      return tri_experts_ffn(t.p[0], t.p[1], t.p[2], t.p[3], t.p[4], t.p[5], t.p[6], t.p[7], t.p[8], &r, out, s);
+    });
+    if (st != 0) return PyLong_FromLong(st);
+    if (made.defined()) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(a[9]);
+    return a[9];
+  });
+}
+PyObject* fp4_workspace_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) return PyErr_Format(PyExc_TypeError, "expected 4 arguments, got %zd", n);
+  const long long m = PyLong_AsLongLong(a[0]), k = PyLong_AsLongLong(a[1]), c = PyLong_AsLongLong(a[2]);
+  const long four = PyLong_AsLong(a[3]);
+  if (PyErr_Occurred() != nullptr) return nullptr;
+  return PyLong_FromLongLong(tri_fp4_workspace_bytes(m, k, c, four != 0));
+}
+PyObject* experts_workspace_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) return PyErr_Format(PyExc_TypeError, "expected 5 arguments, got %zd", n);
+  long long v[5];
+  for (int i = 0; i < 5; ++i) v[i] = PyLong_AsLongLong(a[i]);
+  if (PyErr_Occurred() != nullptr) return nullptr;
+  return PyLong_FromLongLong(tri_experts_workspace_bytes(v[0], v[1], v[2], v[3], v[4]));
+}
+
 PyObject* cache_scratch_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) return PyErr_Format(PyExc_TypeError, "expected 2 arguments, got %zd", n);
   const CacheParams p(a[0]);
@@ -478,6 +701,11 @@ PyMethodDef methods[] = {
     TRI_METHOD("cache_append", cache_append), TRI_METHOD("cache_read", cache_read),
     TRI_METHOD("cache_attention", cache_attention), TRI_METHOD("cache_append_rows", cache_append_rows),
     TRI_METHOD("cache_read_rows", cache_read_rows), TRI_METHOD("cache_attend", cache_attend), TRI_METHOD("cache_scratch_bytes", cache_scratch_bytes),
+    TRI_METHOD("fp4_quantize", fp4_quantize), TRI_METHOD("fp4_dequantize", fp4_dequantize), TRI_METHOD("fp4_matmul", fp4_matmul),
+    TRI_METHOD("route", route), TRI_METHOD("experts_ffn", experts_ffn), TRI_METHOD("fp4_quantize_new", fp4_quantize_new),
+    TRI_METHOD("fp4_dequantize_new", fp4_dequantize_new), TRI_METHOD("fp4_matmul_new", fp4_matmul_new), TRI_METHOD("route_new", route_new),
+    TRI_METHOD("experts_ffn_new", experts_ffn_new), TRI_METHOD("fp4_workspace_bytes", fp4_workspace_bytes),
+    TRI_METHOD("experts_workspace_bytes", experts_workspace_bytes),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

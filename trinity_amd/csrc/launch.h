@@ -311,6 +311,93 @@ struct CachePlan {
 CachePlan cache_plan(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
 int64_t cache_attn_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int kv_len, int window, int sinks, bool four_bit);
 
+// ---- 4-bit blocks of 32 along rows (fp4.h), and products over weights in them or in 16 bits, of all rows or of each expert's
+struct Fp4RowsArgs {
+  half_t* x;  // [M, K]
+  int64_t ldx;
+  uint8_t *codes, *scales;  // [M, K / 2], [M, K / 32]
+  int64_t ldc, lds;
+  int M, K;
+};
+int launch_fp4_quantize(const Fp4RowsArgs& a, hipStream_t stream);
+int launch_fp4_dequantize(const Fp4RowsArgs& a, hipStream_t stream);
+
+struct RouteArgs {
+  const void* logits;  // [T, E]; dtype: 0 fp16, 1 bf16, 2 fp32
+  int64_t ldl;
+  int dtype;
+  const float* bias;  // nullable [E]
+  int32_t* ids;       // [T, k]
+  float* weights;     // [T, k]
+  int64_t T;
+  int E, k, sigmoid, groups, top_groups, group_top, renormalize;
+  float scale;
+};
+int launch_route(const RouteArgs& a, hipStream_t stream);
+
+// rows: choices (token * k + i) of expert 0, 1, ... in ascending order each; tiles: {number of tiles, of rows}, then {expert, first
+// place in rows, rows} of tiles of bm rows
+struct ExpertRowsArgs {
+  const int32_t* ids;
+  int n, E, bm;
+  int32_t* rows;
+  int4* tiles;
+};
+int launch_expert_rows(const ExpertRowsArgs& a, hipStream_t stream);
+constexpr int kMaxExperts = 512;
+
+struct JoinRowsArgs {
+  const float* y;
+  const int32_t* ids;    // with weights: choices out of [0, E) count nothing
+  const float* weights;  // nullable: the k parts of a product are summed
+  half_t* out;
+  int64_t ldo, T;
+  int k, E, N;
+};
+int launch_join_rows(const JoinRowsArgs& a, hipStream_t stream);
+
+// out[r, n] = sum over k of x[r, k] * w[n, k].  Strides of weights in bytes: w_ld between the columns n, w_se between experts.
+enum GroupKind {
+  kGroupRows,      // out = the product of M rows
+  kGroupParts,     // ... its parts of K: y [ksplit][M][N]
+  kGroupGate,      // out[place] = silu(x . w[0]) * (x . w[1]) for every choice of an expert
+  kGroupDown,      // y[choice] = the product, in 32 bits
+  kGroupDownOne,   // few rows only: out = the sum over the choices of one token, weighted
+};
+struct GroupArgs {
+  const uint8_t* x;  // 16-bit rows, or codes (xs: their scales); strides in bytes
+  int64_t ldx;
+  const uint8_t* xs;
+  int64_t ldxs;
+  const uint8_t* w[2];
+  int64_t w_se[2], w_ld[2];
+  const uint8_t* ws[2];  // scales of 4-bit weights (nullptr: 16 bits)
+  int64_t ws_se[2], ws_ld[2];
+  half_t* out;
+  int64_t ldo;
+  float* y;  // [.., N]
+  int M, N, K;
+  // experts
+  const int32_t* ids;    // [n] choices
+  const float* weights;  // [n] (kGroupDownOne)
+  const int32_t* rows;   // ExpertRowsArgs: nullptr on the few-row path, whose places are the choices themselves
+  const int4* tiles;
+  int n, top_k, E;
+  int ksplit;  // parts that K is cut into (kGroupParts; 1 otherwise)
+};
+// few rows (at most kStripRows, or kStripChoices choices of experts)
+constexpr int kStripRows = 16, kStripChoices = 64;
+bool group_strip_takes(const GroupArgs& a, GroupKind kind);
+int launch_group_strip(const GroupArgs& a, GroupKind kind, hipStream_t stream);
+// tiles of rows
+struct GroupPlan {
+  int bm, ksplit;  // rows of a tile, parts of K
+};
+GroupPlan group_rows_plan(int M, int K, int N, bool x4);
+int64_t fp4_matmul_workspace(int M, int K, int N, bool x4);  // bytes for the plan's parts
+int group_tile_rows(int choices, int experts);  // rows of a tile for the rows of experts
+int launch_group_tile(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream);
+
 }  // namespace tri
 
 #endif  // once per element type

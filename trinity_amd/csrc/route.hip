@@ -1,0 +1,286 @@
+// Routing of tokens to experts (tri_route), and the order in which the experts' products take their rows.
+//
+// Routing: with s the softmax or sigmoid of a token's logits and c = s + bias, the top_k experts of the largest c in descending
+// order (ties: the lowest index), out of the top_groups best groups (a group counts the sum of its group_top largest c); weights
+// are s of the chosen, over their sum if renormalised, times a factor.
+//
+// Scores and choices are computed in 64 bits: which expert is chosen is a whole number, and two scores that 32 bits cannot tell
+// apart are common among millions of them.  The arithmetic is small all the same (4096 x 256 exponentials: the matrix would take
+// as long to read as they to compute).
+//
+// A token has LPT lanes of a wave, each with EPL experts next to each other.
+#include "common.h"
+#include "launch.h"
+
+namespace tri {
+
+constexpr int kRouteThreads = 256;
+
+// a double's bits in an order that unsigned integers have; NaN (of either sign) below everything
+__device__ __forceinline__ uint64_t order_key(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  if (x != x) return 0;
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+
+template <int LPT>
+__device__ __forceinline__ double lanes_sum(double x) {
+#pragma unroll
+  for (int o = LPT / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+template <int LPT>
+__device__ __forceinline__ double lanes_max(double x) {
+#pragma unroll
+  for (int o = LPT / 2; o > 0; o >>= 1) x = fmax(x, __shfl_xor(x, o));
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ double logit_of(const void* p, int64_t i) { return (double)(float)static_cast<const T*>(p)[i]; }
+
+template <int LPT, int EPL>
+__global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a) {
+  constexpr int TPB = kRouteThreads / LPT;  // tokens per workgroup
+  __shared__ double choice_s[LPT == 64 ? TPB * 64 * EPL : 1];  // (groups: a wave per token)
+  const int lane = threadIdx.x & (LPT - 1), slot = threadIdx.x / LPT;
+  const int64_t token = (int64_t)blockIdx.x * TPB + slot;
+  const bool live = token < a.T;  // (lanes of other tokens take part in the exchanges below)
+  const int64_t row = (live ? token : a.T - 1) * a.ldl;
+  double s[EPL];
+  bool in[EPL];
+  double top = -__builtin_inf();
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = lane * EPL + j;
+    in[j] = e < a.E;
+    double z = -__builtin_inf();
+    if (in[j]) {
+      z = a.dtype == 2 ? logit_of<float>(a.logits, row + e)
+                       : (a.dtype == 1 ? logit_of<__bf16>(a.logits, row + e) : logit_of<_Float16>(a.logits, row + e));
+    }
+    s[j] = z;
+    top = fmax(top, z);
+  }
+  if (a.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s[j] = in[j] ? 1.0 / (1.0 + exp(-s[j])) : 0.0;
+  } else {
+    top = lanes_max<LPT>(top);
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      s[j] = in[j] ? (s[j] == -__builtin_inf() ? 0.0 : exp(s[j] - top)) : 0.0;  // (no logit above -inf: zeros, not NaN)
+      sum += s[j];
+    }
+    sum = lanes_sum<LPT>(sum);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] / sum;
+  }
+  double c[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) c[j] = s[j] + (a.bias != nullptr && in[j] ? (double)a.bias[lane * EPL + j] : 0.0);
+  if constexpr (LPT == 64) {
+    if (a.groups > 1) {
+      double* const mine = choice_s + slot * 64 * EPL;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) mine[lane * EPL + j] = c[j];
+      __syncthreads();
+      // lane g: the score of group g, and its place among all
+      const int size = a.E / a.groups;
+      uint64_t key = 0;
+      if (lane < a.groups) {
+        double m1 = -__builtin_inf(), m2 = -__builtin_inf();
+        for (int i = 0; i < size; ++i) {
+          const double v = mine[lane * size + i];
+          if (v > m1) {
+            m2 = m1;
+            m1 = v;
+          } else if (v > m2) {
+            m2 = v;
+          }
+        }
+        key = order_key(a.group_top == 2 ? m1 + m2 : m1);
+      }
+      int place = 0;
+      for (int g = 0; g < a.groups; ++g) {
+        const uint64_t other = __shfl(key, g);
+        place += (other > key || (other == key && g < lane)) ? 1 : 0;
+      }
+      const uint64_t stays = __ballot(lane < a.groups && place < a.top_groups);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) in[j] = in[j] && ((stays >> ((lane * EPL + j) / size)) & 1);
+    }
+  }
+  uint64_t key[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) key[j] = order_key(c[j]);
+  double sum = 0.0, my_w = 0.0;
+  int my_id = 0;
+  for (int r = 0; r < a.k; ++r) {
+    // this lane's best: largest key, lowest index
+    uint64_t bk = 0;
+    int be = 1 << 30;
+    double bs = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (in[j] && (be == (1 << 30) || key[j] > bk)) {
+        bk = key[j];
+        be = lane * EPL + j;
+        bs = s[j];
+      }
+    }
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) {
+      const uint64_t ok = __shfl_xor(bk, o);
+      const int oe = __shfl_xor(be, o);
+      const double os = __shfl_xor(bs, o);
+      const bool take = oe != (1 << 30) && (be == (1 << 30) || ok > bk || (ok == bk && oe < be));
+      bk = take ? ok : bk;
+      be = take ? oe : be;
+      bs = take ? os : bs;
+    }
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) in[j] = in[j] && be != lane * EPL + j;
+    sum += bs;
+    my_id = r == lane ? be : my_id;
+    my_w = r == lane ? bs : my_w;
+  }
+  if (live && lane < a.k) {  // (top_k is at most LPT)
+    a.ids[token * a.k + lane] = my_id;
+    const double w = !a.renormalize ? my_w : (sum == 0.0 ? 0.0 : my_w / sum);
+    a.weights[token * a.k + lane] = (float)(w * (double)a.scale);
+  }
+}
+
+template <int LPT, int EPL>
+static int launch_route_t(const RouteArgs& a, hipStream_t stream) {
+  constexpr int TPB = kRouteThreads / LPT;
+  hipLaunchKernelGGL((route_kernel<LPT, EPL>), dim3((unsigned)((a.T + TPB - 1) / TPB)), dim3(kRouteThreads), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+int launch_route(const RouteArgs& a, hipStream_t stream) {
+  // (lanes per token are at least the experts, up to 64, and so at least top_k; groups want a wave per token)
+  if (a.E <= 8 && a.groups == 1) return launch_route_t<8, 1>(a, stream);
+  if (a.E <= 16 && a.groups == 1) return launch_route_t<16, 1>(a, stream);
+  if (a.E <= 32 && a.groups == 1) return launch_route_t<32, 1>(a, stream);
+  if (a.E <= 64) return launch_route_t<64, 1>(a, stream);
+  if (a.E <= 128) return launch_route_t<64, 2>(a, stream);
+  if (a.E <= 256) return launch_route_t<64, 4>(a, stream);
+  return launch_route_t<64, 8>(a, stream);
+}
+
+
+// ---------------------------------------------------------------------------
+// The rows of every expert next to each other: places (row of a token's choice, token * top_k + i) in ascending order for each
+// expert, and the row tiles of `bm` that the experts' products take.  One workgroup: a wave counts and places a contiguous
+// sixteenth of the choices, 64 at a time, so that the order does not depend on timing.
+// ---------------------------------------------------------------------------
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+
+__global__ __launch_bounds__(kSortThreads) void expert_rows_kernel(ExpertRowsArgs a) {
+  extern __shared__ int sort_lds[];
+  int* const base = sort_lds;                  // [waves][E]: counts, then where a wave's rows of an expert begin
+  int* const start = base + kSortWaves * a.E;  // [E]
+  int* const tiles = start + a.E;              // [E]
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  for (int i = t; i < kSortWaves * a.E; i += kSortThreads) base[i] = 0;
+  __syncthreads();
+  const int rounds = (a.n + kSortThreads - 1) / kSortThreads;  // of 64 choices per wave
+  const int s0 = wave * rounds * 64 + lane;
+  int* const mine = base + wave * a.E;
+  for (int r = 0; r < rounds; ++r) {
+    const int s = s0 + r * 64;
+    const int e = s < a.n ? a.ids[s] : -1;
+    if (e >= 0 && e < a.E) atomicAdd(&mine[e], 1);
+  }
+  __syncthreads();
+  for (int e = t; e < a.E; e += kSortThreads) {
+    int sum = 0;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = base[w * a.E + e];
+      base[w * a.E + e] = sum;
+      sum += c;
+    }
+    start[e] = sum;
+    tiles[e] = (sum + a.bm - 1) / a.bm;
+  }
+  __syncthreads();
+  if (wave == 0) {  // exclusive sums over the experts
+    int rows0 = 0, tiles0 = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+      const int e = e0 + lane;
+      const int rc = e < a.E ? start[e] : 0, tc = e < a.E ? tiles[e] : 0;
+      int ri = rc, ti = tc;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int ro = __shfl_up(ri, o), to = __shfl_up(ti, o);
+        ri += lane >= o ? ro : 0;
+        ti += lane >= o ? to : 0;
+      }
+      if (e < a.E) {
+        const int rb = rows0 + ri - rc, tb = tiles0 + ti - tc;
+        start[e] = rb;
+        for (int i = 0; i < tc; ++i) a.tiles[1 + tb + i] = make_int4(e, rb + i * a.bm, min(a.bm, rc - i * a.bm), 0);
+      }
+      rows0 += __shfl(ri, 63);
+      tiles0 += __shfl(ti, 63);
+    }
+    if (lane == 0) a.tiles[0] = make_int4(tiles0, rows0, 0, 0);
+  }
+  __syncthreads();
+  for (int r = 0; r < rounds; ++r) {
+    const int s = s0 + r * 64;
+    const int e = s < a.n ? a.ids[s] : -1;
+    const bool real = e >= 0 && e < a.E;
+    uint64_t same = __ballot(real);  // lanes of this one's expert
+    for (int b = 0; (1 << b) < a.E; ++b) {
+      const uint64_t bit = __ballot((e >> b) & 1);
+      same &= ((e >> b) & 1) ? bit : ~bit;
+    }
+    if (real) {
+      const int rank = __popcll(same & ((1ull << lane) - 1)), at = mine[e];
+      a.rows[start[e] + at + rank] = s;
+      if (rank == 0) mine[e] = at + __popcll(same);  // (a wave's reads of LDS come before its later writes)
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+int launch_expert_rows(const ExpertRowsArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(expert_rows_kernel, dim3(1), dim3(kSortThreads), (kSortWaves + 2) * a.E * sizeof(int), stream, a);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+// out[t] = sum of w[t, i] * y[t * k + i] over the choices i that are experts, in 32 bits; or (no weights) the sum of the k parts
+// of a product, y[i * T + t].
+__global__ __launch_bounds__(256) void join_rows_kernel(JoinRowsArgs a) {
+  const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+  if (c >= a.N) return;
+  for (int64_t t = blockIdx.y; t < a.T; t += gridDim.y) {
+    float4v s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.k; ++i) {
+      float w = 1.0f;
+      int64_t row = i * a.T + t;
+      if (a.weights != nullptr) {
+        row = t * a.k + i;
+        const int e = a.ids[row];
+        if (e < 0 || e >= a.E) continue;
+        w = a.weights[row];
+      }
+      const float4v v = *reinterpret_cast<const float4v*>(a.y + row * a.N + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = fmaf(w, v[j], s[j]);
+    }
+    const half4v h = {(half_t)s[0], (half_t)s[1], (half_t)s[2], (half_t)s[3]};
+    *reinterpret_cast<half4v*>(a.out + t * a.ldo + c) = h;
+  }
+}
+
+int launch_join_rows(const JoinRowsArgs& a, hipStream_t stream) {
+  const dim3 grid((a.N / 4 + 255) / 256, (unsigned)(a.T < 65535 ? a.T : 65535));
+  hipLaunchKernelGGL(join_rows_kernel, grid, dim3(256), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace tri

@@ -67,6 +67,18 @@ class TriCacheParams(ctypes.Structure):
     ]
 
 
+class TriRouteParams(ctypes.Structure):
+    _fields_ = [
+        ("top_k", ctypes.c_int32),
+        ("sigmoid", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("top_groups", ctypes.c_int32),
+        ("group_top", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 class TrinityError(RuntimeError):
     def __init__(self, fn, status, text):
         super().__init__("%s failed: status %d (%s)" % (fn, status, text))
@@ -91,6 +103,10 @@ EXPORTS = [
     "tri_cache_append", "tri_validate_cache_append",
     "tri_cache_read", "tri_validate_cache_read",
     "tri_cache_scratch_bytes", "tri_cache_attention", "tri_validate_cache_attention",
+    "tri_fp4_quantize", "tri_validate_fp4_quantize", "tri_fp4_dequantize", "tri_validate_fp4_dequantize",
+    "tri_fp4_workspace_bytes", "tri_fp4_matmul", "tri_validate_fp4_matmul",
+    "tri_route", "tri_validate_route",
+    "tri_experts_workspace_bytes", "tri_experts_ffn", "tri_validate_experts_ffn",
     "tri_diag_issue_probe", "tri_diag_power_probe",
 ]
 
@@ -374,6 +390,76 @@ def cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse,
     st = native().cache_attention(q, k_cache, k_scales, v_cache, v_scales, lens, scratch, lse, out, params, _stream_or_none(q))
     if st:
         _check("tri_cache_attention", st)
+    return st
+
+
+def fp4_quantize(x, codes, scales, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_fp4_quantize", [x, codes, scales], True)
+    st = native().fp4_quantize(x, codes, scales, _stream_or_none(x))
+    if st:
+        _check("tri_fp4_quantize", st)
+    return st
+
+
+def fp4_dequantize(codes, scales, x, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_fp4_dequantize", [codes, scales, x], True)
+    st = native().fp4_dequantize(codes, scales, x, _stream_or_none(codes))
+    if st:
+        _check("tri_fp4_dequantize", st)
+    return st
+
+
+def fp4_workspace_bytes(m, k, n, four_bit_x):
+    """Bytes of workspace with which fp4_matmul runs its fastest plan (0: it needs none)."""
+    b = native().fp4_workspace_bytes(m, k, n, int(bool(four_bit_x)))
+    if b < 0:
+        _check("tri_fp4_workspace_bytes", b)
+    return b
+
+
+def fp4_matmul(x, x_scales, w, w_scales, workspace, out, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_fp4_matmul", [x, x_scales, w, w_scales, workspace, out], True)
+    st = native().fp4_matmul(x, x_scales, w, w_scales, workspace, out, _stream_or_none(x))
+    if st:
+        _check("tri_fp4_matmul", st)
+    return st
+
+
+def route_params(top_k, sigmoid=False, groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0):
+    p = TriRouteParams()
+    p.top_k, p.sigmoid, p.groups, p.top_groups, p.group_top = top_k, int(bool(sigmoid)), groups, top_groups, group_top
+    p.renormalize, p.scale = int(bool(renormalize)), scale
+    return p
+
+
+def route(logits, bias, ids, weights, params, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_route", [logits, bias, _lens(ids), weights, ctypes.byref(params)], True)
+    st = native().route(logits, bias, ids, weights, params, _stream_or_none(logits))
+    if st:
+        _check("tri_route", st)
+    return st
+
+
+def experts_workspace_bytes(tokens, top_k, experts, n, f):
+    """Bytes of workspace of experts_ffn on x [tokens, n] with `experts` experts of width f."""
+    b = native().experts_workspace_bytes(tokens, top_k, experts, n, f)
+    if b < 0:
+        _check("tri_experts_workspace_bytes", b)
+    return b
+
+
+def experts_ffn(x, ids, weights, gate, gate_scales, up, up_scales, down, down_scales, workspace, out, validate_only=False):
+    if validate_only:
+        return _call("tri_validate_experts_ffn", [x, _lens(ids), weights, gate, gate_scales, up, up_scales, down, down_scales,
+                                                  workspace, out], True)
+    st = native().experts_ffn(x, ids, weights, gate, gate_scales, up, up_scales, down, down_scales, workspace, out,
+                              _stream_or_none(x))
+    if st:
+        _check("tri_experts_ffn", st)
     return st
 
 
