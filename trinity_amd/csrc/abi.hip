@@ -507,7 +507,7 @@ struct ExpertLayout {
     const int64_t n = z.n();
     hidden = 0;
     y = align256(n * z.F * 2);
-    rows = y + align256(n * z.N * 4);
+    rows = y + align256(n * z.N * 4 * tri::experts_parts((int)n, (int)z.E, (int)z.N, (int)z.F));
     tiles = rows + align256(n * 4);
     total = tiles + align256(16 * (1 + (n + 31) / 32 + (z.E < n ? z.E : n)));
   }

@@ -14,12 +14,12 @@
 
 namespace tri {
 
-constexpr int kGsCols = 16, kGsWaves = 4, kGsPieceBytes = 128;
+constexpr int kGsCols = 16, kGsPieceBytes = 128;
 
 // LDS piece [16 columns][128 bytes]: 16-byte chunk j (of 8) of column c at slot j ^ ((c >> 1) & 7) - the lanes of a fragment
 // read (16 columns, one chunk) then fall on different banks.  A load instruction fetches 128 bytes of eight columns.
-template <bool W4, GroupKind KIND, int NST>
-__global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a) {
+template <bool W4, GroupKind KIND, int NW, int NST>
+__global__ __launch_bounds__(NW * 64) void group_strip_kernel(GroupArgs a) {
   extern __shared__ __attribute__((aligned(16))) half_t lds[];
   __shared__ int list[kStripChoices];
   constexpr int NM = KIND == kGroupGate ? 2 : 1;       // weight matrices
@@ -30,11 +30,11 @@ __global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  // neighbouring columns on one XCD
-  const int strips = (a.N + kGsCols - 1) / kGsCols;
-  const int total = gridDim.x, per = total >> 3, rem = total & 7, xcd = (int)blockIdx.x & 7;
-  const int id = xcd * per + (xcd < rem ? xcd : rem) + ((int)blockIdx.x >> 3);
-  const int n0 = id % strips * kGsCols, choice = id / strips;
+  // neighbouring columns on one XCD, every choice's on all of them
+  const int per = (a.N + 8 * kGsCols - 1) / (8 * kGsCols);  // strips per XCD
+  const int choice = (int)blockIdx.x / (8 * per), at8 = (int)blockIdx.x - choice * 8 * per;
+  const int n0 = ((at8 & 7) * per + (at8 >> 3)) * kGsCols;
+  if (n0 >= a.N) return;
 
   int rows = a.M, expert = 0;
   if constexpr (KIND == kGroupGate || KIND == kGroupDown) {
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a)
   }
   const int np = (a.K + PK - 1) / PK;
   const int pieces = KIND == kGroupDownOne ? np * a.n : np;  // (of all choices of the token, one after the other)
-  const int mine = (pieces - wave + kGsWaves - 1) / kGsWaves;  // pieces wave, wave + 4, ...
+  const int mine = (pieces - wave + NW - 1) / NW;  // pieces wave, wave + 4, ...
 
   char* const ring = reinterpret_cast<char*>(lds) + wave * NST * PIECE;
   int64_t wofs[NM][2], sofs[NM];
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a)
     // piece i of this wave: its first value (the last piece is moved back where K ends within it; its first `skip` steps were
     // those of the piece before), past the end the last one again (the waits count on every load)
     auto at = [&](int i) __attribute__((always_inline)) {
-      const int q = wave + min(i, mine - 1) * kGsWaves;
+      const int q = wave + min(i, mine - 1) * NW;
       At p;
       p.seg = KIND == kGroupDownOne ? q / np : 0;
       const int k = (q - p.seg * np) * PK;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a)
     __syncthreads();
     if (wave == 0) {
 #pragma unroll
-      for (int w = 0; w < kGsWaves - 1; ++w)
+      for (int w = 0; w < NW - 1; ++w)
 #pragma unroll
         for (int m = 0; m < NM; ++m) acc[m] += part[(w * NM + m) * 64 + lane];
       // lane: row c, columns n0 + 4 g .. + 3
@@ -196,18 +196,29 @@ __global__ __launch_bounds__(kGsWaves * 64) void group_strip_kernel(GroupArgs a)
   }
 }
 
+#ifndef STRIPN
+#define STRIPN kStripChoices
+#endif
 bool group_strip_takes(const GroupArgs& a, GroupKind kind) {
   if (a.xs != nullptr || a.K < (a.ws[0] != nullptr ? 256 : 64) || a.K % 32 != 0) return false;
-  return kind == kGroupRows ? a.M <= kStripRows : a.n <= kStripChoices;
+  return kind == kGroupRows ? a.M <= kStripRows : a.n <= STRIPN;
 }
 
 template <bool W4, GroupKind KIND>
 static int launch_strip_kind(const GroupArgs& a, hipStream_t stream) {
-  constexpr int NST = 3, NM = KIND == kGroupGate ? 2 : 1;
-  constexpr int LDS = kGsWaves * NST * NM * kGsCols * kGsPieceBytes;
-  const int strips = (a.N + kGsCols - 1) / kGsCols;
+#ifndef SNW
+#define SNW 4
+#define SNST 3
+#define SNW1 8
+#define SNST1 4
+#endif
+  constexpr bool ONE = KIND == kGroupDownOne || KIND == kGroupRows;
+  constexpr int NW = ONE ? SNW1 : SNW, NST = ONE ? SNST1 : SNST, NM = KIND == kGroupGate ? 2 : 1;
+  constexpr int LDS = NW * NST * NM * kGsCols * kGsPieceBytes;
+  constexpr auto kern = group_strip_kernel<W4, KIND, NW, NST>;
+  if (set_max_lds<kern, LDS>() != 0) return -1;
   const int groups = KIND == kGroupGate || KIND == kGroupDown ? a.n : 1;
-  hipLaunchKernelGGL((group_strip_kernel<W4, KIND, NST>), dim3(strips * groups), dim3(kGsWaves * 64), LDS, stream, a);
+  hipLaunchKernelGGL(kern, dim3((a.N + 8 * kGsCols - 1) / (8 * kGsCols) * 8 * groups), dim3(NW * 64), LDS, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 template <bool W4>

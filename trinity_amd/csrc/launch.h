@@ -349,10 +349,10 @@ constexpr int kMaxExperts = 512;
 struct JoinRowsArgs {
   const float* y;
   const int32_t* ids;    // with weights: choices out of [0, E) count nothing
-  const float* weights;  // nullable: the k parts of a product are summed
+  const float* weights;  // nullable: k is one
   half_t* out;
   int64_t ldo, T;
-  int k, E, N;
+  int k, E, N, parts;  // y: [parts] of them
 };
 int launch_join_rows(const JoinRowsArgs& a, hipStream_t stream);
 
@@ -383,7 +383,7 @@ struct GroupArgs {
   const int32_t* rows;   // ExpertRowsArgs: nullptr on the few-row path, whose places are the choices themselves
   const int4* tiles;
   int n, top_k, E;
-  int ksplit;  // parts that K is cut into (kGroupParts; 1 otherwise)
+  int ksplit;  // parts that K is cut into: y [ksplit][.., N] (kGroupParts, kGroupDown; 1 otherwise)
 };
 // few rows (at most kStripRows, or kStripChoices choices of experts)
 constexpr int kStripRows = 16, kStripChoices = 64;
@@ -395,8 +395,10 @@ struct GroupPlan {
 };
 GroupPlan group_rows_plan(int M, int K, int N, bool x4);
 int64_t fp4_matmul_workspace(int M, int K, int N, bool x4);  // bytes for the plan's parts
-int group_tile_rows(int choices, int experts);  // rows of a tile for the rows of experts
+int experts_parts(int choices, int experts, int N, int F);  // most parts of the down projection, whatever the weights' type
+GroupPlan experts_plan(int choices, int experts, int N, int F, bool w4);  // ksplit: of the down projection
 int launch_group_tile(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream);
+int launch_group_tile_small(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream);
 
 }  // namespace tri
 

@@ -252,23 +252,22 @@ int launch_expert_rows(const ExpertRowsArgs& a, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-// out[t] = sum of w[t, i] * y[t * k + i] over the choices i that are experts, in 32 bits; or (no weights) the sum of the k parts
-// of a product, y[i * T + t].
+// out[t] = sum of w[t, i] * y[t * k + i] over the choices i that are experts, in 32 bits, y being the sum of its parts; or
+// (no weights, k = 1) that sum itself.
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinRowsArgs a) {
   const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
   if (c >= a.N) return;
   for (int64_t t = blockIdx.y; t < a.T; t += gridDim.y) {
     float4v s = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < a.k; ++i) {
+      const int64_t row = t * a.k + i;
       float w = 1.0f;
-      int64_t row = i * a.T + t;
       if (a.weights != nullptr) {
-        row = t * a.k + i;
         const int e = a.ids[row];
         if (e < 0 || e >= a.E) continue;
         w = a.weights[row];
       }
-      const float4v v = *reinterpret_cast<const float4v*>(a.y + row * a.N + c);
+      const float4v v = sum_splits(a.y, a.parts, a.T * a.k * a.N, row * a.N + c);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[j] = fmaf(w, v[j], s[j]);
     }
