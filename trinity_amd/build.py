@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrinity_amd.so")
 NATIVE = os.path.join(HERE, "_native.so")  # CPython binding of LIB for torch tensors (csrc/bind.cpp)
 KERNEL_SOURCES = ["rmsnorm.hip", "ring.hip", "ring_qkv.hip", "strip.hip", "gemm.hip", "attn.hip", "attn_few.hip", "scores.hip", "kvfp8.hip",
-                  "cache_rows.hip", "cache_attn.hip", "fp4_rows.hip", "route.hip", "group_strip.hip", "group_tile.hip",
+                  "cache_rows.hip", "cache_attn.hip", "fp4_rows.hip", "route.hip", "group_strip.hip", "group_stream.hip", "group_tile.hip",
                   "group_tile_small.hip"]
 # every kernel translation unit is compiled twice: for fp16 elements (namespace tri) and, with these defines, for
 # bf16 elements (the same text in namespace tri_bf16); abi.hip dispatches on the element type of a call

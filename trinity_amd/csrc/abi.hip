@@ -489,7 +489,7 @@ struct ExpertSizes {
   int64_t T, k, E, N, F;
   int64_t n() const { return T * k; }
 };
-// most workgroups of a call: row tiles of 32 by column tiles of 128
+// most workgroups of a call: row tiles by column tiles of 128
 bool too_many_tiles(int64_t row_tiles, int64_t cols) { return row_tiles * ((cols + 127) / 128) > kMaxBlocks; }
 int check_expert_sizes(const ExpertSizes& z) {
   if (z.T < 0 || z.k < 1 || z.E < 1 || z.N < 1 || z.F < 1) return TRI_ERR_SHAPE;
@@ -497,7 +497,7 @@ int check_expert_sizes(const ExpertSizes& z) {
   TRI_TRY(check_deep(z.N));
   TRI_TRY(check_deep(z.F));
   if (z.T > (1 << 24) || z.n() > (1 << 24)) return TRI_ERR_UNSUPPORTED;
-  const int64_t tiles = (z.n() + 31) / 32 + z.E;
+  const int64_t tiles = (z.n() + 15) / 16 + z.E;
   return too_many_tiles(tiles, 2 * z.F) || too_many_tiles(tiles, z.N) ? TRI_ERR_UNSUPPORTED : TRI_OK;
 }
 // where a call's buffers begin
@@ -507,9 +507,9 @@ struct ExpertLayout {
     const int64_t n = z.n();
     hidden = 0;
     y = align256(n * z.F * 2);
-    rows = y + align256(n * z.N * 4 * tri::experts_parts((int)n, (int)z.E, (int)z.N, (int)z.F));
+    rows = y + align256(n * z.N * 4 * tri::experts_parts((int)n, (int)z.k, (int)z.E, (int)z.N, (int)z.F));
     tiles = rows + align256(n * 4);
-    total = tiles + align256(16 * (1 + (n + 31) / 32 + (z.E < n ? z.E : n)));
+    total = tiles + align256(16 * (1 + (n + 15) / 16 + (z.E < n ? z.E : n)));
   }
 };
 

@@ -3,6 +3,9 @@
 
 namespace tri {
 
+#ifndef STREAMMEAN
+#define STREAMMEAN 10
+#endif
 // parts of K for `tiles` tiles: so many that every CU has one, of at least 512 values
 static int parts_of(int tiles, int K) {
   const int deep = (K + 255) / 256;
@@ -12,9 +15,15 @@ static int parts_of(int tiles, int K) {
   return (deep + per - 1) / per;  // (no part is empty)
 }
 
-GroupPlan experts_plan(int choices, int experts, int N, int F, bool w4) {
+GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w4) {
   GroupPlan p;
   const int mean = (choices + experts - 1) / experts;
+  const int rows = choices / top_k < 16 ? choices / top_k : 16;  // (of an expert, at most, if a token chooses it once)
+  if (w4 && mean <= STREAMMEAN && group_stream_takes(rows, N, false) && group_stream_takes(rows, F, true)) {
+    p.bm = 16;
+    p.ksplit = group_stream_parts(rows, F, N, choices < experts ? choices : experts);
+    return p;
+  }
   p.bm = mean <= 24 ? 32 : (mean <= 64 ? 64 : (mean <= 256 ? 128 : 256));
   const int bn = p.bm == 32 || p.bm == 256 ? 256 : 128;
   const int groups = choices < experts ? choices : experts;
@@ -22,8 +31,8 @@ GroupPlan experts_plan(int choices, int experts, int N, int F, bool w4) {
   return p;
 }
 
-int experts_parts(int choices, int experts, int N, int F) {
-  const int a = experts_plan(choices, experts, N, F, false).ksplit, b = experts_plan(choices, experts, N, F, true).ksplit;
+int experts_parts(int choices, int top_k, int experts, int N, int F) {
+  const int a = experts_plan(choices, top_k, experts, N, F, false).ksplit, b = experts_plan(choices, top_k, experts, N, F, true).ksplit;
   return a > b ? a : b;
 }
 
@@ -36,15 +45,8 @@ GroupPlan group_rows_plan(int M, int K, int N, bool x4) {
 }
 
 int64_t fp4_matmul_workspace(int M, int K, int N, bool x4) {
-  GroupArgs a{};
-  a.M = M;
-  a.K = K;
-  const uint8_t any = 0;
-  a.ws[0] = &any;
-  a.xs = x4 ? &any : nullptr;
-  if (group_strip_takes(a, kGroupRows)) return 0;
-  const GroupPlan p = group_rows_plan(M, K, N, x4);
-  return p.ksplit > 1 ? (int64_t)p.ksplit * M * N * 4 : 0;
+  const int parts = !x4 && group_stream_takes(M, K, true) ? group_stream_parts(M, K, N, 1) : group_rows_plan(M, K, N, x4).ksplit;
+  return parts > 1 ? (int64_t)parts * M * N * 4 : 0;
 }
 
 template <GroupMul MUL, GroupKind KIND>

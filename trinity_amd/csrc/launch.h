@@ -362,7 +362,6 @@ enum GroupKind {
   kGroupParts,     // ... its parts of K: y [ksplit][M][N]
   kGroupGate,      // out[place] = silu(x . w[0]) * (x . w[1]) for every choice of an expert
   kGroupDown,      // y[choice] = the product, in 32 bits
-  kGroupDownOne,   // few rows only: out = the sum over the choices of one token, weighted
 };
 struct GroupArgs {
   const uint8_t* x;  // 16-bit rows, or codes (xs: their scales); strides in bytes
@@ -379,24 +378,28 @@ struct GroupArgs {
   int M, N, K;
   // experts
   const int32_t* ids;    // [n] choices
-  const float* weights;  // [n] (kGroupDownOne)
   const int32_t* rows;   // ExpertRowsArgs: nullptr on the few-row path, whose places are the choices themselves
   const int4* tiles;
   int n, top_k, E;
   int ksplit;  // parts that K is cut into: y [ksplit][.., N] (kGroupParts, kGroupDown; 1 otherwise)
+  int kw, tpw, row_block, col_blocks;  // set by launch_group_stream
 };
-// few rows (at most kStripRows, or kStripChoices choices of experts)
+// a decode step's experts: at most kStripChoices choices, over 16-bit weights
 constexpr int kStripRows = 16, kStripChoices = 64;
-bool group_strip_takes(const GroupArgs& a, GroupKind kind);
+bool group_strip_takes(const GroupArgs& a);
 int launch_group_strip(const GroupArgs& a, GroupKind kind, hipStream_t stream);
+// few rows over 4-bit weights (at most 16 of all, or `rows` of each of about `groups` groups; grid_groups: as many as there can be)
+bool group_stream_takes(int rows, int K, bool may_split);  // may_split: kGroupParts, kGroupDown
+int group_stream_parts(int rows, int K, int N, int groups);  // parts of K (kGroupParts, kGroupDown)
+int launch_group_stream(const GroupArgs& a, GroupKind kind, int rows, int groups, int grid_groups, hipStream_t stream);
 // tiles of rows
 struct GroupPlan {
   int bm, ksplit;  // rows of a tile, parts of K
 };
 GroupPlan group_rows_plan(int M, int K, int N, bool x4);
 int64_t fp4_matmul_workspace(int M, int K, int N, bool x4);  // bytes for the plan's parts
-int experts_parts(int choices, int experts, int N, int F);  // most parts of the down projection, whatever the weights' type
-GroupPlan experts_plan(int choices, int experts, int N, int F, bool w4);  // ksplit: of the down projection
+int experts_parts(int choices, int top_k, int experts, int N, int F);  // most parts of the down projection, whatever the weights' type
+GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w4);  // bm 16: group_stream; ksplit: of the down projection
 int launch_group_tile(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream);
 int launch_group_tile_small(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream);
 
