@@ -41,26 +41,36 @@ template <int BM_, int BN_, int WM_, int WN_, int NA_, int NB_, GroupMul MUL_>
 struct GroupTile {
   static constexpr GroupMul MUL = MUL_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NA = NA_, NB = NB_;
+  static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
-  static constexpr int XI = BM / 32, WI = BN / 32;  // 1 KB load instructions per wave and tile
+  static constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW;  // 1 KB load instructions per wave and tile
   static constexpr bool XS = MUL == kMul44, WS = MUL != kMul16;
-  static constexpr int SROWS = (WS ? BN : 0) + (XS ? BM : 0), SR = (SROWS + 255) / 256;  // rows of scales, per thread
+  static constexpr int SROWS = (WS ? BN : 0) + (XS ? BM : 0), SR = (SROWS + NT - 1) / NT;  // rows of scales, per thread
   static constexpr int SUB = MUL == kMul164 ? 4 : 1;  // k tiles of rows per tile of weights
   static constexpr int KX = MUL == kMul44 ? 256 : 64, KW = MUL == kMul16 ? 64 : 256;
-  static constexpr int X_BYTES = BM * 128, W_BYTES = BN * 128, S_BYTES = SROWS * 8;
-  static constexpr int X_OFF = 0, W_OFF = NA * X_BYTES, S_OFF = W_OFF + NB * W_BYTES;
-  static constexpr int LOOP_BYTES = S_OFF + 2 * S_BYTES, STAGED_BYTES = 4 * TM * (TN + 8) * 2;  // (STAGED: of the epilogue)
+  static constexpr int W_BYTES = BN * 128, S_BYTES = SROWS * 8;
+  // a tile whose waves have `live` row blocks: bytes of a k tile's rows, and how many k tiles of them LDS holds
+  static constexpr int x_bytes(int live) { return live * WM * 32 * 128; }
+  static constexpr int na(int live) { return MUL == kMul164 && MI == 4 && live < 4 ? (live == 3 ? 3 : 4) : NA; }
+  static constexpr int x_room() {
+    int most = 0;
+    for (int l = 1; l <= MI; ++l) most = most > na(l) * x_bytes(l) ? most : na(l) * x_bytes(l);
+    return most;
+  }
+  static constexpr int X_OFF = 0, W_OFF = x_room(), S_OFF = W_OFF + NB * W_BYTES;
+  static constexpr int LOOP_BYTES = S_OFF + 2 * S_BYTES, STAGED_BYTES = NW * TM * (TN + 8) * 2;  // (STAGED: of the epilogue)
   static constexpr int LDS_BYTES = LOOP_BYTES > STAGED_BYTES ? LOOP_BYTES : STAGED_BYTES;
   static constexpr bool DEEP = MI * NI <= 4;  // fragments are read a whole k tile ahead (see there)
   static constexpr bool LATE = NB > NA && SUB == 1;  // weights are requested in the first step of a tile
-  static_assert(WM * WN == 4 && BM % 32 == 0 && BN % 32 == 0 && TM % 32 == 0 && TN % 32 == 0, "four waves");
+  static_assert((NW == 4 || NW == 8) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0, "four or eight waves");
+  static_assert(WM * 4 % NW == 0, "whole load instructions for a row block of every wave");
   static_assert(NA >= 2 && NB >= 2 && LDS_BYTES <= 160 * 1024, "LDS budget");
   static_assert(NA == NB || LATE || SUB == 4, "waits below");
   static_assert(!LATE || (NA == 2 && NB == 3), "waits below");
   static_assert(SUB == 1 || NA <= 4, "waits below");
-  // loads that may be on their way at the barrier of a tile
-  static constexpr int INFLIGHT = SUB == 4 ? (NA - 2) * XI : (LATE ? WI : (NA - 2) * (XI + WI));
-  static_assert(INFLIGHT + WI < 64, "vmcnt");
+  // loads that may be on their way at the barrier of a tile; xi: those of rows per wave and tile
+  static constexpr int inflight(int na, int xi) { return SUB == 4 ? (na - 2) * xi : (LATE ? WI : (na - 2) * (xi + WI)); }
+  static_assert(inflight(NA, XI) + WI < 64, "vmcnt");
 };
 
 __device__ __forceinline__ void dma16(const void* g, void* l) {
@@ -68,7 +78,7 @@ __device__ __forceinline__ void dma16(const void* g, void* l) {
 }
 
 template <class T, GroupKind KIND>
-__global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
+__global__ __launch_bounds__(T::NT) void group_tile_kernel(GroupArgs a) {
   extern __shared__ __attribute__((aligned(16))) half_t lds_h[];
   char* const lds = reinterpret_cast<char*>(lds_h);
   constexpr bool GATE = KIND == kGroupGate, ALL = KIND == kGroupRows || KIND == kGroupParts;
@@ -128,34 +138,34 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
   };
   uint32_t xofs[T::XI], wofs[T::WI];
 #pragma unroll
-  for (int i = 0; i < T::XI; ++i) xofs[i] = (uint32_t)input_row((i * 4 + wave) * 8 + (lane >> 3)) * (uint32_t)a.ldx;
+  for (int i = 0; i < T::XI; ++i) xofs[i] = (uint32_t)input_row((i * T::NW + wave) * 8 + (lane >> 3)) * (uint32_t)a.ldx;
 #pragma unroll
   for (int i = 0; i < T::WI; ++i) {
     int m;
-    const int col = column((i * 4 + wave) * 8 + (lane >> 3), m);
+    const int col = column((i * T::NW + wave) * 8 + (lane >> 3), m);
     wofs[i] = (uint32_t)col * (m ? ldw2 : ldw);
   }
   const int nb = (k1 - k0) / 32;  // blocks of this part
   const int xend = (MUL == kMul44 ? (k1 - k0) / 2 : (k1 - k0) * 2) - 16, wend = (MUL == kMul16 ? (k1 - k0) * 2 : (k1 - k0) / 2) - 16;
   // (past the end the loop keeps its load count, which the waits assume)
-  auto load_x = [&](int kt, int buf, int i) {
+  auto load_x = [&](int kt, int buf, int i, int live) __attribute__((always_inline)) {
     const uint32_t k = (uint32_t)min(kt * 128 + chunk * 16, xend);
-    dma16(xbase + (xofs[i] + k), lds + T::X_OFF + buf * T::X_BYTES + (i * 4 + wave) * 1024);
+    dma16(xbase + (xofs[i] + k), lds + T::X_OFF + buf * T::x_bytes(live) + (i * T::NW + wave) * 1024);
   };
   auto load_w = [&](int mt, int buf, int i) {
     const uint32_t k = (uint32_t)min(mt * 128 + chunk * 16, wend);
     int m = 0;
-    if constexpr (GATE) m = (i * 4 + wave) * 8 % T::TN / OUT_TN;
-    dma16((m ? wbase2 : wbase) + (wofs[i] + k), lds + T::W_OFF + buf * T::W_BYTES + (i * 4 + wave) * 1024);
+    if constexpr (GATE) m = (i * T::NW + wave) * 8 % T::TN / OUT_TN;
+    dma16((m ? wbase2 : wbase) + (wofs[i] + k), lds + T::W_OFF + buf * T::W_BYTES + (i * T::NW + wave) * 1024);
   };
-  // scales of rows t and t + 256 (the weights' rows, then the rows')
+  // scales of a thread's rows (the weights', then the rows')
   constexpr int SR = T::SR > 0 ? T::SR : 1;
   const uint8_t* ssrc[SR];
   uint4v skept[SR][2];
   if constexpr (T::WS) {
 #pragma unroll
     for (int j = 0; j < T::SR; ++j) {
-      const int r = min(t + j * 256, T::SROWS - 1);
+      const int r = min(t + j * T::NT, T::SROWS - 1);
       int m;
       const int col = column(min(r, T::BN - 1), m);
       ssrc[j] = T::XS && r >= T::BN ? xsbase + (uint32_t)input_row(r - T::BN) * (uint32_t)a.ldxs
@@ -186,7 +196,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
     const int q = mt & 3;
 #pragma unroll
     for (int j = 0; j < T::SR; ++j) {
-      const int r = t + j * 256;
+      const int r = t + j * T::NT;
       uint2v v;
 #pragma unroll
       for (int e = 0; e < 2; ++e) v[e] = q == 0 ? skept[j][0][e] : (q == 1 ? skept[j][0][2 + e] : (q == 2 ? skept[j][1][e] : skept[j][1][2 + e]));
@@ -204,9 +214,9 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
 
   // ---- fragments
   const int sx = (l32 >> 1) & 7;
-  const int xrow = (wm * T::TM + l32) * 128, wrow = (wn * T::TN + l32) * 128;
+  const int xrow = (wm * 32 + l32) * 128, wrow = (wn * T::TN + l32) * 128;
   const char* const scales = lds + T::S_OFF;  // of a tile: [rows][8]
-  const int s_row = (wn * T::TN + l32) * 8, xs_row = (T::BN + wm * T::TM + l32) * 8;
+  const int s_row = (wn * T::TN + l32) * 8, xs_row = (T::BN + wm * 32 + l32) * 8;
   // Fragments: two sets of a step's, or (DEEP) of a k tile's four steps'.  kMul164 keeps codes and converts them for their MFMAs.
   constexpr int FS = T::DEEP ? 8 : 2;
   half8v xf[FS][T::MI], wf[MUL == kMul164 && T::DEEP ? 1 : FS][T::NI];
@@ -214,7 +224,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
   // scales of the fragments: kMul164 of the block that they are in, kMul44 of the k tile's four steps, for this one and the next
   uint32_t wsc[T::WS ? (MUL == kMul164 ? (T::DEEP ? FS / 2 : 1) : 2) : 1][T::NI], xsc[T::XS ? 2 : 1][T::MI];
   // fragment i of step kk of k tile kt in buffers (xb, wb), into set `buf`: the weights' first, then the rows'
-  auto read_one = [&](int kt, int xb, int wb, int kk, int buf, int i) __attribute__((always_inline)) {
+  auto read_one = [&](int kt, int xb, int wb, int kk, int buf, int i, int live) __attribute__((always_inline)) {
     const int c = MUL == kMul44 ? g * 4 + kk : kk * 2 + g;  // chunk
     const int next = T::DEEP ? buf / 4 : 1;
     if (i < T::NI) {
@@ -230,9 +240,9 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
       }
     } else {
       const int mi = i - T::NI;
-      xf[buf][mi] = *reinterpret_cast<const half8v*>(lds + T::X_OFF + xb * T::X_BYTES + xrow + mi * 32 * 128 + ((c ^ sx) << 4));
+      xf[buf][mi] = *reinterpret_cast<const half8v*>(lds + T::X_OFF + xb * T::x_bytes(live) + xrow + mi * T::WM * 32 * 128 + ((c ^ sx) << 4));
       if constexpr (MUL == kMul44)
-        if (kk == 0) xsc[next][mi] = *reinterpret_cast<const uint32_t*>(scales + (kt & 1) * T::S_BYTES + xs_row + mi * 256 + g * 4);
+        if (kk == 0) xsc[next][mi] = *reinterpret_cast<const uint32_t*>(scales + (kt & 1) * T::S_BYTES + xs_row + mi * T::WM * 256 + g * 4);
     }
   };
   auto convert_one = [&](int buf, int i) __attribute__((always_inline)) {
@@ -248,10 +258,10 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
     for (int mi = 0; mi < T::MI; ++mi)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[ni][mi][r] = 0.f;
-  // MFMA i of step kk, on set `buf`
-  auto mfma_one = [&](int buf, int kk, int i) __attribute__((always_inline)) {
-    const int ni = i / T::MI, mq = i % T::MI;
-    const int mi = (ni & 1) ? T::MI - 1 - mq : mq;  // serpentine: consecutive MFMAs share a source operand
+  // MFMA i of step kk, on set `buf`; `live` row blocks
+  auto mfma_one = [&](int buf, int kk, int i, int live) __attribute__((always_inline)) {
+    const int ni = i / live, mq = i % live;
+    const int mi = (ni & 1) ? live - 1 - mq : mq;  // serpentine: consecutive MFMAs share a source operand
     if constexpr (MUL == kMul44) {
       const uint4v w = __builtin_bit_cast(uint4v, wf[buf][ni]), x = __builtin_bit_cast(uint4v, xf[buf][mi]);
       const int8x w8 = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0}, x8 = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
@@ -274,70 +284,48 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
       for (int i = 0; i < T::MI; ++i) xsc[0][i] = xsc[1][i];
     }
   };
-  constexpr int NM = T::NI * T::MI, NF = T::NI + T::MI;
-  // step kk, slot by slot (a schedule fence after each): MFMA i, its share of `n` loads, and of the fragments of
-  // step rkk of tile rkt into the other set (rkk < 0: none)
-  auto step = [&](int kk, int n, auto load, int rkt, int rxb, int rwb, int rkk) __attribute__((always_inline)) {
-    const int buf = kk & 1;
-#pragma unroll
-    for (int i = 0; i < NM; ++i) {
-      mfma_one(buf, kk, i);
-#pragma unroll
-      for (int j = i * n / NM; j < (i + 1) * n / NM; ++j) load(j);
-      if (rkk >= 0) {
-        if (NM >= 2 * NF) {
-          if (i < NF) read_one(rkt, rxb, rwb, rkk, buf ^ 1, i);
-          if (i >= NM - T::NI) convert_one(buf ^ 1, i - (NM - T::NI));
-        } else {
-#pragma unroll
-          for (int j = i * NF / NM; j < (i + 1) * NF / NM; ++j) read_one(rkt, rxb, rwb, rkk, buf ^ 1, j);
-          if (i == NM - 1) {
-#pragma unroll
-            for (int j = 0; j < T::NI; ++j) convert_one(buf ^ 1, j);
-          }
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
   auto none = [](int) {};
 
-  // ---- prologue: the first tile, then the others
-  if constexpr (T::WS) fetch_scales(0);
+  // ---- prologue: the first tile, then the others (live: row blocks of a wave)
+  auto prologue = [&](auto LIVEC) __attribute__((always_inline)) {
+    constexpr int live = decltype(LIVEC)::value, xi = live * T::WM * 4 / T::NW, NA = T::na(live);
+    if constexpr (T::WS) fetch_scales(0);
 #pragma unroll
-  for (int i = 0; i < WL; ++i) load_w(0, 0, i);
+    for (int i = 0; i < WL; ++i) load_w(0, 0, i);
 #pragma unroll
-  for (int s = 0; s < T::NA; ++s) {
+    for (int s = 0; s < NA; ++s) {
 #pragma unroll
-    for (int i = 0; i < T::XI; ++i) load_x(s, s, i);
-    if (T::SUB == 1 && s + 1 < T::NA) {
+      for (int i = 0; i < xi; ++i) load_x(s, s, i, live);
+      if (T::SUB == 1 && s + 1 < NA) {
 #pragma unroll
-      for (int i = 0; i < WL; ++i) load_w(s + 1, s + 1, i);
+        for (int i = 0; i < WL; ++i) load_w(s + 1, s + 1, i);
+      }
     }
-  }
-  constexpr int V0 = T::SUB == 4 ? (T::NA - 1) * T::XI + (T::NB - 1) * WL : (T::NA - 1) * (T::XI + WL);
-  if constexpr (T::SUB == 4) {
+    constexpr int V0 = T::SUB == 4 ? (NA - 1) * xi + (T::NB - 1) * WL : (NA - 1) * (xi + WL);
+    if constexpr (T::SUB == 4) {
 #pragma unroll
-    for (int s = 1; s < T::NB; ++s)
+      for (int s = 1; s < T::NB; ++s)
 #pragma unroll
-      for (int i = 0; i < WL; ++i) load_w(s, s, i);
-  }
-  pass_scales(0);
-  __builtin_amdgcn_s_waitcnt(((V0 < 63 ? V0 : 63) & 15) | (((V0 < 63 ? V0 : 63) >> 4) << 14) | 0x0070);  // vmcnt, lgkmcnt(0)
-  __builtin_amdgcn_s_barrier();
+        for (int i = 0; i < WL; ++i) load_w(s, s, i);
+    }
+    pass_scales(0);
+    __builtin_amdgcn_s_waitcnt(((V0 < 63 ? V0 : 63) & 15) | (((V0 < 63 ? V0 : 63) >> 4) << 14) | 0x0070);  // vmcnt, lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+  };
   int kt = 0, xb = 0, wb = 0;  // k tile and its buffers
   int xb1 = 0, wb1 = 0;        // the next one's
   bool wnext = false;          // whether its weights are another tile
-  auto next_buffers = [&](int kt) {
-    xb1 = xb == T::NA - 1 ? 0 : xb + 1;
+  auto next_buffers = [&](int kt, int na) {
+    xb1 = xb == na - 1 ? 0 : xb + 1;
     wnext = T::SUB == 1 || (kt & 3) == 3;
     wb1 = !wnext ? wb : (wb == T::NB - 1 ? 0 : wb + 1);
   };
   // this wave's reads of tile kt are in its registers and its share of tile kt + 1 has landed; everybody's, behind the barrier
-  auto landed = [&](int kt) {
+  auto landed = [&](int kt, auto LIVEC) {
+    constexpr int live = decltype(LIVEC)::value, xi = live * T::WM * 4 / T::NW, NA = T::na(live);
     if (wnext) pass_scales((T::SUB == 4 ? kt >> 2 : kt) + 1);
-    constexpr int V = T::INFLIGHT, V2 = T::SUB == 4 ? V + WL : V;
-    if (T::SUB == 4 && (kt & 3) <= T::NA - 2) {  // (weights requested after the rows of tile kt + 1 may be on their way, too)
+    constexpr int V = T::inflight(NA, xi), V2 = T::SUB == 4 ? V + WL : V;
+    if (T::SUB == 4 && (kt & 3) <= NA - 2) {  // (weights requested after the rows of tile kt + 1 may be on their way, too)
       __builtin_amdgcn_s_waitcnt((V2 & 15) | ((V2 >> 4) << 14) | 0x0070);  // vmcnt, lgkmcnt(0)
     } else {
       __builtin_amdgcn_s_waitcnt((V & 15) | ((V >> 4) << 14) | 0x0070);
@@ -346,7 +334,10 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
   const bool half = MUL != kMul44 && (k1 - k0) % 64 != 0;  // the last tile's second half lies behind K
+  typedef std::integral_constant<int, T::MI> AllRows;
   if constexpr (T::DEEP) {
+    constexpr int NM = T::NI * T::MI, NF = T::NI + T::MI;
+    prologue(AllRows{});
     // Waves of few MFMAs per step read the fragments of all four steps of the next k tile while they multiply this one's: step by
     // step each waits for an LDS read, its conversion and two or four MFMAs in a row, with nothing beside them (32 x 256 tiles,
     // 4-bit weights: 2500 clocks a k tile of 32 MFMAs).
@@ -357,23 +348,23 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
         for (int ni = 0; ni < T::NI; ++ni) convert_one(set + kk, ni);
       }
-      mfma_one(set + kk, kk, j);
+      mfma_one(set + kk, kk, j, T::MI);
     };
     auto tile = [&](auto SET) __attribute__((always_inline)) {
       constexpr int set = decltype(SET)::value;
-      next_buffers(kt);
-      landed(kt);
+      next_buffers(kt, T::NA);
+      landed(kt, AllRows{});
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         multiply(set, i);
         constexpr int NL = T::XI + WL;
 #pragma unroll
         for (int j = i * NL / NS; j < (i + 1) * NL / NS; ++j) {
-          if (j < T::XI) load_x(kt + T::NA, xb, j);
+          if (j < T::XI) load_x(kt + T::NA, xb, j, T::MI);
           else if (wnext) load_w((T::SUB == 4 ? kt >> 2 : kt) + T::NB, wb, j - T::XI);
         }
 #pragma unroll
-        for (int j = i * NR / NS; j < (i + 1) * NR / NS; ++j) read_one(kt + 1, xb1, wb1, j / NF, (4 - set) + j / NF, j % NF);
+        for (int j = i * NR / NS; j < (i + 1) * NR / NS; ++j) read_one(kt + 1, xb1, wb1, j / NF, (4 - set) + j / NF, j % NF, T::MI);
         __builtin_amdgcn_sched_barrier(0);
       }
       xb = xb1;
@@ -389,7 +380,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
     typedef std::integral_constant<int, 0> Set0;
     typedef std::integral_constant<int, 4> Set1;
 #pragma unroll
-    for (int j = 0; j < NR; ++j) read_one(0, 0, 0, j / NF, j / NF, j % NF);
+    for (int j = 0; j < NR; ++j) read_one(0, 0, 0, j / NF, j / NF, j % NF, T::MI);
     while (kt + 2 < KT) {
       tile(Set0{});
       tile(Set1{});
@@ -401,40 +392,76 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
       last(Set0{});
     }
   } else {
+    // LIVE: blocks of 32 rows that a wave has; the row blocks of a tile go to its waves in turn, so that a tile of fewer rows costs
+    // less whole steps' MFMAs, loads and fragments - not time alone, the large products run at the power limit.
+    auto run = [&](auto LIVEC) __attribute__((always_inline)) {
+      constexpr int LIVE = decltype(LIVEC)::value, NM = T::NI * LIVE, NF = T::NI + LIVE, XL = LIVE * T::WM * 4 / T::NW, NA = T::na(LIVE);
+      typedef std::integral_constant<int, LIVE> Rows;
+      // step kk, slot by slot (a schedule fence after each): MFMA i, its share of `n` loads, and of the fragments of
+      // step rkk of tile rkt into the other set (rkk < 0: none)
+      auto step = [&](int kk, int n, auto load, int rkt, int rxb, int rwb, int rkk) __attribute__((always_inline)) {
+        const int buf = kk & 1;
 #pragma unroll
-    for (int i = 0; i < NF; ++i) read_one(0, 0, 0, 0, 0, i);
+        for (int i = 0; i < NM; ++i) {
+          mfma_one(buf, kk, i, LIVE);
 #pragma unroll
-    for (int i = 0; i < T::NI; ++i) convert_one(0, i);
-    turn_scales();
-
-    for (; kt < KT - 1; ++kt) {
-      next_buffers(kt);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (T::LATE) {
-        const int wb2 = wb == 0 ? T::NB - 1 : wb - 1;  // tile kt - 1 has left it
-        step(0, WL, [&](int j) { load_w(kt + 2, wb2, j); }, kt, xb, wb, 1);
-      } else {
-        step(0, 0, none, kt, xb, wb, 1);
-      }
-      step(1, 0, none, kt, xb, wb, 2);
-      step(2, 0, none, kt, xb, wb, 3);
-      landed(kt);
-      // rows of tile kt + NA, and weights where a tile of them is over
-      step(3, T::LATE ? T::XI : T::XI + WL, [&](int j) {
-        if (j < T::XI) load_x(kt + T::NA, xb, j);
-        else if (wnext) load_w((T::SUB == 4 ? kt >> 2 : kt) + T::NB, wb, j - T::XI);
-      }, kt + 1, xb1, wb1, 0);
-      xb = xb1;
-      wb = wb1;
+          for (int j = i * n / NM; j < (i + 1) * n / NM; ++j) load(j);
+          if (rkk >= 0) {
+            // (reads in the first half of the step, so that none is waited for; conversions in the last slots)
+            constexpr int RPS = (2 * NF + NM - 1) / NM;
+#pragma unroll
+            for (int j = i * RPS; j < (i + 1) * RPS && j < NF; ++j) read_one(rkt, rxb, rwb, rkk, buf ^ 1, j, LIVE);
+            constexpr int C0 = NM * 5 / 8, CS = NM - C0;
+            if (i >= C0) {
+#pragma unroll
+              for (int j = (i - C0) * T::NI / CS; j < (i - C0 + 1) * T::NI / CS; ++j) convert_one(buf ^ 1, j);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      prologue(Rows{});
+#pragma unroll
+      for (int i = 0; i < NF; ++i) read_one(0, 0, 0, 0, 0, i, LIVE);
+#pragma unroll
+      for (int i = 0; i < T::NI; ++i) convert_one(0, i);
       turn_scales();
-    }
-    // the last tile, whole or half
-    step(0, 0, none, kt, xb, wb, 1);
-    if (!half) {
-      step(1, 0, none, kt, xb, wb, 2);
-      step(2, 0, none, kt, xb, wb, 3);
-    }
-    step(3, 0, none, kt, xb, wb, -1);
+
+      for (; kt < KT - 1; ++kt) {
+        next_buffers(kt, NA);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (T::LATE) {
+          const int wb2 = wb == 0 ? T::NB - 1 : wb - 1;  // tile kt - 1 has left it
+          step(0, WL, [&](int j) { load_w(kt + 2, wb2, j); }, kt, xb, wb, 1);
+        } else {
+          step(0, 0, none, kt, xb, wb, 1);
+        }
+        step(1, 0, none, kt, xb, wb, 2);
+        step(2, 0, none, kt, xb, wb, 3);
+        landed(kt, Rows{});
+        // rows of tile kt + NA, and weights where a tile of them is over
+        step(3, T::LATE ? XL : XL + WL, [&](int j) {
+          if (j < XL) load_x(kt + NA, xb, j, LIVE);
+          else if (wnext) load_w((T::SUB == 4 ? kt >> 2 : kt) + T::NB, wb, j - XL);
+        }, kt + 1, xb1, wb1, 0);
+        xb = xb1;
+        wb = wb1;
+        turn_scales();
+      }
+      // the last tile, whole or half
+      step(0, 0, none, kt, xb, wb, 1);
+      if (!half) {
+        step(1, 0, none, kt, xb, wb, 2);
+        step(2, 0, none, kt, xb, wb, 3);
+      }
+      step(3, 0, none, kt, xb, wb, -1);
+    };
+    static_assert(T::MI == 2 || T::MI == 4, "row blocks of a wave");
+    const int live = MUL == kMul44 ? T::MI : (rows + 32 * T::WM - 1) / (32 * T::WM);  // (kMul44: there is one such tile a column at most)
+    if (MUL == kMul44 || live == T::MI) run(std::integral_constant<int, T::MI>{});
+    else if (live == 1) run(std::integral_constant<int, 1>{});
+    else if (live == 2) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, T::MI == 4 ? 3 : 1>{});
   }
   TRI_WAIT_VMCNT(0);
   __syncthreads();  // every wave is done with the tiles in LDS, and every load into them has landed
@@ -443,7 +470,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
   // wave's own region) and leave as 16-byte pieces of rows.
   if constexpr (KIND == kGroupDown || KIND == kGroupParts) {
     constexpr int RS = T::TN + 4;  // floats per staged row
-    static_assert(4 * 32 * RS * 4 <= T::LDS_BYTES, "the staged rows fit");
+    static_assert(T::NW * 32 * RS * 4 <= T::LDS_BYTES, "the staged rows fit");
     float* const stg = reinterpret_cast<float*>(lds) + wave * 32 * RS;
 #pragma unroll
     for (int mi = 0; mi < T::MI; ++mi) {
@@ -458,7 +485,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
 #pragma unroll 4
       for (int idx = lane; idx < 32 * LPR; idx += 64) {
         const int row = idx / LPR, ch = idx % LPR;
-        const int r = wm * T::TM + mi * 32 + row, n = n0 + wn * T::TN + ch * 4;
+        const int r = (mi * T::WM + wm) * 32 + row, n = n0 + wn * T::TN + ch * 4;
         const float4v v = *reinterpret_cast<const float4v*>(stg + row * RS + ch * 4);
         if (r < rows && n < a.N) {
           const int64_t at = KIND == kGroupDown ? (int64_t)split * a.n + a.rows[place0 + r] : (int64_t)split * a.M + place0 + r;
@@ -469,7 +496,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
   } else {
     constexpr int ONI = GATE ? T::NI / 2 : T::NI;
     constexpr int RS = OUT_TN + 8;  // halfs per staged row
-    static_assert(4 * T::TM * RS * 2 <= T::LDS_BYTES, "the staged output tile fits");
+    static_assert(T::NW * T::TM * RS * 2 <= T::LDS_BYTES, "the staged output tile fits");
     half_t* const stg = lds_h + wave * (T::TM * RS);
   #pragma unroll
     for (int mi = 0; mi < T::MI; ++mi)
@@ -489,7 +516,7 @@ __global__ __launch_bounds__(256) void group_tile_kernel(GroupArgs a) {
   #pragma unroll 4
     for (int idx = lane; idx < T::TM * LPR; idx += 64) {
       const int row = idx / LPR, ch = idx % LPR;
-      const int r = wm * T::TM + row, n = n0 + wn * OUT_TN + ch * 8;
+      const int r = (row / 32 * T::WM + wm) * 32 + row % 32, n = n0 + wn * OUT_TN + ch * 8;
       const half8v v = *reinterpret_cast<const half8v*>(stg + row * RS + ch * 8);
       if (r < rows && n < a.N) *reinterpret_cast<half8v*>(a.out + (int64_t)(place0 + r) * a.ldo + n) = v;
     }
@@ -505,7 +532,7 @@ int launch_tile_t(const GroupArgs& a, hipStream_t stream) {
   // (experts: as many tiles as there can be)
   const int64_t tiles_m = ALL ? (a.M + T::BM - 1) / T::BM : (a.n + T::BM - 1) / T::BM + (a.E < a.n ? a.E : a.n);
   const int64_t tiles = tiles_m * ((a.N + OUT_BN - 1) / OUT_BN) * a.ksplit;
-  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), T::LDS_BYTES, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(T::NT), T::LDS_BYTES, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

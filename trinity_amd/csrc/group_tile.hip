@@ -3,31 +3,36 @@
 
 namespace tri {
 
-#ifndef STREAMMEAN
-#define STREAMMEAN 10
-#endif
-// parts of K for `tiles` tiles: so many that every CU has one, of at least 512 values
-static int parts_of(int tiles, int K) {
+// Workgroups that a CU holds side by side (by their LDS): two of the small tiles, and they hide each other's waits; one of 256 x 256.
+static int tile_slots(int bm) { return bm == 256 ? 256 : 512; }
+static int tile_cols(int bm) { return bm == 32 || bm == 256 ? 256 : 128; }
+
+// parts of K for `tiles` tiles: so many that all slots are taken, of at least 512 values
+static int parts_of(int tiles, int K, int slots) {
   const int deep = (K + 255) / 256;
-  int parts = tiles >= 256 ? 1 : 256 / tiles;
+  int parts = tiles >= slots ? 1 : slots / tiles;
   if (parts > deep / 2) parts = deep / 2 > 0 ? deep / 2 : 1;
   const int per = (deep + parts - 1) / parts;
   return (deep + per - 1) / per;  // (no part is empty)
 }
 
+// Rows of a tile by the mean rows of an expert.  us of both products of 8 experts of [4096, 14336], by 32, 64, 128, 256 rows:
+//   16-bit weights, 32 rows each 555, 501, 574, 499; 42 of 32 experts of [4544, 2272] -, 401, -, 435; 64 818, 669, 588, 507; 150 1395,
+//     1116, 740, 591; 500 3800, 2710, 1990, 1540
+//   4-bit weights, 32 rows 228, 281, 371, 312; 64 373, 387, 384, 361; 100 479, 459, 404, 383; 150 681, 705, 611, 499; 250 1067, 1010,
+//     859, 935; 500 2043, 1963, 1511, 1615
 GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w4) {
   GroupPlan p;
-  const int mean = (choices + experts - 1) / experts;
+  const int mean = (choices + experts - 1) / experts, groups = choices < experts ? choices : experts;
   const int rows = choices / top_k < 16 ? choices / top_k : 16;  // (of an expert, at most, if a token chooses it once)
-  if (w4 && mean <= STREAMMEAN && group_stream_takes(rows, N, false) && group_stream_takes(rows, F, true)) {
+  if (w4 && mean <= 10 && group_stream_takes(rows, N, false) && group_stream_takes(rows, F, true)) {
     p.bm = 16;
-    p.ksplit = group_stream_parts(rows, F, N, choices < experts ? choices : experts);
+    p.ksplit = group_stream_parts(rows, F, N, groups);
     return p;
   }
-  p.bm = mean <= 24 ? 32 : (mean <= 64 ? 64 : (mean <= 256 ? 128 : 256));
-  const int bn = p.bm == 32 || p.bm == 256 ? 256 : 128;
-  const int groups = choices < experts ? choices : experts;
-  p.ksplit = parts_of(((mean + p.bm - 1) / p.bm) * groups * ((N + bn - 1) / bn), F);
+  p.bm = w4 ? (mean <= 48 ? 32 : (mean <= 180 ? 256 : 128)) : (mean <= 48 ? 64 : 256);
+  const int tiles = ((mean + p.bm - 1) / p.bm) * groups * ((N + tile_cols(p.bm) - 1) / tile_cols(p.bm));
+  p.ksplit = parts_of(tiles, F, tile_slots(p.bm));
   return p;
 }
 
@@ -36,12 +41,38 @@ int experts_parts(int choices, int top_k, int experts, int N, int F) {
   return a > b ? a : b;
 }
 
+// The cheapest tile and number of parts, by what a round of workgroups takes for a k tile (us; measured over [4544, 18176] and
+// [14336, 4096] at 24 to 4096 rows): with every slot taken, and with one workgroup a CU at most; 3 us to begin and end a round; the parts'
+// sums cost their trip to memory and the launch that joins them.
 GroupPlan group_rows_plan(int M, int K, int N, bool x4) {
-  GroupPlan p;
-  p.bm = M <= 32 ? 32 : (M <= 64 ? 64 : (M <= 256 ? 128 : 256));
-  const int bn = p.bm == 32 || p.bm == 256 ? 256 : 128;
-  p.ksplit = parts_of(((M + p.bm - 1) / p.bm) * ((N + bn - 1) / bn), K);
-  return p;
+  struct Cost {
+    int bm;
+    float full, half;
+  };
+  static const Cost k164[4] = {{32, 0.68f, 0.33f}, {64, 0.64f, 0.46f}, {128, 0.90f, 0.57f}, {256, 1.40f, 1.40f}};
+  static const Cost k44[4] = {{32, 2.4f, 1.3f}, {64, 1.7f, 1.05f}, {128, 1.85f, 1.3f}, {256, 2.6f, 2.6f}};
+  GroupPlan best = {256, 1};
+  float least = 1e30f;
+  const int deep = (K + 255) / 256;
+  for (const Cost& c : x4 ? k44 : k164) {
+    const int row_tiles = (M - 1) / c.bm + 1, col_tiles = (N - 1) / tile_cols(c.bm) + 1, slots = tile_slots(c.bm);
+    const int64_t tiles = (int64_t)row_tiles * col_tiles;
+    const int most = parts_of(tiles < slots ? (int)tiles : slots, K, slots);
+    // (a 256-row tile of fewer rows, the only one in a column, costs less)
+    const float share = c.bm == 256 && row_tiles == 1 && !x4 ? 0.22f + 0.08f * (float)((M + 63) / 64) : 1.0f;
+    for (int want = 1; want <= most; ++want) {
+      const int per = (deep + want - 1) / want, parts = (deep + per - 1) / per;  // (no part is empty)
+      const int64_t units = tiles * parts, rounds = (units - 1) / slots, last = (units - 1) % slots + 1;
+      const float round = (float)rounds * c.full + (last > 256 || slots == 256 ? c.full : c.half);
+      float us = round * share * (float)per * (x4 ? 1.0f : 4.0f) + 3.0f * (float)(rounds + 1);
+      if (parts > 1) us += 4.0f + (float)parts * (float)M * (float)N * 2.5e-6f;
+      if (us < least) {
+        least = us;
+        best = {c.bm, parts};
+      }
+    }
+  }
+  return best;
 }
 
 int64_t fp4_matmul_workspace(int M, int K, int N, bool x4) {
@@ -51,7 +82,7 @@ int64_t fp4_matmul_workspace(int M, int K, int N, bool x4) {
 
 template <GroupMul MUL, GroupKind KIND>
 static int launch_tile_kind(const GroupArgs& a, int, hipStream_t stream) {
-  return launch_tile_t<GroupTile<256, 256, 2, 2, 2, MUL == kMul16 ? 3 : 2, MUL>, KIND>(a, stream);
+  return launch_tile_t<GroupTile<256, 256, 2, MUL == kMul164 ? 4 : 2, 2, MUL == kMul16 ? 3 : 2, MUL>, KIND>(a, stream);
 }
 
 int launch_group_tile(const GroupArgs& a, GroupKind kind, int bm, hipStream_t stream) {

@@ -6,14 +6,14 @@ namespace tri {
 
 template <GroupMul MUL, GroupKind KIND>
 static int launch_tile_kind(const GroupArgs& a, int bm, hipStream_t stream) {
-#ifndef NB164
-#define NB164 2
-#endif
-  constexpr int D = MUL == kMul164 ? NB164 : 3;
+  // (k tiles in LDS: as many as leave room for two workgroups a CU)
+  constexpr int D = MUL == kMul164 ? 2 : 3;
   switch (bm) {
-    case 32: return launch_tile_t<GroupTile<32, 256, 1, 4, 3, D, MUL>, KIND>(a, stream);
+    case 32:
+      if constexpr (MUL == kMul16) return -1;  // (experts_plan has none)
+      else return launch_tile_t<GroupTile<32, 256, 1, 4, 3, D, MUL>, KIND>(a, stream);
     case 64: return launch_tile_t<GroupTile<64, 128, 2, 2, 3, D, MUL>, KIND>(a, stream);
-    default: return launch_tile_t<GroupTile<128, 128, 2, 2, 3, D, MUL>, KIND>(a, stream);
+    default: return launch_tile_t<GroupTile<128, 128, 2, 2, 2, 2, MUL>, KIND>(a, stream);
   }
 }
 

@@ -189,10 +189,20 @@ __global__ __launch_bounds__(kSortThreads) void expert_rows_kernel(ExpertRowsArg
   const int rounds = (a.n + kSortThreads - 1) / kSortThreads;  // of 64 choices per wave
   const int s0 = wave * rounds * 64 + lane;
   int* const mine = base + wave * a.E;
-  for (int r = 0; r < rounds; ++r) {
-    const int s = s0 + r * 64;
-    const int e = s < a.n ? a.ids[s] : -1;
-    if (e >= 0 && e < a.E) atomicAdd(&mine[e], 1);
+  constexpr int B = 8;  // rounds whose choices are on their way at a time
+  auto fetch = [&](int r, int (&e)[B]) {
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int s = s0 + (r + u) * 64;
+      e[u] = r + u < rounds && s < a.n ? a.ids[s] : -1;
+    }
+  };
+  int kept[B];
+  for (int r = 0; r < rounds; r += B) {
+    fetch(r, kept);
+#pragma unroll
+    for (int u = 0; u < B; ++u)
+      if (kept[u] >= 0 && kept[u] < a.E) atomicAdd(&mine[kept[u]], 1);
   }
   __syncthreads();
   for (int e = t; e < a.E; e += kSortThreads) {
@@ -229,21 +239,24 @@ __global__ __launch_bounds__(kSortThreads) void expert_rows_kernel(ExpertRowsArg
     if (lane == 0) a.tiles[0] = make_int4(tiles0, rows0, 0, 0);
   }
   __syncthreads();
-  for (int r = 0; r < rounds; ++r) {
-    const int s = s0 + r * 64;
-    const int e = s < a.n ? a.ids[s] : -1;
-    const bool real = e >= 0 && e < a.E;
-    uint64_t same = __ballot(real);  // lanes of this one's expert
-    for (int b = 0; (1 << b) < a.E; ++b) {
-      const uint64_t bit = __ballot((e >> b) & 1);
-      same &= ((e >> b) & 1) ? bit : ~bit;
+  for (int r0 = 0; r0 < rounds; r0 += B) {
+    if (rounds > B) fetch(r0, kept);
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int s = s0 + (r0 + u) * 64, e = kept[u];
+      const bool real = e >= 0 && e < a.E;
+      uint64_t same = __ballot(real);  // lanes of this one's expert
+      for (int b = 0; (1 << b) < a.E; ++b) {
+        const uint64_t bit = __ballot((e >> b) & 1);
+        same &= ((e >> b) & 1) ? bit : ~bit;
+      }
+      if (real) {
+        const int rank = __popcll(same & ((1ull << lane) - 1)), at = mine[e];
+        a.rows[start[e] + at + rank] = s;
+        if (rank == 0) mine[e] = at + __popcll(same);  // (a wave's reads of LDS come before its later writes)
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    if (real) {
-      const int rank = __popcll(same & ((1ull << lane) - 1)), at = mine[e];
-      a.rows[start[e] + at + rank] = s;
-      if (rank == 0) mine[e] = at + __popcll(same);  // (a wave's reads of LDS come before its later writes)
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -254,22 +267,35 @@ int launch_expert_rows(const ExpertRowsArgs& a, hipStream_t stream) {
 
 // out[t] = sum of w[t, i] * y[t * k + i] over the choices i that are experts, in 32 bits, y being the sum of its parts; or
 // (no weights, k = 1) that sum itself.
+// Bound by the bytes of y.  Rows of four choices (or parts) are on their way at a time.
+template <bool PARTS>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinRowsArgs a) {
   const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
   if (c >= a.N) return;
   for (int64_t t = blockIdx.y; t < a.T; t += gridDim.y) {
     float4v s = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.k; ++i) {
-      const int64_t row = t * a.k + i;
-      float w = 1.0f;
-      if (a.weights != nullptr) {
-        const int e = a.ids[row];
-        if (e < 0 || e >= a.E) continue;
-        w = a.weights[row];
-      }
-      const float4v v = sum_splits(a.y, a.parts, a.T * a.k * a.N, row * a.N + c);
+    for (int i0 = 0; i0 < a.k; i0 += 4) {
+      float4v v[4];
+      float w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = fmaf(w, v[j], s[j]);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t row = t * a.k + min(i0 + u, a.k - 1);
+        w[u] = 1.0f;
+        bool real = i0 + u < a.k;
+        if (a.weights != nullptr) {
+          const int e = a.ids[row];
+          real = real && e >= 0 && e < a.E;
+          w[u] = a.weights[row];
+        }
+        v[u] = float4v{0.f, 0.f, 0.f, 0.f};
+        if (!real) w[u] = 0.0f;  // (rows without an expert are not there: their memory may hold anything)
+        else if (PARTS) v[u] = sum_splits(a.y, a.parts, a.T * a.k * a.N, row * a.N + c);
+        else v[u] = *reinterpret_cast<const float4v*>(a.y + row * a.N + c);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = fmaf(w[u], v[u][j], s[j]);
     }
     const half4v h = {(half_t)s[0], (half_t)s[1], (half_t)s[2], (half_t)s[3]};
     *reinterpret_cast<half4v*>(a.out + t * a.ldo + c) = h;
@@ -278,7 +304,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinRowsArgs a) {
 
 int launch_join_rows(const JoinRowsArgs& a, hipStream_t stream) {
   const dim3 grid((a.N / 4 + 255) / 256, (unsigned)(a.T < 65535 ? a.T : 65535));
-  hipLaunchKernelGGL(join_rows_kernel, grid, dim3(256), 0, stream, a);
+  if (a.parts > 1) hipLaunchKernelGGL((join_rows_kernel<true>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((join_rows_kernel<false>), grid, dim3(256), 0, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
