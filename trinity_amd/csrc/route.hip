@@ -16,24 +16,66 @@ namespace tri {
 
 constexpr int kRouteThreads = 256;
 
-// a double's bits in an order that unsigned integers have; NaN (of either sign) below everything
+// a double's bits in an order that unsigned integers have; NaN (of either sign) below all numbers; none is 0
 __device__ __forceinline__ uint64_t order_key(double x) {
   const uint64_t b = (uint64_t)__double_as_longlong(x);
-  if (x != x) return 0;
+  if (x != x) return 1;
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 
-template <int LPT>
-__device__ __forceinline__ double lanes_sum(double x) {
-#pragma unroll
-  for (int o = LPT / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// Both halves of an exchange between lanes `O` apart, for a reduction that takes O = 1, 2, 4, ... in turn: within 16 lanes through
+// the data path of an instruction's operand (a mirror serves for 4 and 8, smaller groups being alike by then), beyond by swaps of
+// whole rows of lanes.  (An exchange through LDS takes about ten times as long, and every choice waits for six.)
+template <int O>
+__device__ __forceinline__ void exchange(uint32_t x, uint32_t& p, uint32_t& q) {
+  if constexpr (O <= 8) {
+    constexpr int kHow = O == 1 ? 0xB1 : (O == 2 ? 0x4E : (O == 4 ? 0x141 : 0x140));
+    p = x;
+    q = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kHow, 0xF, 0xF, true);
+  } else {
+    const uint2v r = O == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false) : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    p = r[0];
+    q = r[1];
+  }
 }
-template <int LPT>
+template <int O>
+__device__ __forceinline__ void exchange(double x, double& p, double& q) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  uint32_t pl, ql, ph, qh;
+  exchange<O>((uint32_t)b, pl, ql);
+  exchange<O>((uint32_t)(b >> 32), ph, qh);
+  p = __builtin_bit_cast(double, (uint64_t)ph << 32 | pl);
+  q = __builtin_bit_cast(double, (uint64_t)qh << 32 | ql);
+}
+template <int LPT, int O = 1>
+__device__ __forceinline__ double lanes_sum(double x) {
+  if constexpr (O < LPT) {
+    double p, q;
+    exchange<O>(x, p, q);
+    return lanes_sum<LPT, O * 2>(p + q);
+  } else {
+    return x;
+  }
+}
+template <int LPT, int O = 1>
 __device__ __forceinline__ double lanes_max(double x) {
-#pragma unroll
-  for (int o = LPT / 2; o > 0; o >>= 1) x = fmax(x, __shfl_xor(x, o));
-  return x;
+  if constexpr (O < LPT) {
+    double p, q;
+    exchange<O>(x, p, q);
+    return lanes_max<LPT, O * 2>(fmax(p, q));
+  } else {
+    return x;
+  }
+}
+template <int LPT, int O = 1>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+  if constexpr (O < LPT) {
+    uint32_t p, q;
+    exchange<O>(x, p, q);
+    return lanes_max<LPT, O * 2>(p > q ? p : q);
+  } else {
+    return x;
+  }
 }
 
 template <typename T>
@@ -114,34 +156,38 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a) {
   }
   uint64_t key[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) key[j] = order_key(c[j]);
+  for (int j = 0; j < EPL; ++j) key[j] = in[j] ? order_key(c[j]) : 0;
   double sum = 0.0, my_w = 0.0;
   int my_id = 0;
+  constexpr uint64_t kMine = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
+  const int first = (int)(threadIdx.x & 63) - lane;  // (of this token's lanes in the wave)
   for (int r = 0; r < a.k; ++r) {
     // this lane's best: largest key, lowest index
-    uint64_t bk = 0;
-    int be = 1 << 30;
-    double bs = 0.0;
+    uint64_t bk = key[0];
+    int bj = 0;
+    double bs = s[0];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (in[j] && (be == (1 << 30) || key[j] > bk)) {
-        bk = key[j];
-        be = lane * EPL + j;
-        bs = s[j];
-      }
+    for (int j = 1; j < EPL; ++j) {
+      const bool take = key[j] > bk;
+      bk = take ? key[j] : bk;
+      bj = take ? j : bj;
+      bs = take ? s[j] : bs;
     }
-#pragma unroll
-    for (int o = LPT / 2; o > 0; o >>= 1) {
-      const uint64_t ok = __shfl_xor(bk, o);
-      const int oe = __shfl_xor(be, o);
-      const double os = __shfl_xor(bs, o);
-      const bool take = oe != (1 << 30) && (be == (1 << 30) || ok > bk || (ok == bk && oe < be));
-      bk = take ? ok : bk;
-      be = take ? oe : be;
-      bs = take ? os : bs;
+    // of all lanes: by the upper 32 bits, and by the lower ones where those are not enough; then the first such lane
+    const uint32_t hi = (uint32_t)(bk >> 32), lo = (uint32_t)bk;
+    const bool near = hi == lanes_max<LPT>(hi);
+    uint64_t who = (__ballot(near) >> first) & kMine;
+    if (__ballot((who & (who - 1)) != 0) != 0) {  // (of any token of the wave)
+      const uint32_t best = lanes_max<LPT>(near ? lo : 0u);
+      who = (__ballot(near && lo == best) >> first) & kMine;
     }
+    const int owner = __builtin_ctzll(who);
+    const int be = __shfl(lane * EPL + bj, first + owner);
+    bs = __shfl(bs, first + owner);
+    if (lane == owner) {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) in[j] = in[j] && be != lane * EPL + j;
+      for (int j = 0; j < EPL; ++j) key[j] = j == bj ? 0 : key[j];
+    }
     sum += bs;
     my_id = r == lane ? be : my_id;
     my_w = r == lane ? bs : my_w;
