@@ -1,6 +1,6 @@
 """Products over 4-bit weights, routing to experts and the experts' FFN, in fp64 (the reference has no counterpart: these
 functions are the definition).  tests/test_experts_oracle.py pins them: products against decoded matrices entry by entry,
-routing against a search over all subsets of experts, the FFN against the dense one of oracle/blocks.py.  4-bit matrices are
+routing against a search over all subsets of experts, the FFN against a dense one per token.  4-bit matrices are
 those of oracle/cache.py."""
 import math
 

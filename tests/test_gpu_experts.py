@@ -94,6 +94,11 @@ EXPERTS = [
     (13, 70, 6, 32, 64, "spread"), (50, 512, 2, 64, 32, "spread"), (100, 4, 2, 224, 416, "spread"), (130, 4, 2, 128, 96, "one"),
     (300, 5, 3, 160, 256, "spread"), (301, 9, 4, 96, 544, "few"), (520, 2, 2, 288, 160, "spread"), (600, 3, 2, 544, 352, "few"),
     (700, 2, 1, 96, 1056, "one"), (257, 1, 1, 64, 32, "spread"), (64, 3, 1, 64, 96, "twice"), (530, 2, 3, 32, 64, "twice"),
+    # choices one by one, rows of one, four and sixteen; rows put in order (more than 64 choices)
+    (1, 6, 2, 544, 1056, "spread"), (1, 9, 3, 1056, 512, "twice"), (4, 8, 3, 512, 544, "few"), (16, 8, 4, 1056, 512, "spread"),
+    (13, 70, 6, 544, 512, "spread"), (5, 20, 16, 512, 544, "twice"), (40, 8, 2, 544, 800, "spread"), (15, 90, 40, 512, 576, "few"),
+    # parts of K; two row blocks of four
+    (50, 3, 2, 64, 1056, "spread"), (50, 2, 2, 96, 1088, "one"), (200, 2, 2, 64, 1056, "few"), (110, 2, 2, 96, 160, "one"),
 ]
 
 
@@ -199,6 +204,35 @@ def test_captured_and_replayed(dev, T, w4):
         torch.cuda.synchronize()
         for graph in graphs:
             assert torch.equal(graph.res[0], ids) and torch.equal(graph.res[1], out)
+
+
+@pytest.mark.parametrize("w4", [False, True])
+def test_two_streams_at_once(dev, w4):
+    """Calls of one object on two streams, behind one another on the host and side by side on the GPU."""
+    g = torch.Generator().manual_seed(8)
+    E, k, N, F = 8, 2, 544, 1056
+    stored, _ = _weights(g, E, F, N, BF16, w4, 0)
+    d = [(to_dev(a, dev), to_dev(b, dev)) for a, b in stored]
+    op, router, calls = blocks.ExpertsFfn(), blocks.Router(k), []
+    for T in (1, 30, 200, 700):
+        x, z = torch.randn(T, N, generator=g).bfloat16().to(dev), torch.randn(T, E, generator=g).to(dev)
+        calls.append((x, z))
+
+    def step(x, z):
+        return op.run(x, *router.route(z), d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
+
+    want = [step(*c) for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for i, c in enumerate(calls):
+            for s in (streams[i % 2], streams[1 - i % 2]):
+                with torch.cuda.stream(s):
+                    got.append((i, step(*c)))
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i])
 
 
 def test_results_do_not_depend_on_timing(dev):

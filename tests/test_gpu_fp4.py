@@ -94,6 +94,29 @@ def test_product(dev, M, K, N, pad, shift, dtype, x4):
     assert bool((big[:, :8] == 3).all()) and bool((big[:, N + 8:] == 3).all())
 
 
+# M, K, N, x in 4 bits: a product for each tile, number of row blocks in it, and whole K or parts (test_experts_plans.py)
+FORMS = [
+    (200, 96, 8200, True), (20, 8224, 4104, True), (20, 96, 136, True), (33, 2080, 136, True), (1000, 96, 2056, True),
+    (70, 4128, 4104, True), (1000, 96, 8200, True), (333, 14336, 8192, True),
+    (20, 96, 136, False), (20, 2080, 136, False), (400, 96, 8200, False), (257, 8224, 4104, False), (1000, 96, 2056, False),
+    (2500, 4128, 264, False), (1300, 96, 8200, False), (40, 4128, 8200, False), (70, 8224, 8200, False), (130, 8224, 8200, False),
+    (1000, 96, 8200, False), (1, 96, 136, False), (1, 544, 136, False), (4, 4544, 136, False), (3, 36896, 72, False),
+    (16, 800, 200, False), (16, 18176, 136, False), (1, 90016, 40, False),
+]
+
+
+@pytest.mark.parametrize("M,K,N,x4", FORMS)
+def test_product_in_every_form(dev, M, K, N, x4):
+    g = torch.Generator().manual_seed(M + K + N)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    ws = torch.randint(117, 124, (N, K // 32), generator=g, dtype=torch.uint8)
+    x, op = _x(g, M, K, BF16), blocks.Fp4Matmul(quantize_x=x4)
+    rows, xs = oc.fp4_encode(x) if x4 else (x, None)
+    want, mag = oe.fp4_matmul(rows, w, ws, xs)
+    got = op.run(x.to(dev), w.to(dev), ws.to(dev))
+    assert_within(got, want, product_tolerance(want, mag, K, BF16), "product")
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 @pytest.mark.parametrize("x4", [False, True])
 def test_every_value_of_k_counts_once(dev, M, x4):

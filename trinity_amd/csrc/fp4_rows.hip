@@ -22,7 +22,7 @@ __device__ __forceinline__ uint32_t amax_bits8(half8v x) {
 template <bool READ, int U>
 __global__ __launch_bounds__(256) void fp4_rows_kernel(Fp4RowsArgs a) {
   const int pieces = a.K / 8, c0 = (int)blockIdx.x * 256 * U + (int)threadIdx.x;
-  for (int row = blockIdx.y; row < a.M; row += gridDim.y) {
+  for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
     half_t* const x = a.x + row * a.ldx;
     uint8_t* const codes = a.codes + row * a.ldc;
     uint8_t* const scales = a.scales + row * a.lds;

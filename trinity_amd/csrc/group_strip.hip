@@ -151,13 +151,8 @@ bool group_strip_takes(const GroupArgs& a) {
 
 template <GroupKind KIND>
 static int launch_strip_kind(const GroupArgs& a, hipStream_t stream) {
-#ifndef SNW
-#define SNW 4
-#define SNST 3
-#define SNW1 4
-#define SNST1 4
-#endif
-  constexpr int NW = KIND == kGroupGate ? SNW : SNW1, NST = KIND == kGroupGate ? SNST : SNST1, NM = KIND == kGroupGate ? 2 : 1;
+  // (48 and 32 KB of LDS a workgroup: three and five of them a CU have about 96 KB of weights on their way)
+  constexpr int NW = 4, NST = KIND == kGroupGate ? 3 : 4, NM = KIND == kGroupGate ? 2 : 1;
   constexpr int LDS = NW * NST * NM * kGsCols * kGsPieceBytes;
   constexpr auto kern = group_strip_kernel<KIND, NW, NST>;
   if (set_max_lds<kern, LDS>() != 0) return -1;
