@@ -20,7 +20,8 @@ static int parts_of(int tiles, int K, int slots) {
 //   16-bit weights, 32 rows each 555, 501, 574, 499; 42 of 32 experts of [4544, 2272] -, 401, -, 435; 64 818, 669, 588, 507; 150 1395,
 //     1116, 740, 591; 500 3800, 2710, 1990, 1540
 //   4-bit weights, 32 rows 228, 281, 371, 312; 64 373, 387, 384, 361; 100 479, 459, 404, 383; 150 681, 705, 611, 499; 250 1067, 1010,
-//     859, 935; 500 2043, 1963, 1511, 1615
+//     859, 935; 500 2043, 1963, 1511, 1615.  Around 200 rows it hangs on how the experts' numbers of rows fall: 192 of 64 experts of
+//     [4096, 1792] -, -, 791, 676; 200 of 8 -, -, 653, 720 (fastest runs 631, 615); 225 of 32 of [4544, 2272] 576, 576; 240 of 8 957, 941
 GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w4) {
   GroupPlan p;
   const int mean = (choices + experts - 1) / experts, groups = choices < experts ? choices : experts;
@@ -30,7 +31,7 @@ GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w
     p.ksplit = group_stream_parts(rows, F, N, groups);
     return p;
   }
-  p.bm = w4 ? (mean <= 48 ? 32 : (mean <= 180 ? 256 : 128)) : (mean <= 48 ? 64 : 256);
+  p.bm = w4 ? (mean <= 48 ? 32 : (mean <= 208 ? 256 : 128)) : (mean <= 48 ? 64 : 256);
   const int tiles = ((mean + p.bm - 1) / p.bm) * groups * ((N + tile_cols(p.bm) - 1) / tile_cols(p.bm));
   p.ksplit = parts_of(tiles, F, tile_slots(p.bm));
   return p;
