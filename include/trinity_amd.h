@@ -53,8 +53,8 @@ extern "C" {
  * signatures, a different noise stream for a given seed.
  * 7: tri_diag_issue_probe added; nothing else changed.
  * 8: tri_diag_power_probe added; nothing else changed.
- * (The tri_cache_*, tri_fp4_*, tri_route and tri_experts_* entry points came later: nothing that was there changed for them, and a caller finds them by their
- * symbols.) */
+ * (The tri_cache_*, tri_fp4_*, tri_route and tri_experts_* entry points came later: nothing that was there changed for
+ * them, and a caller finds them by their symbols.) */
 #define TRI_ABI_VERSION 8
 
 typedef enum tri_dtype {
@@ -357,8 +357,8 @@ int tri_validate_cache_attention(const tri_tensor* q, const tri_tensor* k_cache,
  * 4-bit matrices are two byte tensors, in the format of the 4-bit caches above with blocks along rows: codes TRI_U8
  * [rows, K / 2] (two codes a byte, the even column in the low half; rows 16-byte aligned) and scales TRI_U8 [rows, K / 32]
  * (any alignment and row stride).  Weights of a product are [N, K], a row for each output column - torch.nn.Linear's layout;
- * of experts [E, N, K], their strides free.  K is a multiple of 32 (at most 2^22), N of 8.  A matrix (of one expert) and the rows that experts
- * read each span less than 4 GB, rows are less than 16 MB apart.
+ * of experts [E, N, K], their strides free.  K is a multiple of 32 (at most 2^22), N of 8.  A matrix (of one expert) and the rows
+ * that experts read each span less than 4 GB, rows are less than 16 MB apart.
  * The element type of a product has to hold its weights' values (fp16: from 2^-24 to 65504; beyond, they count as
  * zeros and infinities); a block whose scale is 255 is NaN.  Sums are in fp32, results are rounded once. */
 
@@ -405,8 +405,8 @@ int tri_validate_route(const tri_tensor* logits, const tri_tensor* bias, const t
  *   x, out [T, N]; ids, weights [T, top_k] as tri_route leaves them (an expert may occur twice; ids outside [0, E) count nothing);
  *   gate, up [E, F, N], down [E, N, F]: of x's type, or 4-bit (codes and scales of all three).  N and F multiples of 32, E and
  *   top_k at most 512 and 64.  16-bit weights: rows 16-byte aligned.
- * The hidden rows are rounded to x's type, the experts' outputs are summed in fp32, in the order of the choices.  workspace: 1-D TRI_U8, 256-byte
- * aligned, tri_experts_workspace_bytes or more, this call's own until it has run. */
+ * The hidden rows are rounded to x's type, the experts' outputs are summed in fp32, in the order of the choices.  workspace: 1-D
+ * TRI_U8, 256-byte aligned, tri_experts_workspace_bytes or more, this call's own until it has run. */
 int64_t tri_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts, int64_t n, int64_t f);
 int tri_experts_ffn(const tri_tensor* x, const tri_tensor* ids, const tri_tensor* weights, const tri_tensor* gate,
                     const tri_tensor* gate_scales /* nullable */, const tri_tensor* up, const tri_tensor* up_scales /* nullable */,

@@ -272,6 +272,45 @@ def test_routed_ffn_plan(dev, T, w4):
     assert_within(got, out, off * 1.05 + UNIT[F16] * (out.abs() + off) + 2.0 ** -25, "routed FFN")
 
 
+@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("w4", [False, True])
+def test_routed_ffn_plan_captured(dev, T, w4):
+    g = torch.Generator().manual_seed(T)
+    E, k, N, F = 16, 4, 544, 576
+    stored, _ = _weights(g, E, F, N, BF16, w4, 0)
+    d = [(to_dev(a, dev), to_dev(b, dev)) for a, b in stored]
+    wr = (0.1 * torch.randn(N, E, generator=g)).bfloat16().to(dev)
+    plan = blocks.RoutedFfnPlan(k, groups=4, top_groups=2, prenorm=True, eps=1e-5)
+    x = torch.zeros(T, N, dtype=BF16, device=dev)
+    step = lambda x: plan.run(x, wr, d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
+    step(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x)
+    for i in range(4):
+        new = torch.randn(T, N, generator=g).bfloat16().to(dev)
+        x.copy_(new)
+        graph.replay()
+        eager = step(new)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+
+
+def test_a_few_choices_of_one_expert_more_often_than_tokens(dev):
+    """More rows of an expert than tokens, more than a launch for few rows holds at a time."""
+    g = torch.Generator().manual_seed(6)
+    for T, E, k, N, F in ((1, 2, 40, 512, 544), (3, 3, 64, 544, 512), (2, 100, 64, 512, 544)):
+        ids = torch.randint(0, 2, (T, k), generator=g).int()
+        for w4 in (False, True):
+            stored, values = _weights(g, E, F, N, F16, w4, 0)
+            x, weights = torch.randn(T, N, generator=g).half(), torch.randn(T, k, generator=g)
+            out, off = oe.experts_ffn(x, ids, weights, *values, unit=UNIT[F16], sums=sums)
+            d = [(to_dev(a, dev), to_dev(b, dev)) for a, b in stored]
+            got = blocks.ExpertsFfn().run(x.to(dev), ids.to(dev), weights.to(dev), d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
+            assert_within(got, out, off * 1.01 + UNIT[F16] * (out.abs() + off) + 2.0 ** -25, "experts")
+
+
 def test_empty(dev):
     g = torch.Generator().manual_seed(1)
     w = [s[0].to(dev) for s in _weights(g, 4, 64, 96, F16, False, 0)[0]]

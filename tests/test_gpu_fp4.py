@@ -157,6 +157,33 @@ def test_values_that_are_no_numbers_stay_in_their_row_and_column(dev, M, x4):
         assert bool(torch.isinf(got[2][keep]).all())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_every_code_at_every_scale(dev, dtype):
+    """What the element type cannot hold counts as the type has it: subnormals, zeros, infinities; 255 is NaN."""
+    codes = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(1, 256).repeat(256, 1)      # both halves of a byte
+    scales = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(256, 1).repeat(1, 16)
+    want = oc.fp4_decode(codes, scales).to(dtype)
+    got = blocks.Fp4Matmul.dequantize(codes.to(dev), scales.to(dev), dtype).cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M", [1, 16, 40, 300])
+@pytest.mark.parametrize("x4", [False, True])
+def test_products_at_every_scale(dev, dtype, M, x4):
+    """One value of K at a time against weights of every scale whose values the type holds as normal numbers."""
+    lo, hi = (127 - 13, 127 + 13) if dtype == F16 else (127 - 100, 127 + 100)
+    N, K = hi - lo + 1 + (-(hi - lo + 1)) % 8, 512
+    g = torch.Generator().manual_seed(M)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    scales = (lo + torch.arange(N) % (hi - lo + 1)).to(torch.uint8).view(N, 1).repeat(1, K // 32)
+    x = torch.zeros(M, K, dtype=dtype)
+    at = torch.randint(0, K, (M,), generator=g)
+    x[torch.arange(M), at] = 1
+    got = blocks.Fp4Matmul(quantize_x=x4).run(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    assert torch.equal(got, oc.fp4_decode(codes, scales)[:, at].t().to(dtype))
+
+
 def test_empty(dev):
     w, ws = four_bit(torch.Generator().manual_seed(1), 16, 64)
     op = blocks.Fp4Matmul()

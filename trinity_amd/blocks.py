@@ -363,7 +363,8 @@ class ExpertsFfn:
 
 class RoutedFfnPlan:
     """The FFN half of a layer with experts: [RMSNorm,] the router's product, routing, and the experts' FFN: X [T, N], W_router
-    [N, E], and what `Router` and `ExpertsFfn` take.  A call's buffers come from the allocator."""
+    [N, E] (E a multiple of 8, as the product wants it), and what `Router` and `ExpertsFfn` take.  A call's buffers come from the
+    allocator."""
 
     def __init__(self, top_k, scores="softmax", groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0, prenorm=False,
                  eps=0.0):

@@ -3,7 +3,8 @@
 // through an LDS ring of its own, and add up through LDS at the end.
 //
 // What bounds them: streaming the weights once.  Weights go global -> LDS without passing through registers; the rows' fragments
-// come straight from the cache, which they stay in.
+// come straight from the cache, which they stay in.  One token through two experts of [4096, 14336]: 470 MB of gate and up in 69
+// to 72 us, 235 MB of down in 37, 6.4 to 6.8 TB/s.
 //
 // The experts' rows are found without a launch that sorts them: the workgroups of choice s look for its expert among all
 // choices (at most 64: one load, one ballot) and work only if s is the first to have it.

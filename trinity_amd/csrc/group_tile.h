@@ -18,6 +18,15 @@
 //
 // One barrier per k tile, in front of the last of its four steps, when the next tile must have landed; that step then requests
 // the tile that takes its place.
+//
+// What bounds them and what they take:
+//   kMul16   4096 tokens x 2 of 8 experts of [4096, 14336], 256 x 256 tiles, fp16: gate and up 1.68 to 1.87 ms, down 1.16 to 1.24, 1.03
+//            and 0.83 PFLOP/s: the power limit (a library product of 8192 cubed 1.16).  333 tokens x 4 of 32 experts of [4544, 2272], 64 x
+//            128 tiles: 250 + 152 us, the weights' bytes at 4.9 TB/s
+//   kMul164  333 rows x [4544, 18176], 128 x 128 tiles: 68 us, 0.81 PFLOP/s, conversions between MFMAs; 256 x 256 tiles, eight waves:
+//            2048 tokens x 6 of 64 experts of [4096, 1792] 417 + 232 us
+//   kMul44   4096 rows x [4096, 14336], 256 x 256 tiles: 153 to 160 us, 3.1 PFLOP/s; [14336, 4096] 125, 3.8.  A k tile takes 2.6 us, its
+//            MFMAs 0.9: 64 KB a CU from the L2 with room for two k tiles (four of half a line each: 177 and 145 us)
 #if (defined(TRI_BF16) && !defined(TRI_GROUP_TILE_H_BF16)) || (!defined(TRI_BF16) && !defined(TRI_GROUP_TILE_H_F16))
 #ifdef TRI_BF16
 #define TRI_GROUP_TILE_H_BF16

@@ -8,7 +8,8 @@
 // apart are common among millions of them.  The arithmetic is small all the same (4096 x 256 exponentials: the matrix would take
 // as long to read as they to compute).
 //
-// A token has LPT lanes of a wave, each with EPL experts next to each other.
+// A token has LPT lanes of a wave, each with EPL experts next to each other.  What bounds it is the chain of top_k searches, each a
+// reduction over the lanes: 4096 tokens x 256 experts in 8 groups, 8 chosen, 12.6 us (21 with exchanges through LDS).
 #include "common.h"
 #include "launch.h"
 
@@ -220,7 +221,8 @@ int launch_route(const RouteArgs& a, hipStream_t stream) {
 // ---------------------------------------------------------------------------
 // The rows of every expert next to each other: places (row of a token's choice, token * top_k + i) in ascending order for each
 // expert, and the row tiles of `bm` that the experts' products take.  One workgroup: a wave counts and places a contiguous
-// sixteenth of the choices, 64 at a time, so that the order does not depend on timing.
+// sixteenth of the choices, 64 at a time, so that the order does not depend on timing.  Bound by trips to memory and LDS in a row:
+// 5 us, 8192 choices of 8 experts 7 to 10, 12288 of 64 14.
 // ---------------------------------------------------------------------------
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 
@@ -313,7 +315,8 @@ int launch_expert_rows(const ExpertRowsArgs& a, hipStream_t stream) {
 
 // out[t] = sum of w[t, i] * y[t * k + i] over the choices i that are experts, in 32 bits, y being the sum of its parts; or
 // (no weights, k = 1) that sum itself.
-// Bound by the bytes of y.  Rows of four choices (or parts) are on their way at a time.
+// Bound by the bytes of y, of which rows of four choices (or eight parts) are on their way at a time: 4096 tokens x 2 x 4096 in 43 us,
+// 2048 x 6 x 4096 in 46, 4.7 TB/s.
 template <bool PARTS>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinRowsArgs a) {
   const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
