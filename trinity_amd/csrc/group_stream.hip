@@ -1,11 +1,12 @@
 // Products of up to 16 rows (of a group) over 4-bit weights: weights go from memory to registers, 16 bytes - a block - per lane,
-// a segment of 512 values of K ahead, and meet rows that wait in LDS.
+// a segment of 512 values of K (or two) ahead, and meet rows that wait in LDS.
 //
 // What bounds them: streaming the weights once, 4.25 bits a value.  At that width the rows are what costs: a wave that reads them
 // from the cache beside its weights moves four bytes of each row pair for every byte of weights (16 rows x [4096, 14336]: 43 us),
 // so a workgroup fetches its part of K of all rows once and takes several column tiles over it: 14 us; one row 25 -> 10.5, [14336,
-// 4096] 10.2, 16 rows 16.7; 32 tokens over 8 experts of [4096, 14336 x 2] 99 us, 5.0 TB/s.  (More segments ahead cost registers and
-// give nothing: 11.3 us for one row with two, 11.6 with three.)
+// 4096] 10.2, 16 rows 16.7; 32 tokens over 8 experts of [4096, 14336 x 2] 99 us, 5.0 TB/s.  (Two segments ahead
+// cost registers and give nothing elsewhere - one row 10.6 -> 11.8 us, gate and up 101 -> 120 -, but 2 to 10 % in the down projection,
+// whose parts of K are short: 64 experts of [1792, 4096] 104 -> 94.)
 //
 // A workgroup has eight waves, `kw` of which share a tile of 16 columns (of gate and of up: 16 each) and take a part of K each -
 // short sums are then spread over many waves, and they add up through LDS - and runs `tpw` tiles with every such set.  A 16x16x32
@@ -24,17 +25,16 @@ template <GroupKind KIND, int RB>
 __global__ __launch_bounds__(kStreamWaves * 64, 2) void group_stream_kernel(GroupArgs a) {
   extern __shared__ __attribute__((aligned(16))) half_t lds[];
   constexpr bool GATE = KIND == kGroupGate, ALL = KIND == kGroupRows || KIND == kGroupParts;
-  constexpr int NM = GATE ? 2 : 1, NST = 2;
+  constexpr int NM = GATE ? 2 : 1, NST = KIND == kGroupDown ? 3 : 2;  // (segments in registers, one of them in use)
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int kw = a.kw, cw = kStreamWaves / kw;  // ways of K, column tiles side by side
   const int way = wave % kw, col_way = wave / kw;
 
-  // ---- which columns, part of K, group: neighbouring columns on one XCD, every group's on all of them
-  const int blocks8 = a.col_blocks / 8;  // (a multiple of eight)
+  // ---- which columns, part of K, group (column blocks are padded to a multiple of eight: every group's go to all XCDs)
   int id = blockIdx.x;
-  const int cb8 = id % a.col_blocks, cb = (cb8 & 7) * blocks8 + (cb8 >> 3);
+  const int cb = id % a.col_blocks;
   id /= a.col_blocks;
   const int part = id % a.ksplit, group = id / a.ksplit;
   const int tiles = (a.N + 15) / 16, tile0 = cb * cw * a.tpw;
@@ -257,9 +257,10 @@ static StreamPlan stream_plan(int rows, int K, int N, int groups, bool gate, boo
   while (p.kw < kStreamWaves && bytes + sums <= room && (waves * p.kw < 256 * kStreamWaves || p.kw < 2) && p.kw * 2 <= per) p.kw *= 2;
   p.lds = list + (p.kw > 1 ? sums : 0) + bytes;
   const int cw = kStreamWaves / p.kw, most = (tiles + cw - 1) / cw;
-  const int64_t sets = (int64_t)groups * p.ksplit * most;
-  p.tpw = (int)((sets + 255) / 256);
-  if (p.tpw > most) p.tpw = most;
+  // a workgroup a CU, and eight of a group at least, which go to the XCDs in turn: with a workgroup a CU alone, four of each of 64 experts
+  // ran on four XCDs (64 tokens x 6 of 64 experts of [4096, 1792]: 166 + 96 -> 106 + 61 us; of 128 experts 593 + 336 -> 204 + 115)
+  const int units = groups * p.ksplit, share = (255 + units) / units, blocks = share > 8 ? share : 8;
+  p.tpw = (most + blocks - 1) / blocks;
   p.col_blocks = ((most + p.tpw - 1) / p.tpw + 7) / 8 * 8;
   return p;
 }
