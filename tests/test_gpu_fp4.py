@@ -117,6 +117,19 @@ def test_product_in_every_form(dev, M, K, N, x4):
     assert_within(got, want, product_tolerance(want, mag, K, BF16), "product")
 
 
+@pytest.mark.parametrize("M,K", [(1, 81600), (1, 81664), (1, 90016), (3, 90016), (16, 90016), (16, 18176), (17, 90016)])
+def test_long_rows_without_a_workspace(dev, M, K):
+    """Rows of which the LDS holds none, or one as a whole."""
+    N, g = 40, torch.Generator().manual_seed(K)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    ws = torch.randint(117, 124, (N, K // 32), generator=g, dtype=torch.uint8)
+    x, out = _x(g, M, K, BF16), torch.zeros(M, N, dtype=BF16, device=dev)
+    want, mag = oe.fp4_matmul(x, w, ws)
+    for room in (None, torch.empty(256, dtype=torch.uint8, device=dev)):
+        ext.fp4_matmul(x.to(dev), None, w.to(dev), ws.to(dev), room, out)
+        assert_within(out, want, product_tolerance(want, mag, K, BF16), "product")
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 @pytest.mark.parametrize("x4", [False, True])
 def test_every_value_of_k_counts_once(dev, M, x4):
