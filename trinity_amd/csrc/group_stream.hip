@@ -288,6 +288,8 @@ static int launch_stream_kind(GroupArgs a, const StreamPlan& p, int groups, hipS
   return p.room_rows == 4 ? launch_stream_rows<KIND, 4>(a, p, groups, stream) : launch_stream_rows<KIND, 16>(a, p, groups, stream);
 }
 
+// (by tiles of 32 rows instead, us, [4096, 14336], [14336, 4096], [4544, 4544]: one row 17.3, 17.6, 15.6 for 10.8, 10.4, 6.6; 16 rows 18.4,
+// 18.6, 16.2 for 14.0, 16.8, 10.8)
 bool group_stream_takes(int rows, int K, bool may_split) { return rows <= 16 && K >= kSegment && (may_split || stream_fits(rows, K)); }
 int group_stream_parts(int rows, int K, int N, int groups) { return stream_plan(rows, K, N, groups, false, true).ksplit; }
 
