@@ -1,0 +1,64 @@
+"""The calls of perf/more_operators.py, its listed cases and some thousand of the range that it draws from, against the entry points'
+own checks, on the CPU: none is refused.  (Descriptors without memory: checks read no elements.)"""
+import importlib.util
+import os
+import random
+
+import pytest
+import torch
+
+from trinity_amd import blocks, ext
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _cases():
+    spec = importlib.util.spec_from_file_location("more_operators", os.path.join(ROOT, "perf", "more_operators.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def _like(dtype, *shape, i32=False):
+    """A contiguous tensor's descriptor, at an address that nothing reads."""
+    s = ext.TriTensor()
+    s.ptr, s.ndim = 1 << 20, len(shape)
+    s.dtype = ext.TRI_I32 if i32 else ext._DTYPES[dtype]
+    step = 1
+    for i in reversed(range(len(shape))):
+        s.shape[i], s.stride[i] = shape[i], step
+        step *= shape[i]
+    return s
+
+
+def _status(mod, c):
+    u8, f32 = torch.uint8, torch.float32
+    dt = mod.DTYPES[c["dtype"]]
+    four = lambda *shape: (_like(u8, *shape[:-1], shape[-1] // 2), _like(u8, *shape[:-1], shape[-1] // 32))
+    if c["kind"] == "quantize":
+        x, q = _like(dt, c["rows"], c["k"]), four(c["rows"], c["k"])
+        return [ext.fp4_quantize(x, *q, validate_only=True), ext.fp4_dequantize(*q, x, validate_only=True)]
+    if c["kind"] == "product":
+        m, k, n = c["rows"], c["k"], c["n"]
+        x = four(m, k) if c["x4"] else (_like(dt, m, k), None)
+        need = ext.fp4_workspace_bytes(m, k, n, c["x4"])
+        return [ext.fp4_matmul(*x, *four(n, k), _like(u8, need) if need else None, _like(dt, m, n), validate_only=True)]
+    if c["kind"] == "route":
+        t, e, k = c["tokens"], c["experts"], c["top_k"]
+        op = blocks.Router(k, scores=c["scores"], groups=c["groups"], top_groups=c["top_groups"], group_top=c["group_top"],
+                           renormalize=c["renormalize"], scale=c["scale"])
+        return [ext.route(_like(dt, t, e), _like(f32, e) if c["bias"] else None, _like(None, t, k, i32=True), _like(f32, t, k), op._p,
+                          validate_only=True)]
+    e, k, n, f = mod.EXPERTS[c["config"]]
+    t = c["tokens"]
+    w = lambda rows, deep: four(e, rows, deep) if c["w4"] else (_like(dt, e, rows, deep), None)
+    need = ext.experts_workspace_bytes(t, k, e, n, f)
+    return [ext.experts_ffn(_like(dt, t, n), _like(None, t, k, i32=True), _like(f32, t, k), *w(f, n), *w(f, n), *w(n, f), _like(u8, need),
+                            _like(dt, t, n), validate_only=True)]
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_no_case_is_refused(seed):
+    mod, rng = _cases(), random.Random(seed)
+    for c in mod.listed() + [mod.draw(rng) for _ in range(3000)]:
+        assert not any(_status(mod, c)), c

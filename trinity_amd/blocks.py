@@ -326,11 +326,13 @@ class Router:
     """Experts of every token and their weights from a router's logits: scores are the softmax or sigmoid of the logits, experts
     are chosen by score + bias, `top_k` of them in descending order (ties: the lowest index), out of the `top_groups` best of
     `groups` groups of neighbours - a group counts its `group_top` (1 or 2) largest - and weighted with their scores, over the
-    sum of the chosen if `renormalize`, times `scale`."""
+    sum of the chosen if `renormalize`, times `scale`.  (One group stays whatever it counts: 1 and 2 are the same there.)"""
 
     def __init__(self, top_k, scores="softmax", groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0):
         if scores not in ("softmax", "sigmoid"):
             raise ValueError("scores must be softmax or sigmoid")
+        if groups == 1 and group_top == 2:
+            group_top = 1  # (the entry point has that as the one way to say it)
         self.top_k = top_k
         self._p = ext.route_params(top_k, sigmoid=scores == "sigmoid", groups=groups, top_groups=top_groups, group_top=group_top,
                                    renormalize=renormalize, scale=scale)
