@@ -385,7 +385,8 @@ int tri_validate_fp4_matmul(const tri_tensor* x, const tri_tensor* x_scales, con
  * order, ties to the lowest index; with groups > 1 (dividing E, at most 64) out of the top_groups best groups of E / groups
  * neighbours, a group counting the sum of its group_top (1 or 2) largest c.  weights = s of the chosen (without the bias), with
  * renormalize over their sum, times scale.  Computed in 64 bits.  A logit of -inf has s = 0; where no logit is above that, all
- * weights are 0; a NaN makes weights NaN, and ids still top_k different experts.
+ * weights are 0; a NaN among a token's logits, or in the bias, makes all its weights NaN, whichever experts are chosen (softmax: a
+ * logit of +inf, too), and ids still top_k different experts.
  *   ids TRI_I32 [T, top_k], weights TRI_F32 [T, top_k], contiguous. */
 typedef struct tri_route_params {
   int32_t top_k; /* 1 to 64, and at most the experts of the groups that stay */

@@ -1,4 +1,6 @@
 """GPU: calls of blocks.Router, Fp4Matmul and ExpertsFfn at the borders of what they take, against oracle/experts.py."""
+import math
+
 import pytest
 import torch
 
@@ -18,3 +20,28 @@ def test_what_a_group_counts_means_nothing_where_there_is_one(dev, T, E, k, scor
     want, w = oe.route(z, b, top_k=k, sigmoid=scores == "sigmoid", scale=2.5)
     assert torch.equal(ids.cpu().long(), want)
     assert_within(weights, w, 2.0 ** -24 * w.abs() * 1.01, "weights")
+
+
+@pytest.mark.parametrize("E,groups,top_groups", [(7, 1, 1), (12, 1, 1), (12, 3, 2), (30, 1, 1), (64, 1, 1), (64, 8, 1), (100, 1, 1),
+                                                 (256, 8, 2), (400, 1, 1)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_a_nan_makes_its_tokens_weights_nan(dev, E, groups, top_groups, sigmoid, renormalize):
+    """Of whichever expert it is - chosen, passed over or in a group that goes - and no other token's."""
+    g, k = torch.Generator().manual_seed(E), 3
+    z = torch.randn(45, E, generator=g)
+    bad = torch.arange(45) % 4 == 1
+    for i, t in enumerate(bad.nonzero().flatten().tolist()):
+        z[t, (0, E - 1, E // 2, int(z[t].argmin()), int(z[t].argmax()))[i % 5]] = math.nan
+    op = blocks.Router(k, scores="sigmoid" if sigmoid else "softmax", groups=groups, top_groups=top_groups, renormalize=renormalize)
+    ids, w = (t.cpu() for t in op.route(z.to(dev)))
+    assert torch.equal(w.isnan(), bad[:, None].expand(45, k))
+    assert bool((ids.sort(-1).values.diff(dim=-1) > 0).all()) and bool(((ids >= 0) & (ids < E)).all())
+    want, value = oe.route(z[~bad], top_k=k, sigmoid=sigmoid, groups=groups, top_groups=top_groups, renormalize=renormalize)
+    assert torch.equal(ids[~bad].long(), want)
+    assert_within(w[~bad], value, 2.0 ** -24 * value * 1.01, "weights")
+    bias = torch.zeros(E)
+    bias[E // 3] = math.nan  # (every token's)
+    ids, w = (t.cpu() for t in op.route(z.to(dev), bias.to(dev)))
+    assert bool(w.isnan().all())
+    assert bool((ids.sort(-1).values.diff(dim=-1) > 0).all()) and bool(((ids >= 0) & (ids < E)).all())

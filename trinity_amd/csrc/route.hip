@@ -123,6 +123,13 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a) {
   double c[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) c[j] = s[j] + (a.bias != nullptr && in[j] ? (double)a.bias[lane * EPL + j] : 0.0);
+  constexpr uint64_t kMine = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
+  const int first = (int)(threadIdx.x & 63) - lane;  // (of this token's lanes in the wave)
+  // a NaN of the token's makes all its weights NaN: an expert that has one is the last to be chosen, and would not be seen
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) nan = nan || c[j] != c[j];
+  nan = ((__ballot(nan) >> first) & kMine) != 0;
   if constexpr (LPT == 64) {
     if (a.groups > 1) {
       double* const mine = choice_s + slot * 64 * EPL;
@@ -160,8 +167,6 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a) {
   for (int j = 0; j < EPL; ++j) key[j] = in[j] ? order_key(c[j]) : 0;
   double sum = 0.0, my_w = 0.0;
   int my_id = 0;
-  constexpr uint64_t kMine = LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1;
-  const int first = (int)(threadIdx.x & 63) - lane;  // (of this token's lanes in the wave)
   for (int r = 0; r < a.k; ++r) {
     // this lane's best: largest key, lowest index
     uint64_t bk = key[0];
@@ -196,7 +201,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a) {
   if (live && lane < a.k) {  // (top_k is at most LPT)
     a.ids[token * a.k + lane] = my_id;
     const double w = !a.renormalize ? my_w : (sum == 0.0 ? 0.0 : my_w / sum);
-    a.weights[token * a.k + lane] = (float)(w * (double)a.scale);
+    a.weights[token * a.k + lane] = nan ? __builtin_nanf("") : (float)(w * (double)a.scale);
   }
 }
 
