@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from test_experts_plans import experts_plan
 from trinity_amd import blocks, ext
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -62,3 +63,13 @@ def test_no_case_is_refused(seed):
     mod, rng = _cases(), random.Random(seed)
     for c in mod.listed() + [mod.draw(rng) for _ in range(3000)]:
         assert not any(_status(mod, c)), c
+
+
+@pytest.mark.parametrize("E,k,N,F", [(8, 2, 4096, 14336), (64, 6, 4096, 1792), (32, 4, 4544, 2272), (5, 1, 512, 96)])
+def test_rows_of_tiles_go_by_whole_tiles(E, k, N, F):
+    """Beyond few rows the tile of 4-bit experts changes where one or one and a half of its largest are full, and nowhere else."""
+    for mean, bm in ((64, 256), (150, 256), (192, 256), (193, 256), (208, 256), (209, 256), (256, 256), (257, 128), (384, 128), (385, 256),
+                     (2000, 256)):
+        T = mean * E // k
+        if -(-T * k // E) == mean:  # (the plan's mean, rounded up)
+            assert experts_plan(T, k, E, N, F, True)[0] == bm, mean

@@ -4,11 +4,14 @@ import math
 import pytest
 import torch
 
-from cache_util import assert_within
+from cache_util import UNIT, assert_within
+from experts_util import sums, to_dev
 from oracle import experts as oe
+from test_gpu_experts import _ids, _weights
 from trinity_amd import blocks
 
 pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
 
 
 @pytest.mark.parametrize("T,E,k", [(1, 8, 2), (1, 1, 1), (70, 16, 4), (33, 128, 8), (40, 256, 8)])
@@ -45,3 +48,16 @@ def test_a_nan_makes_its_tokens_weights_nan(dev, E, groups, top_groups, sigmoid,
     ids, w = (t.cpu() for t in op.route(z.to(dev), bias.to(dev)))
     assert bool(w.isnan().all())
     assert bool((ids.sort(-1).values.diff(dim=-1) > 0).all()) and bool(((ids >= 0) & (ids < E)).all())
+
+
+@pytest.mark.parametrize("T,E,k,N,F,how", [(416, 2, 1, 96, 160, "spread"), (512, 2, 1, 96, 160, "spread"), (514, 2, 1, 96, 160, "spread"),
+                                           (384, 1, 1, 64, 544, "spread"), (385, 1, 1, 64, 544, "spread"), (770, 6, 3, 64, 96, "one")])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_four_bit_experts_where_their_tiles_change(dev, T, E, k, N, F, how, dtype):
+    g = torch.Generator().manual_seed(T)
+    x, weights, ids = torch.randn(T, N, generator=g).to(dtype), torch.randn(T, k, generator=g), _ids(g, T, E, k, how)
+    stored, values = _weights(g, E, F, N, dtype, True, 0)
+    out, off = oe.experts_ffn(x, ids, weights, *values, unit=UNIT[dtype], sums=sums)
+    d = [(to_dev(a, dev), to_dev(b, dev)) for a, b in stored]
+    got = blocks.ExpertsFfn().run(x.to(dev), ids.to(dev), weights.to(dev), d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
+    assert_within(got, out, off * 1.01 + UNIT[dtype] * (out.abs() + off) + 2.0 ** -25, "experts")

@@ -19,9 +19,13 @@ static int parts_of(int tiles, int K, int slots) {
 // Rows of a tile by the mean rows of an expert.  us of both products of 8 experts of [4096, 14336], by 32, 64, 128, 256 rows:
 //   16-bit weights, 32 rows each 555, 501, 574, 499; 42 of 32 experts of [4544, 2272] -, 401, -, 435; 64 818, 669, 588, 507; 150 1395,
 //     1116, 740, 591; 500 3800, 2710, 1990, 1540
-//   4-bit weights, 32 rows 228, 281, 371, 312; 64 373, 387, 384, 361; 100 479, 459, 404, 383; 150 681, 705, 611, 499; 250 1067, 1010,
-//     859, 935; 500 2043, 1963, 1511, 1615.  Around 200 rows it hangs on how the experts' numbers of rows fall: 192 of 64 experts of
-//     [4096, 1792] -, -, 791, 676; 200 of 8 -, -, 653, 720 (fastest runs 631, 615); 225 of 32 of [4544, 2272] 576, 576; 240 of 8 957, 941
+//   4-bit weights, 32 rows 228, 281, 371, 312; 64 373, 387, 384, 361; 100 479, 459, 404, 383
+// From there on 4-bit weights go by whole tiles: 256 rows while an expert has one of them, 128 where a second one would be half empty, and
+// 256 beyond.  Time of a call with 256 over that with 128 rows, of 8 experts of [4096, 14336], 64 of [4096, 1792], 32 of [4544, 2272], 16 of
+// [2048, 8192] and 128 of [2048, 1024] - their mean; without the last from 700 on, and the second at 2000 -, first with the same rows for
+// each, then as a router's random choices fall:
+//   150 0.83, 1.03; 190 0.84, 1.05; 225 0.98, 1.03; 256 0.98, 1.02; 270 1.07, 1.02; 350 1.08, 0.98; 400 0.90, 1.00; 700 0.92, 0.96;
+//   1000 0.90, 0.96; 2000 0.90, 0.93.  (One call of random choices is off from its neighbours by up to 20 % either way.)
 GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w4) {
   GroupPlan p;
   const int mean = (choices + experts - 1) / experts, groups = choices < experts ? choices : experts;
@@ -33,7 +37,7 @@ GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w
     p.ksplit = group_stream_parts(rows, F, N, groups);
     return p;
   }
-  p.bm = w4 ? (mean <= 48 ? 32 : (mean <= 208 ? 256 : 128)) : (mean <= 48 ? 64 : 256);
+  p.bm = w4 ? (mean <= 48 ? 32 : (mean <= 256 || mean > 384 ? 256 : 128)) : (mean <= 48 ? 64 : 256);
   const int tiles = ((mean + p.bm - 1) / p.bm) * groups * ((N + tile_cols(p.bm) - 1) / tile_cols(p.bm));
   p.ksplit = parts_of(tiles, F, tile_slots(p.bm));
   return p;
