@@ -73,3 +73,8 @@ def test_rows_of_tiles_go_by_whole_tiles(E, k, N, F):
         T = mean * E // k
         if -(-T * k // E) == mean:  # (the plan's mean, rounded up)
             assert experts_plan(T, k, E, N, F, True)[0] == bm, mean
+
+
+def test_few_rows_stream_as_far_as_lds_holds_them():
+    for T, wide in ((32, 4608), (5, 4608), (4, 19968), (1, 81408)):
+        assert experts_plan(T, 2, 8, wide, 2048, True)[0] == 16 and experts_plan(T, 2, 8, wide + 32, 2048, True)[0] == 32

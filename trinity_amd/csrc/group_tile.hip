@@ -32,6 +32,11 @@ GroupPlan experts_plan(int choices, int top_k, int experts, int N, int F, bool w
   const int rows = choices / top_k < 16 ? choices / top_k : 16;  // (of an expert, at most, if a token chooses it once)
   // (few rows stream past the weights at once: 8 each of 8 experts of [4096, 14336] 165 us, 183 by tiles of 32 rows; where an expert is
   // likely to have more than 16, twice: 9.4 each of 64 of [4096, 1792] 247, 193)
+  // Rows wider than LDS holds as many as an expert may have (16 of up to 4608 values, 4 of 19968, one of 81408) go by tiles: four rows at a
+  // time would have the experts of more than four stream their weights again.  That and tiles, us: 8, 16 and 32 tokens x 2 of 8 of [5120,
+  // 14336] 252 for 198, 279 for 214, 470 for 227; 8, 32 and 64 x 6 of 64 of [5120, 1792] 177 for 129, 297 for 224, 405 for 234; of
+  // [7168, 2048] 237 for 220, 413 for 301, 606 for 320; x 8 of 256 of [7168, 2048] 274 for 299, 673 for 704, 1026 for 1009 and,
+  // 128 tokens, 1589 for 1185.  (At [4096, 14336] 16 rows in LDS 145, 158 and 164 for 170, 176 and 178.)
   if (w4 && mean <= 8 && group_stream_takes(rows, N, false) && group_stream_takes(rows, F, true)) {
     p.bm = 16;
     p.ksplit = group_stream_parts(rows, F, N, groups);
