@@ -359,8 +359,10 @@ int tri_validate_cache_attention(const tri_tensor* q, const tri_tensor* k_cache,
  * (any alignment and row stride).  Weights of a product are [N, K], a row for each output column - torch.nn.Linear's layout;
  * of experts [E, N, K], their strides free.  K is a multiple of 32 (at most 2^22), N of 8.  A matrix (of one expert) and the rows
  * that experts read each span less than 4 GB, rows are less than 16 MB apart.
- * The element type of a product has to hold its weights' values (fp16: from 2^-24 to 65504; beyond, they count as
- * zeros and infinities); a block whose scale is 255 is NaN.  Sums are in fp32, results are rounded once. */
+ * Beside 16-bit rows weights pass through the product's element type, and count as that holds them: bf16 every value up to its
+ * largest, fp16 those of scales from 2^-23 (whose least is 2^-24, a subnormal) to 2^13 exactly, smaller ones rounded to
+ * multiples of 2^-24, and what is beyond 65504 as infinities.  A block whose scale is 255 is NaN.  Sums are in fp32, results are
+ * rounded once. */
 
 /* codes, scales of x [M, K] (fp16 or bf16), as tri_cache_append has them: e is the least exponent >= -110 with max |x| < 7 * 2^e
  * over the block, x / 2^e goes to the nearest magnitude, ties to the even code; a block that holds an infinity or NaN

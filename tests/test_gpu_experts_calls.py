@@ -6,6 +6,7 @@ import torch
 
 from cache_util import UNIT, assert_within
 from experts_util import sums, to_dev
+from oracle import cache as oc
 from oracle import experts as oe
 from test_gpu_experts import _ids, _weights
 from trinity_amd import blocks
@@ -61,3 +62,45 @@ def test_four_bit_experts_where_their_tiles_change(dev, T, E, k, N, F, how, dtyp
     d = [(to_dev(a, dev), to_dev(b, dev)) for a, b in stored]
     got = blocks.ExpertsFfn().run(x.to(dev), ids.to(dev), weights.to(dev), d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
     assert_within(got, out, off * 1.01 + UNIT[dtype] * (out.abs() + off) + 2.0 ** -25, "experts")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M", [1, 3, 16, 30, 40, 100, 300])
+@pytest.mark.parametrize("x4", [False, True])
+def test_products_of_weights_that_the_type_holds_as_subnormals(dev, dtype, M, x4):
+    """Every scale from that on whose values the type holds exactly (its least subnormal is half of 2^e): one value of K at a time, times
+    a power of two that makes the product a normal number, exactly."""
+    least, up = (-23, 10) if dtype == F16 else (-127, 20)
+    scale = torch.arange(least, least + 16)
+    N, K = 16, 512
+    g = torch.Generator().manual_seed(M)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    scales = (scale + 127).to(torch.uint8).view(N, 1).repeat(1, K // 32)
+    x = torch.zeros(M, K, dtype=dtype)
+    at = torch.randint(0, K, (M,), generator=g)
+    x[torch.arange(M), at] = 2.0 ** up
+    values = oc.fp4_decode(codes, scales)
+    assert torch.equal(values.to(dtype).double(), values) and bool((values.abs()[values != 0].min() < torch.finfo(dtype).smallest_normal))
+    want = (values[:, at].t() * 2.0 ** up).to(dtype)
+    assert torch.equal(want.double(), values[:, at].t() * 2.0 ** up)
+    got = blocks.Fp4Matmul(quantize_x=x4).run(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_experts_of_weights_that_the_type_holds_as_subnormals(dev, T):
+    """Both products over 4-bit weights of every scale down to the last that fp16 holds: x and the hidden rows are large enough
+    for results that count."""
+    g = torch.Generator().manual_seed(T)
+    E, k, N, F = 2, 1, 64, 96
+    w = lambda *s: (torch.randint(0, 256, s[:-1] + (s[-1] // 2,), generator=g, dtype=torch.uint8),
+                    (127 - 23 + torch.randint(0, 6, s[:-1] + (s[-1] // 32,), generator=g)).to(torch.uint8))
+    stored = [w(E, F, N), w(E, F, N), w(E, N, F)]
+    values = [oc.fp4_decode(*s) for s in stored]
+    x = (4096 * torch.randn(T, N, generator=g)).half()
+    ids, weights = _ids(g, T, E, k, "spread"), torch.full((T, k), 2.0 ** 14)
+    out, off = oe.experts_ffn(x, ids, weights, *values, unit=UNIT[F16], sums=sums)
+    assert float(out.abs().max()) > 100 * float(off.max())
+    d = [t.to(dev) for s in stored for t in s]
+    got = blocks.ExpertsFfn().run(x.to(dev), ids.to(dev), weights.to(dev), d[0], d[2], d[4], d[1], d[3], d[5])
+    assert_within(got, out, off * 1.01 + UNIT[F16] * (out.abs() + off) + 2.0 ** -25, "experts")
