@@ -3,6 +3,7 @@ own checks, on the CPU: none is refused.  (Descriptors without memory: checks re
 import importlib.util
 import os
 import random
+import re
 
 import pytest
 import torch
@@ -78,3 +79,14 @@ def test_rows_of_tiles_go_by_whole_tiles(E, k, N, F):
 def test_few_rows_stream_as_far_as_lds_holds_them():
     for T, wide in ((32, 4608), (5, 4608), (4, 19968), (1, 81408)):
         assert experts_plan(T, 2, 8, wide, 2048, True)[0] == 16 and experts_plan(T, 2, 8, wide + 32, 2048, True)[0] == 32
+
+
+def test_every_tile_that_is_compiled_is_one_that_a_plan_takes():
+    """The kernels that the library registers: products of all rows in all four tiles, of experts in those of experts_plan (which
+    test_experts_plans_keep_their_bounds holds to them)."""
+    with open(ext.LIB_PATH, "rb") as f:
+        names = set(re.findall(rb"_ZN3tri17group_tile_kernelINS_9GroupTileILi(\d+)E[^(]*?NS_8GroupMulE(\d)EEELNS_9GroupKindE(\d)E", f.read()))
+    got = {tuple(map(int, n)) for n in names}  # (rows of a tile; 16-bit, 4-bit weights, both in 4 bits; rows, parts, gate and up, down)
+    want = {(bm, mul, kind) for bm in (32, 64, 128, 256) for mul in (1, 2) for kind in (0, 1)}
+    want |= {(bm, 0, kind) for bm in (64, 256) for kind in (2, 3)} | {(bm, 1, kind) for bm in (32, 128, 256) for kind in (2, 3)}
+    assert got == want

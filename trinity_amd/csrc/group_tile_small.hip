@@ -8,12 +8,17 @@ template <GroupMul MUL, GroupKind KIND>
 static int launch_tile_kind(const GroupArgs& a, int bm, hipStream_t stream) {
   // (k tiles in LDS: as many as leave room for two workgroups a CU)
   constexpr int D = MUL == kMul164 ? 2 : 3;
+  constexpr bool EXPERTS = KIND == kGroupGate || KIND == kGroupDown;  // (experts_plan: 64 rows for 16-bit weights, 32 and 128 for 4-bit ones)
   switch (bm) {
     case 32:
-      if constexpr (MUL == kMul16) return -1;  // (experts_plan has none)
+      if constexpr (MUL == kMul16) return -1;
       else return launch_tile_t<GroupTile<32, 256, 1, 4, 3, D, MUL>, KIND>(a, stream);
-    case 64: return launch_tile_t<GroupTile<64, 128, 2, 2, 3, D, MUL>, KIND>(a, stream);
-    default: return launch_tile_t<GroupTile<128, 128, 2, 2, 2, 2, MUL>, KIND>(a, stream);
+    case 64:
+      if constexpr (EXPERTS && MUL == kMul164) return -1;
+      else return launch_tile_t<GroupTile<64, 128, 2, 2, 3, D, MUL>, KIND>(a, stream);
+    default:
+      if constexpr (MUL == kMul16) return -1;
+      else return launch_tile_t<GroupTile<128, 128, 2, 2, 2, 2, MUL>, KIND>(a, stream);
   }
 }
 
