@@ -9,7 +9,7 @@ from experts_util import sums, to_dev
 from oracle import cache as oc
 from oracle import experts as oe
 from test_gpu_experts import _ids, _weights
-from trinity_amd import blocks
+from trinity_amd import blocks, ext
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -104,3 +104,17 @@ def test_experts_of_weights_that_the_type_holds_as_subnormals(dev, T):
     d = [t.to(dev) for s in stored for t in s]
     got = blocks.ExpertsFfn().run(x.to(dev), ids.to(dev), weights.to(dev), d[0], d[2], d[4], d[1], d[3], d[5])
     assert_within(got, out, off * 1.01 + UNIT[F16] * (out.abs() + off) + 2.0 ** -25, "experts")
+
+
+@pytest.mark.parametrize("k", [65, 2 ** 31 - 1, 0, -1])
+def test_choices_that_are_refused_take_no_memory(dev, k):
+    z = torch.zeros(4096, 512, device=dev)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ext.TrinityError):
+        blocks.Router(k).route(z)
+    assert torch.cuda.max_memory_allocated() == before
+    with pytest.raises(ext.TrinityError):
+        blocks.Router(2).route(z.view(-1))
+    assert torch.cuda.max_memory_allocated() == before

@@ -616,7 +616,8 @@ PyObject* route_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const OneDevice device(a, 2);
     void* s = stream_of(a[3]);
     if (!device.ok || PyErr_Occurred() != nullptr) return nullptr;
-    const int64_t sizes[2] = {logits->dim() > 0 ? logits->size(0) : 0, p.p->top_k > 0 ? p.p->top_k : 0};
+    // (a number of choices that the call refuses, before it looks at its results, gets no memory)
+    const int64_t sizes[2] = {logits->dim() == 2 ? logits->size(0) : 0, p.p->top_k > 0 && p.p->top_k <= 64 ? p.p->top_k : 0};
     at::Tensor ids = new_tensor(*logits, sizes, at::kInt), weights = new_tensor(*logits, sizes, at::kFloat);
     tri_tensor i = describe(ids, TRI_I32), w = describe(weights, TRI_F32);
     const int st = call([&] { return tri_route(t.p[0], t.p[1], &i, &w, p.p, s); });
