@@ -90,3 +90,12 @@ def test_every_tile_that_is_compiled_is_one_that_a_plan_takes():
     want = {(bm, mul, kind) for bm in (32, 64, 128, 256) for mul in (1, 2) for kind in (0, 1)}
     want |= {(bm, 0, kind) for bm in (64, 256) for kind in (2, 3)} | {(bm, 1, kind) for bm in (32, 128, 256) for kind in (2, 3)}
     assert got == want
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    for name in ("top_k", "groups", "top_groups", "group_top"):
+        for n in (2 ** 32 + 1, -2 ** 32 + 1, 2 ** 31):
+            with pytest.raises(ValueError):
+                blocks.Router(**{"top_k": 1, name: n})
+    p = ext.route_params(3, sigmoid=True, groups=4, top_groups=2, group_top=2, renormalize=False, scale=0.5)
+    assert [getattr(p, f[0]) for f in p._fields_] == [3, 1, 4, 2, 2, 0, 0.5]

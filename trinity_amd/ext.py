@@ -430,8 +430,11 @@ def fp4_matmul(x, x_scales, w, w_scales, workspace, out, validate_only=False):
 
 def route_params(top_k, sigmoid=False, groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0):
     p = TriRouteParams()
-    p.top_k, p.sigmoid, p.groups, p.top_groups, p.group_top = top_k, int(bool(sigmoid)), groups, top_groups, group_top
-    p.renormalize, p.scale = int(bool(renormalize)), scale
+    for name, n in (("top_k", top_k), ("groups", groups), ("top_groups", top_groups), ("group_top", group_top)):
+        setattr(p, name, n)
+        if getattr(p, name) != n:  # (ctypes drops what does not fit)
+            raise ValueError("%s is beyond 32 bits" % name)
+    p.sigmoid, p.renormalize, p.scale = int(bool(sigmoid)), int(bool(renormalize)), scale
     return p
 
 
