@@ -118,3 +118,36 @@ def test_choices_that_are_refused_take_no_memory(dev, k):
     with pytest.raises(ext.TrinityError):
         blocks.Router(2).route(z.view(-1))
     assert torch.cuda.max_memory_allocated() == before
+
+
+@pytest.mark.parametrize("w4", [False, True])
+@pytest.mark.parametrize("prenorm", [False, True])
+def test_routed_ffn_plan_is_its_parts(dev, w4, prenorm):
+    """Logits in X's type, and an fp32 product in their place by the parts; no tokens; a result over its own input, or into strided rows."""
+    g = torch.Generator().manual_seed(12)
+    T, E, k, N, F = 90, 16, 3, 256, 288
+    stored, _ = _weights(g, E, F, N, BF16, w4, 0)
+    d = [to_dev(t, dev) for s in stored for t in s]
+    args = (d[0], d[2], d[4], d[1], d[3], d[5])
+    x, wr = torch.randn(T, N, generator=g).bfloat16().to(dev), (0.1 * torch.randn(N, E, generator=g)).bfloat16().to(dev)
+    plan = blocks.RoutedFfnPlan(k, prenorm=prenorm, eps=1e-5)
+    got = plan.run(x, wr, *args)
+    xn = x
+    if prenorm:
+        xn = torch.empty_like(x)
+        ext.rmsnorm(x, None, xn, 1e-5)
+    logits = torch.empty(T, E, dtype=BF16, device=dev)
+    ext.matmul(xn, wr, None, logits)
+    assert torch.equal(got, blocks.ExpertsFfn().run(xn, *blocks.Router(k).route(logits), *args))
+    exact = xn.cpu().double() @ wr.cpu().double()
+    ids, w = blocks.Router(k).route(exact.float().to(dev))  # (what a model with fp32 logits does)
+    want, value = oe.route(exact.float(), top_k=k)
+    assert torch.equal(ids.cpu().long(), want)
+    assert_within(w, value, 2.0 ** -24 * value * 1.01, "weights")
+    none = plan.run(x[:0], wr, *args)
+    assert none.shape == (0, N) and none.dtype == BF16
+    big = torch.full((T, N + 16), 3, dtype=BF16, device=dev)
+    assert plan.run(x, wr, *args, out=big[:, 8:N + 8]).data_ptr() == big[:, 8:].data_ptr()
+    assert torch.equal(big[:, 8:N + 8], got) and bool((big[:, :8] == 3).all()) and bool((big[:, N + 8:] == 3).all())
+    plan.run(x, wr, *args, out=x)
+    assert torch.equal(x, got)

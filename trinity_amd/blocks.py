@@ -366,7 +366,11 @@ class ExpertsFfn:
 class RoutedFfnPlan:
     """The FFN half of a layer with experts: [RMSNorm,] the router's product, routing, and the experts' FFN: X [T, N], W_router
     [N, E] (E a multiple of 8, as the product wants it), and what `Router` and `ExpertsFfn` take.  A call's buffers come from the
-    allocator."""
+    allocator.
+
+    The logits are a result of `ext.matmul`, in X's type as all its results are (summed in fp32): in bfloat16 equal logits are common
+    among many experts, and the lowest index wins.  A model that was trained to route on fp32 logits computes those itself and
+    calls `Router` and `ExpertsFfn`, which is all that happens here."""
 
     def __init__(self, top_k, scores="softmax", groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0, prenorm=False,
                  eps=0.0):
