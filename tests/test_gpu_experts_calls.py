@@ -123,7 +123,7 @@ def test_choices_that_are_refused_take_no_memory(dev, k):
 @pytest.mark.parametrize("w4", [False, True])
 @pytest.mark.parametrize("prenorm", [False, True])
 def test_routed_ffn_plan_is_its_parts(dev, w4, prenorm):
-    """Logits in X's type, and an fp32 product in their place by the parts; no tokens; a result over its own input, or into strided rows."""
+    """Logits in X's type, and an fp32 product in their place by the parts; no tokens; strided rows."""
     g = torch.Generator().manual_seed(12)
     T, E, k, N, F = 90, 16, 3, 256, 288
     stored, _ = _weights(g, E, F, N, BF16, w4, 0)
@@ -149,5 +149,3 @@ def test_routed_ffn_plan_is_its_parts(dev, w4, prenorm):
     big = torch.full((T, N + 16), 3, dtype=BF16, device=dev)
     assert plan.run(x, wr, *args, out=big[:, 8:N + 8]).data_ptr() == big[:, 8:].data_ptr()
     assert torch.equal(big[:, 8:N + 8], got) and bool((big[:, :8] == 3).all()) and bool((big[:, N + 8:] == 3).all())
-    plan.run(x, wr, *args, out=x)
-    assert torch.equal(x, got)

@@ -25,8 +25,11 @@
 //            128 tiles: 250 + 152 us, the weights' bytes at 4.9 TB/s
 //   kMul164  333 rows x [4544, 18176], 128 x 128 tiles: 68 us, 0.81 PFLOP/s, conversions between MFMAs; 256 x 256 tiles, eight waves:
 //            2048 tokens x 6 of 64 experts of [4096, 1792] 417 + 232 us
-//   kMul44   4096 rows x [4096, 14336], 256 x 256 tiles: 153 to 160 us, 3.1 PFLOP/s; [14336, 4096] 125, 3.8.  A k tile takes 2.6 us, its
-//            MFMAs 0.9: 64 KB a CU from the L2 with room for two k tiles (four of half a line each: 177 and 145 us)
+//   kMul44   4096 rows x [4096, 14336], 256 x 256 tiles: 153 to 160 us, 3.1 PFLOP/s; [14336, 4096] 125, 3.8.  MFMAs are busy 37 % of that
+//            time (a k tile takes 2.5 us, they 1.0).  Not the L2's rate: 64 KB a CU and k tile are 13 bytes a clock, a read's
+//            latency 340 clocks.  A k tile's loads are asked for in the step before it begins and waited for three steps later,
+//            and a SIMD has one wave: a quarter of the waves' time waits for loads and barriers, a third for an instruction to issue.
+//            LDS has room for two k tiles (four of half a line each: 177 and 145 us)
 #if (defined(TRI_BF16) && !defined(TRI_GROUP_TILE_H_BF16)) || (!defined(TRI_BF16) && !defined(TRI_GROUP_TILE_H_F16))
 #ifdef TRI_BF16
 #define TRI_GROUP_TILE_H_BF16

@@ -8,8 +8,10 @@
 // apart are common among millions of them.  The arithmetic is small all the same (4096 x 256 exponentials: the matrix would take
 // as long to read as they to compute).
 //
-// A token has LPT lanes of a wave, each with EPL experts next to each other.  What bounds it is the chain of top_k searches, each a
-// reduction over the lanes: 4096 tokens x 256 experts in 8 groups, 8 chosen, 12.6 us (21 with exchanges through LDS).
+// A token has LPT lanes of a wave, each with EPL experts next to each other.  What bounds it is a chain of trips in a row: top_k searches, each a
+// reduction over the lanes by operand exchanges (21 us with exchanges through LDS) and three reads of the winner's values through
+// LDS, and before them, where there are groups, a lane's loop over the E / groups scores of its group in LDS.  4096 tokens x 256 experts in
+// 8 groups, 8 chosen: 12.6 us, where a launch takes 2.2.
 #include "common.h"
 #include "launch.h"
 
