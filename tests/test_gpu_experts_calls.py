@@ -1,5 +1,6 @@
 """GPU: calls of blocks.Router, Fp4Matmul and ExpertsFfn at the borders of what they take, against oracle/experts.py."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -149,3 +150,64 @@ def test_routed_ffn_plan_is_its_parts(dev, w4, prenorm):
     big = torch.full((T, N + 16), 3, dtype=BF16, device=dev)
     assert plan.run(x, wr, *args, out=big[:, 8:N + 8]).data_ptr() == big[:, 8:].data_ptr()
     assert torch.equal(big[:, 8:N + 8], got) and bool((big[:, :8] == 3).all()) and bool((big[:, N + 8:] == 3).all())
+
+
+def _inside(t, left, right, fill):
+    """The same values as columns of wider rows, between bytes that no call may read as its own."""
+    rows = t.reshape(-1, t.shape[-1])
+    wide = torch.full((rows.shape[0], left + t.shape[-1] + right), fill, dtype=t.dtype)
+    wide[:, left:left + t.shape[-1]] = rows
+    return wide.view(*t.shape[:-1], -1)[..., left:left + t.shape[-1]]
+
+
+@pytest.mark.parametrize("M", [1, 4, 16, 30, 40, 100, 300])
+@pytest.mark.parametrize("x4", [False, True])
+def test_products_over_matrices_inside_larger_ones(dev, M, x4):
+    """Weights, rows and scales whose rows are parts of wider ones, up to the last byte before what is not theirs (255: codes of -6, NaN)."""
+    K, N = 1120, 72
+    g = torch.Generator().manual_seed(M)
+    w, ws = oc.fp4_encode(torch.randn(N, K, generator=g))
+    x = torch.randn(M, K, generator=g).bfloat16()
+    if x4:
+        rows, xs = oc.fp4_encode(x)
+        a = to_dev(_inside(rows, 16, 32, 255), dev), to_dev(_inside(xs, 3, 2, 255), dev)
+        b = rows.to(dev), xs.to(dev)
+    else:
+        a, b = (to_dev(_inside(x, 8, 16, math.nan), dev), None), (x.to(dev), None)
+    op = blocks.Fp4Matmul()
+    want = op.run(b[0], w.to(dev), ws.to(dev), x_scales=b[1], dtype=BF16)
+    got = op.run(a[0], to_dev(_inside(w, 32, 16, 255), dev), to_dev(_inside(ws, 5, 1, 255), dev), x_scales=a[1], dtype=BF16)
+    assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T", [1, 6, 90, 600])
+@pytest.mark.parametrize("w4", [False, True])
+def test_experts_over_matrices_inside_larger_ones(dev, T, w4):
+    E, k, N, F = 5, 2, 544, 288
+    g = torch.Generator().manual_seed(T)
+    x, ids, weights = torch.randn(T, N, generator=g).bfloat16(), _ids(g, T, E, k, "few"), torch.rand(T, k, generator=g)
+    stored, _ = _weights(g, E, F, N, BF16, w4, 0)
+    plain = [(t.to(dev), None if s is None else s.to(dev)) for t, s in stored]
+    inside = [(to_dev(_inside(t, 16, 32, 255 if w4 else math.nan), dev), to_dev(None if s is None else _inside(s, 3, 4, 255), dev)) for t, s in stored]
+    op = blocks.ExpertsFfn()
+    call = lambda x, d: op.run(x, ids.to(dev), weights.to(dev), d[0][0], d[1][0], d[2][0], d[0][1], d[1][1], d[2][1])
+    want = call(x.to(dev), plain)
+    assert bool(torch.isfinite(want).all())
+    assert torch.equal(call(to_dev(_inside(x, 8, 24, math.nan), dev), inside), want)
+
+
+@pytest.mark.parametrize("w4", [False, True])
+def test_threads_share_objects_and_a_stream(dev, w4):
+    E, k, N, F = 8, 2, 544, 1056
+    g = torch.Generator().manual_seed(3)
+    stored, _ = _weights(g, E, F, N, F16, w4, 0)
+    d = [t.to(dev) if t is not None else None for s in stored for t in s]
+    router, op = blocks.Router(k), blocks.ExpertsFfn()
+    calls = [(torch.randn(T, N, generator=g).half().to(dev), torch.randn(T, E, generator=g).to(dev)) for T in (1, 20, 100, 700)]
+    step = lambda x, z: op.run(x, *router.route(z), d[0], d[2], d[4], d[1], d[3], d[5])
+    want = [step(*c) for c in calls]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as threads:
+        got = list(threads.map(lambda i: (i % 4, step(*calls[i % 4])), range(80)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
